@@ -96,6 +96,39 @@ typedef struct molten_attn_args {
   int batch;                     /* stacked independent problems (0 or 1: one) */
 } molten_attn_args;
 
+/* Parameter block of the rotary-embedding kernels at given positions
+ * (device side: molten::RopePosArgs in molten/rope_positions.cuh). */
+typedef struct molten_rope_pos_args {
+  const void* x;                 /* [tokens, heads, dim], strides below, dim contiguous */
+  const void* cos_t;             /* [table_rows, dim/2], or packed [table_rows, dim] */
+  const void* sin_t;
+  const int* pos;                /* [axes, tokens]; negative: padding */
+  void* out;                     /* [tokens, heads, dim] contiguous */
+  int* status;
+  long long tokens, x_token, x_head, table_rows;
+  int heads, dim, axes, head_lanes;
+  int bound[4];                  /* first pair after each section */
+  int tokens_per_cta, reserved;
+} molten_rope_pos_args;
+
+/* Parameter block of the 4-bit matrix-vector kernels
+ * (device side: molten::Q4Args in molten/q4_matvec.cuh). */
+typedef struct molten_q4_args {
+  const void* x;                 /* [m, k], rows x_stride elements apart */
+  const uint8_t* q;              /* [n, k/2], the even k in the low nibble */
+  const void* scales;            /* [n, k/G] */
+  const void* zeros;             /* [n, k/G] or null */
+  void* out;                     /* [m, n] */
+  long long x_stride, n;
+  int m, k;
+  int warps_n_log;               /* log2 of the warps along the rows of q */
+  int ksplit_log;                /* log2 of the CTAs of the cluster, along k */
+  int chunk;                     /* groups of k staged at once */
+  int tiles;                     /* row tiles of 16 * warps_n */
+  int teams;                     /* CTAs (clusters) that share the tiles */
+  int reserved;
+} molten_q4_args;
+
 /* Version of this ABI (major * 100 + minor). */
 int molten_version(void);
 

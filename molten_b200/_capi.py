@@ -78,6 +78,29 @@ class AttnArgs(ctypes.Structure):
                 ("batch", ctypes.c_int), ("tail_", ctypes.c_ubyte * 12)]
 
 
+class RopePosArgs(ctypes.Structure):
+    """molten_rope_pos_args / molten::RopePosArgs."""
+    _fields_ = [("x", ctypes.c_void_p), ("cos_t", ctypes.c_void_p), ("sin_t", ctypes.c_void_p),
+                ("pos", ctypes.c_void_p), ("out", ctypes.c_void_p), ("status", ctypes.c_void_p),
+                ("tokens", ctypes.c_longlong), ("x_token", ctypes.c_longlong),
+                ("x_head", ctypes.c_longlong), ("table_rows", ctypes.c_longlong),
+                ("heads", ctypes.c_int), ("dim", ctypes.c_int), ("axes", ctypes.c_int),
+                ("head_lanes", ctypes.c_int), ("bound", ctypes.c_int * 4),
+                ("tokens_per_cta", ctypes.c_int), ("reserved", ctypes.c_int)]
+
+
+class Q4Args(ctypes.Structure):
+    """molten_q4_args / molten::Q4Args."""
+    _fields_ = [("x", ctypes.c_void_p), ("q", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("zeros", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("x_stride", ctypes.c_longlong), ("n", ctypes.c_longlong), ("m", ctypes.c_int),
+                ("k", ctypes.c_int), ("warps_n_log", ctypes.c_int), ("ksplit_log", ctypes.c_int),
+                ("chunk", ctypes.c_int), ("tiles", ctypes.c_int),
+                ("teams", ctypes.c_int), ("reserved", ctypes.c_int)]
+
+
+assert ctypes.sizeof(RopePosArgs) == 120
+assert ctypes.sizeof(Q4Args) == 88
 assert ctypes.sizeof(RowArgs) == 160
 assert ctypes.sizeof(AttnArgs) == 448
 assert ctypes.sizeof(GemmArgs) == 448

@@ -28,7 +28,7 @@ from pathlib import Path
 
 from . import __version__
 from .compiler import ZeroCompiler
-from .ir import DataflowGraph, OpType, TensorShape
+from .ir import DataflowGraph, ModelOpType, OpType, TensorShape
 
 _ATTR_KEYS = ("eps", "value", "min", "max", "period", "offset", "kind", "dim")
 
@@ -40,10 +40,13 @@ def graph_from_json(data: dict) -> DataflowGraph:
     order).  OUTPUT ops are registered as graph outputs."""
     g = DataflowGraph(data.get("name", "unnamed"))
     for pos, spec in enumerate(data.get("ops", [])):
-        try:
-            op_type = OpType[spec["type"]]
-        except KeyError as exc:
-            raise ValueError(f"op {pos}: unknown op type {spec.get('type')!r}") from exc
+        kind = spec.get("type")
+        if kind in OpType.__members__:
+            op_type = OpType[kind]
+        elif kind in ModelOpType.__members__:
+            op_type = ModelOpType[kind]
+        else:
+            raise ValueError(f"op {pos}: unknown op type {kind!r}")
         inputs = [int(i) for i in spec.get("inputs", [])]
         for i in inputs:
             if not 0 <= i < pos:

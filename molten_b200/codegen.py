@@ -107,6 +107,9 @@ def launch_records(plan: GroupPlan, name: str) -> list:
             zp = c.get("zpersist", 0)
             rec.update(block=c["threads"], zero_tiles_per_row=c["zt"], zero_tile_cols=c["zcols"],
                        zero_ctas=zp, grid=sk.rows + (zp if zp else sk.rows * c["zt"]), smem=0)
+        elif sk.family == "model":
+            from .decode import launch_record
+            rec.update(launch_record(sk))
         elif sk.family == "attn":
             rec.update(block=c["threads"], bm=128, bn=c["bn"], stages=c["stages"],
                        smem=c["smem_bytes"], tma_store=c["tma_store"],
@@ -144,6 +147,9 @@ def estimate(plan: GroupPlan):
             n *= d
         nbytes += n * DTYPE_SIZE[dt]
     for sk in plan.kernels:
+        if sk.family == "model":
+            flops += sk.config["flops"]
+            continue
         if sk.family == "gemm":
             flops += 2 * sk.m * sk.n * sk.k
         elif sk.family == "attn":
@@ -222,6 +228,11 @@ class CodeGenerator:
                 chunks.append(emit_causal(sk, entry))
                 smem = max(smem, 4)
                 block_x = sk.config["threads"]
+            elif sk.family == "model":
+                from .decode import emit_model_op
+                chunks.append(emit_model_op(sk, entry))
+                block_x = sk.config["block"]
+                smem = max(smem, sk.config.get("smem", 0))
             elif sk.family == "attn":
                 chunks.append(emit_attn(sk, entry))
                 block_x, block_y = sk.config["threads"], 1
@@ -254,6 +265,8 @@ class CodeGenerator:
         from .lowering import group_boundary
         ext, _, _ = group_boundary(graph, group.op_ids)
         declared = declared_graph_shapes(graph)
+        from .decode import fixed_input_dtypes
+        fixed = fixed_input_dtypes(graph)
         shapes, dtypes = {}, {}
         for i in ext:
             op = graph.ops[i]
@@ -265,7 +278,8 @@ class CodeGenerator:
                 shapes[i] = declared[i]
             else:
                 raise LoweringError(f"cannot infer the shape of op {i} ({op.op_type.name})")
-            dtypes[i] = input_dtypes[i] if input_dtypes and i in input_dtypes else self.io_dtype
+            dtypes[i] = input_dtypes[i] if input_dtypes and i in input_dtypes \
+                else fixed.get(i, self.io_dtype)
         return shapes, dtypes
 
 

@@ -1,0 +1,320 @@
+"""The operators of a decode step: shapes, launch plans and CUDA emission.
+
+``ModelOpType`` (``ir.py``) adds to the graph what answering a batch of
+requests needs next to RMSNorm, RoPE and the GEMM:
+
+* ``MATVEC_Q4``         products of a few rows with 4-bit weights;
+* ``ROTATE_POSITIONS``  RoPE at given positions, on up to four axes;
+* ``WINDOW_ATTENTION``  attention over a sliding window and the first keys;
+* ``SAMPLE``            temperature, top-k, top-p and min-p from given numbers.
+
+Each runs as a sub-kernel of family ``model`` (``lowering.split_group``).
+Unlike the row, elementwise and GEMM families, their sources are
+instantiations of the engine headers with types and head sizes only: batch
+sizes, lengths and strides travel in the parameter block, so every shape runs
+from the same few cubins and inputs may be strided views.
+``decode_launch.py`` fills the parameter blocks.
+"""
+
+from __future__ import annotations
+
+from .ir import DataflowGraph, ModelOpType, OpType
+from .lowering import (
+    DTYPE_CTYPE, DTYPE_SIZE, INT_DTYPES, LoweringError, Operand, OutputSpec, ROPE_STYLES,
+    SubKernel, prod,
+)
+
+SMS = 148                         # streaming multiprocessors of a B200
+
+Q4_GROUPS = (32, 64, 128)
+Q4_MAX_ROWS = 32
+Q4_MAX_KSPLIT = 8                 # portable cluster size
+Q4_SUMS_BYTES = 16 * 1024         # sums of a CTA's tiles, where they are kept
+SMEM_LIMIT = 227 * 1024           # shared memory of a CTA, and of an SM
+SMEM_SM = 228 * 1024
+
+ROPE_MAX_AXES = 4
+ROPE_MAX_DIM = 1024
+
+
+def _need(ok, text: str) -> None:
+    if not ok:
+        raise LoweringError(text)
+
+
+# ------------------------------------------------------------------- shapes
+def infer_shape(op, ins: list) -> tuple:
+    """Result shape of a model operator; raises on shapes it does not take."""
+    ins = [tuple(int(d) for d in s) for s in ins]
+    return _SHAPES[op.op_type](op, ins)
+
+
+def _q4_shape(op, ins):
+    _need(len(ins) in (3, 4), "matvec_q4 takes (x, qweight, scales[, zeros])")
+    x, q, s = ins[:3]
+    _need(len(x) >= 1 and len(q) == 2 and len(s) == 2,
+          f"matvec_q4 needs x [..., K], qweight [N, K/2], scales [N, K/G]: {x}, {q}, {s}")
+    k, n = x[-1], q[0]
+    _need(k > 0 and q[1] * 2 == k, f"matvec_q4: qweight {q} does not pack K = {k} nibbles a row")
+    _need(s[0] == n and s[1] > 0 and k % s[1] == 0 and k // s[1] in Q4_GROUPS,
+          f"matvec_q4: scales {s} for [{n}, {k}] weights; groups of {Q4_GROUPS}")
+    _need(len(ins) == 3 or ins[3] == s, f"matvec_q4: zeros {ins[-1]} and scales {s} differ in shape")
+    return x[:-1] + (n,)
+
+
+def _rope_shape(op, ins):
+    packed = bool(op.attrs.get("packed"))
+    _need(len(ins) == (3 if packed else 4), "rope with positions takes (x, tables, positions)")
+    x, pos = ins[0], ins[-1]
+    _need(len(x) >= 3, f"rope needs x of rank >= 3 ([..., seq, heads, head_dim]), got {x}")
+    d, lead = x[-1], x[:-2]
+    _need(d % 2 == 0 and 0 < d <= ROPE_MAX_DIM,
+          f"rope needs an even head_dim of at most {ROPE_MAX_DIM}, got {d}")
+    _need((op.attrs.get("style") or "interleaved") in ROPE_STYLES,
+          f"rope style {op.attrs.get('style')!r} (interleaved, half)")
+    width = d if packed else d // 2
+    for t in ins[1:-1]:
+        _need(len(t) == 2 and t[0] > 0 and t[1] == width and t == ins[1],
+              f"rope table of shape {t}; expected [rows, {width}]")
+    sections = op.attrs.get("sections") or [d // 2]
+    _need(1 <= len(sections) <= ROPE_MAX_AXES and all(v >= 0 for v in sections)
+          and sum(sections) == d // 2,
+          f"rope sections {sections} must be at most {ROPE_MAX_AXES} counts of pairs with sum {d // 2}")
+    want = (len(sections),) + lead
+    _need(pos == want or (len(sections) == 1 and pos == lead),
+          f"rope positions of shape {pos}; expected {want}")
+    return x
+
+
+_SHAPES = {ModelOpType.MATVEC_Q4: _q4_shape, ModelOpType.ROTATE_POSITIONS: _rope_shape}
+
+
+# -------------------------------------------------------------------- types
+def _slot_dtypes(op) -> dict:
+    """Operand position -> the dtype it has to have."""
+    t = op.op_type
+    if t == ModelOpType.MATVEC_Q4:
+        return {1: "uint8"}
+    if t == ModelOpType.ROTATE_POSITIONS:
+        return {len(op.inputs) - 1: "int32"}
+    if t == ModelOpType.WINDOW_ATTENTION:
+        return {3: "int32"} if len(op.inputs) > 3 else {}
+    slots = {1: "float32"}
+    for i, p in enumerate(op.attrs.get("params", ())):
+        slots[2 + i] = "int32" if p == "top_k" else "float32"
+    return slots
+
+
+def fixed_input_dtypes(graph: DataflowGraph) -> dict:
+    """Graph inputs whose dtype an operator fixes (positions, lengths, packed
+    weights, random numbers ...), and the tables and scales, which keep the
+    dtype they are declared with."""
+    out = {}
+    for op in graph.ops.values():
+        if not isinstance(op.op_type, ModelOpType):
+            continue
+        slots = dict(_slot_dtypes(op))
+        if op.op_type == ModelOpType.MATVEC_Q4:
+            declared = range(2, len(op.inputs))
+        elif op.op_type == ModelOpType.ROTATE_POSITIONS:
+            declared = range(1, len(op.inputs) - 1)
+        else:
+            declared = ()
+        for i, src in enumerate(op.inputs):
+            if graph.ops[src].op_type != OpType.INPUT:
+                continue
+            if i in slots:
+                out[src] = slots[i]
+            elif i in declared:
+                out[src] = graph.ops[src].dtype
+    return out
+
+
+# ------------------------------------------------------------------ planning
+def plan_model_op(graph, op_id: int, outs, shapes: dict, dts: dict, tune: dict) -> SubKernel:
+    """SubKernel of one model operator for concrete shapes and dtypes.  Its
+    ``config`` holds ``op`` (the operator), ``block``, ``flops`` and what the
+    launch needs; scalar operands are in ``config["scalars"]``."""
+    op = graph.ops[op_id]
+    _need(list(outs) == [op_id], f"the {op.op_type.name} sub-kernel has one output")
+    slots = _slot_dtypes(op)
+    operands, scalars = [], {}
+    for pos, j in enumerate(op.inputs):
+        src = graph.ops[j]
+        if src.op_type == OpType.CONSTANT:
+            _need(op.op_type == ModelOpType.SAMPLE and pos >= 2
+                  and isinstance(src.attrs.get("value"), (int, float)),
+                  f"{op.op_type.name}: operand {pos} must be a tensor")
+            scalars[pos] = src.attrs["value"]
+            continue
+        want = slots.get(pos)
+        if want:
+            _need(dts[j] == want, f"{op.op_type.name}: operand {src.name or pos!r} is {dts[j]}, "
+                                  f"expected {want}")
+        else:
+            _need(dts[j] not in INT_DTYPES,
+                  f"{op.op_type.name}: operand {src.name or pos!r} is {dts[j]}, expected a float type")
+        operands.append(Operand(index=pos, op_id=j, name=src.name or f"op{j}", dtype=dts[j],
+                                shape=tuple(shapes[j]), last="vec", row_map="full"))
+    outputs = [OutputSpec(index=0, op_id=op_id, dtype=dts[op_id], shape=tuple(shapes[op_id]),
+                          kind="full")]
+    sk = SubKernel(family="model", op_ids=[op_id], operands=operands, outputs=outputs)
+    sk.config = {"op": op.op_type, "scalars": scalars}
+    sk.config.update(_PLANS[op.op_type](op, sk, tune or {}))
+    return sk
+
+
+def _plan_q4(op, sk, tune) -> dict:
+    x, q, s = sk.operands[:3]
+    k, n = x.shape[-1], q.shape[0]
+    m = prod(x.shape[:-1])
+    _need(m <= Q4_MAX_ROWS, f"matvec_q4 takes at most {Q4_MAX_ROWS} rows of x, got {m}")
+    _need(k < 2 ** 31 and n < 2 ** 31 - 512, "matvec_q4: sizes beyond 2^31")
+    if len(sk.operands) == 4:
+        _need(sk.operands[3].dtype == s.dtype, "matvec_q4: zeros and scales must have one dtype")
+    group = k // s.shape[1]
+    nt = 1 if m <= 8 else (2 if m <= 16 else 4)
+    o = tune.get("q4") or {}
+    groups, w = s.shape[1], group // 32
+    planes = 3 if x.dtype == "float32" else 1
+    # up to 8 rows: small CTAs, several to an SM, one tile's latency behind
+    # another's; more rows: an SM's warps share one staged x
+    warps = int(o.get("warps") or (8 if nt == 1 else 16))
+    few = n <= 16 * 2 * SMS                           # one tile for each of two CTAs an SM
+    # the warps of a CTA split k, as far as there are groups for them
+    warps_n = int(o.get("warps_n") or (1 if few else 2))
+    while "warps_n" not in o and warps_n < warps and warps // warps_n > groups:
+        warps_n *= 2
+    tiles = -(-n // (16 * warps_n))
+    warps_k = warps // warps_n
+    # few row tiles: a cluster per tile splits k until every SM has a CTA, as
+    # long as each warp keeps a group
+    ksplit = 1
+    while ksplit < Q4_MAX_KSPLIT and tiles * ksplit < SMS and groups >= 2 * ksplit * warps_k:
+        ksplit *= 2
+    ksplit = int(o.get("ksplit") or ksplit)
+    occupancy = int(o.get("occupancy") or (1 if warps > 8 else 2 if few else 3))
+    limit = (SMEM_SM // occupancy - 1024) // 1024 * 1024
+    per_cta = -(-groups // ksplit)                    # groups of one CTA
+    group_bytes = m * (planes * 64 * w + 8)
+    fixed = 16 + 2 * warps * nt * 128 * 4
+    sums = warps_n * 16 * m * 4                       # of one tile
+    if warps == 8 and fixed + per_cta * group_bytes > limit and "occupancy" not in o:
+        occupancy, limit = 2, SMEM_SM // 2 - 1024
+    # x is staged whole where it fits, else in the fewest equal chunks
+    chunk, chunks = per_cta, 1
+    if fixed + per_cta * group_bytes + (Q4_SUMS_BYTES if ksplit > 1 else 0) > limit:
+        room = limit - Q4_SUMS_BYTES - fixed
+        _need(room >= group_bytes, f"matvec_q4: {m} rows of K = {k} do not fit")
+        chunks = -(-per_cta // (room // group_bytes))
+        chunk = -(-per_cta // chunks)
+    keep = chunks > 1 or ksplit > 1                   # tiles' sums stay in shared memory
+    teams = max(1, min(tiles, SMS * occupancy // ksplit))
+    if keep:
+        teams = max(teams, -(-tiles // max(1, Q4_SUMS_BYTES // sums)))
+    tiles_per_cta = -(-tiles // teams)
+    smem = fixed + chunk * group_bytes + (tiles_per_cta * sums if keep else 0)
+    _need(smem <= SMEM_LIMIT, f"matvec_q4: {m} rows of K = {k} do not fit")
+    depth = int(o.get("depth") or 2)
+    return {"m": m, "n": n, "k": k, "group": group, "nt": nt, "warps": warps, "warps_n": warps_n,
+            "tiles": tiles, "ksplit": ksplit, "depth": depth, "zeros": len(sk.operands) == 4,
+            "chunk": chunk, "min_ctas": occupancy, "teams": teams,
+            "tiles_per_cta": tiles_per_cta, "smem": smem, "block": 32 * warps,
+            "flops": 2 * m * n * k}
+
+
+def _plan_rope(op, sk, tune) -> dict:
+    packed = bool(op.attrs.get("packed"))
+    style = op.attrs.get("style") or "interleaved"
+    x, pos, out = sk.operands[0], sk.operands[-1], sk.outputs[0]
+    tables = sk.operands[1:-1]
+    _need(packed or tables[0].dtype == tables[1].dtype, "rope: cos and sin must have one dtype")
+    d, heads = x.shape[-1], x.shape[-2]
+    tokens = prod(x.shape[:-2])
+    _need(tokens < 2 ** 31 and heads < 2 ** 31, "rope: sizes beyond 2^31")
+    sections = op.attrs.get("sections") or [d // 2]
+    half = style == "half"
+    span = d // 2 if half else d
+    o = tune.get("rope") or {}
+    vec = 16 // min(DTYPE_SIZE[x.dtype], DTYPE_SIZE[out.dtype])
+    while vec > 1 and span % vec:
+        vec //= 2
+    if not half:
+        vec = max(vec, 2)
+    xvec = o.get("vec") != 1 and not (vec == 1 or vec * DTYPE_SIZE[x.dtype] < 4)
+    pairs = vec if half else vec // 2
+    slot = pairs * (2 if packed else 1) * DTYPE_SIZE[tables[0].dtype]      # table bytes per slot
+    row = tables[0].shape[1] * DTYPE_SIZE[tables[0].dtype]
+    tvec = xvec and row % min(16, slot) == 0 and slot in (2, 4, 8, 16, 32, 64)
+    spr = (d // 2) // pairs
+    # heads per thread (measured, 1 / 2 / 4 / 8: bf16 half-style [2, 4700, 22,
+    # 128] 21.0 / 16.9 / 23.0 / 29.4 us, [48, 1, 40, 128] 2.6 / 2.1 / 3.2, fp32
+    # interleaved [2, 4096, 32, 128] 46.0 / 43.7 / 42.0 / 42.3)
+    hpt = int(o.get("heads") or min(heads, 2))
+    lanes = max(1, min(-(-heads // hpt), 256 // spr if spr <= 256 else 1))
+    per_cta = max(1, 256 // (spr * lanes))
+    return {"dim": d, "heads": heads, "tokens": tokens, "sections": list(sections), "vec": vec,
+            "xvec": xvec, "tvec": tvec, "half": half, "packed": packed, "hpt": hpt,
+            "head_lanes": lanes, "tokens_per_cta": per_cta, "block": spr * lanes * per_cta,
+            "table_rows": tables[0].shape[0], "table_slot": min(16, slot),
+            "flops": 3 * tokens * heads * d}
+
+
+_PLANS = {ModelOpType.MATVEC_Q4: _plan_q4, ModelOpType.ROTATE_POSITIONS: _plan_rope}
+
+
+def launch_record(sk: SubKernel) -> dict:
+    c = sk.config
+    rec = {"op": c["op"].name.lower(), "block": c["block"], "smem": c.get("smem", 0)}
+    if c["op"] == ModelOpType.MATVEC_Q4:
+        rec.update(grid=c["teams"] * c["ksplit"], cluster=c["ksplit"], warps_n=c["warps_n"])
+    elif c["op"] == ModelOpType.ROTATE_POSITIONS:
+        rec.update(head_lanes=c["head_lanes"], tokens_per_cta=c["tokens_per_cta"])
+    return rec
+
+
+# ------------------------------------------------------------------ emission
+def emit_model_op(sk: SubKernel, name: str) -> str:
+    return _EMIT[sk.config["op"]](sk, name)
+
+
+def _bool(v) -> str:
+    return "true" if v else "false"
+
+
+def _emit_q4(sk, name):
+    c = sk.config
+    xt, st = (DTYPE_CTYPE[sk.operands[i].dtype] for i in (0, 2))
+    ot = DTYPE_CTYPE[sk.outputs[0].dtype]
+    return f"""// Molten sm_100a 4-bit matrix-vector product: {name}
+// x {sk.operands[0].dtype}, groups of {c['group']}, up to {8 * c['nt']} rows
+#include "molten/q4_matvec.cuh"
+
+using namespace molten;
+
+extern "C" __global__ void __launch_bounds__({c['block']}, {c['min_ctas']}) {name}(const __grid_constant__ Q4Args args) {{
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  pdl_enter();
+  q4_matvec<{xt}, {st}, {ot}, {c['group']}, {c['nt']}, {_bool(c['zeros'])}, {c['depth']}, {c['warps']}>(args, smem_raw);
+}}
+"""
+
+
+def _emit_rope(sk, name):
+    c = sk.config
+    xt, tt = (DTYPE_CTYPE[sk.operands[i].dtype] for i in (0, 1))
+    ot = DTYPE_CTYPE[sk.outputs[0].dtype]
+    return f"""// Molten sm_100a RoPE at given positions: {name}
+// x {sk.operands[0].dtype}, {'packed table' if c['packed'] else 'tables'} {sk.operands[1].dtype}
+#include "molten/rope_positions.cuh"
+
+using namespace molten;
+
+extern "C" __global__ void __launch_bounds__(1024) {name}(const __grid_constant__ RopePosArgs args) {{
+  pdl_enter();
+  rope_positions<{xt}, {tt}, {ot}, {c['vec']}, {_bool(c['half'])}, {_bool(c['packed'])}, {_bool(c['xvec'])}, {_bool(c['tvec'])}, {c['hpt']}>(args);
+}}
+"""
+
+
+_EMIT = {ModelOpType.MATVEC_Q4: _emit_q4, ModelOpType.ROTATE_POSITIONS: _emit_rope}

@@ -134,3 +134,78 @@ def rmsnorm_gemm(m=8192, k=4096, n=14336, dtype="bfloat16", eps=1e-6) -> Dataflo
 
 
 BUILDERS["rmsnorm_gemm"] = rmsnorm_gemm
+
+
+def matvec_q4(m=1, n=4096, k=4096, group=128, dtype="bfloat16", zeros=False,
+              scale_dtype=None) -> DataflowGraph:
+    """m rows of x times 4-bit weights [n, k] with a scale (and a zero point)
+    per group of k."""
+    g = DataflowGraph("matvec_q4")
+    sdt = scale_dtype or dtype
+    x = g.add_input("x", TensorShape([m, k]), dtype=dtype)
+    q = g.add_input("qweight", TensorShape([n, k // 2]), dtype="uint8")
+    s = g.add_input("scales", TensorShape([n, k // group]), dtype=sdt)
+    z = g.add_input("zeros", TensorShape([n, k // group]), dtype=sdt) if zeros else None
+    g.add_output(g.matvec_q4(x, q, s, zeros=z, name="matvec"))
+    return g
+
+
+BUILDERS["matvec_q4"] = matvec_q4
+
+
+def rope_positions(batch=1, seq=4096, heads=32, head_dim=128, table=8192, sections=None,
+                   dtype="bfloat16", table_dtype="float32", style="half",
+                   packed=False) -> DataflowGraph:
+    """RoPE of x [batch, seq, heads, head_dim] at given positions
+    [axes, batch, seq]; ``sections`` counts the pairs of each axis."""
+    g = DataflowGraph("rope_positions")
+    x = g.add_input("x", TensorShape([batch, seq, heads, head_dim]), dtype=dtype)
+    width = head_dim if packed else head_dim // 2
+    c = g.add_input("freqs" if packed else "cos", TensorShape([table, width]), dtype=table_dtype)
+    s = None if packed else g.add_input("sin", TensorShape([table, width]), dtype=table_dtype)
+    axes = len(sections) if sections else 1
+    p = g.add_input("positions", TensorShape([axes, batch, seq]), dtype="int32")
+    g.add_output(g.rope(x, c, "rope", sin=s, style=style, positions=p, sections=sections))
+    return g
+
+
+BUILDERS["rope_positions"] = rope_positions
+
+
+def window_attention(batch=1, new=1, cache=4096, heads=32, kv_heads=8, head_dim=128, window=1024,
+                     sinks=4, scale=None, dtype="bfloat16", lengths=True) -> DataflowGraph:
+    """Attention of ``new`` tokens over a cache, limited to a window and the
+    first ``sinks`` keys."""
+    g = DataflowGraph("window_attention")
+    q = g.add_input("q", TensorShape([batch, new, heads, head_dim]), dtype=dtype)
+    k = g.add_input("k", TensorShape([batch, cache, kv_heads, head_dim]), dtype=dtype)
+    v = g.add_input("v", TensorShape([batch, cache, kv_heads, head_dim]), dtype=dtype)
+    n = g.add_input("lengths", TensorShape([batch]), dtype="int32") if lengths else None
+    g.add_output(g.window_attention(q, k, v, lengths=n, window=window, sinks=sinks, scale=scale,
+                                    name="attention"))
+    return g
+
+
+BUILDERS["window_attention"] = window_attention
+
+
+def sample(rows=1, vocab=32768, dtype="float32", temperature=True, top_k=False, top_p=False,
+           min_p=False) -> DataflowGraph:
+    """One token per row of logits.  Each parameter is True (a vector input),
+    False (not used) or a number (for every row)."""
+    g = DataflowGraph("sample")
+    x = g.add_input("logits", TensorShape([rows, vocab]), dtype=dtype)
+    u = g.add_input("u", TensorShape([rows]), dtype="float32")
+    given = {}
+    for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p),
+                    ("min_p", min_p)):
+        if v is True:
+            given[name] = g.add_input(name, TensorShape([rows]),
+                                      dtype="int32" if name == "top_k" else "float32")
+        elif v is not False and v is not None:
+            given[name] = g.add_constant(name, v)
+    g.add_output(g.sample(x, u, name="tokens", **given))
+    return g
+
+
+BUILDERS["sample"] = sample

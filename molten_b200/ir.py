@@ -13,6 +13,10 @@ helpers so that reference callers are unaffected:
 * ``causal_mask(period, offset)`` adds a CONSTANT whose value is generated
   from indices: 0 where ``col <= (row mod period) + offset``, ``-inf`` above.
 * small builders for the remaining unary ops (``gelu``, ``silu`` ...).
+* ``ModelOpType``: the operators of a decode step (4-bit products, rotary
+  positions on several axes, window attention, sampling), which the reference
+  does not have.  They are an enum of their own because the members of
+  ``OpType`` and their values are the reference's interface.
 """
 
 from __future__ import annotations
@@ -64,6 +68,14 @@ class OpType(Enum):
     INPUT = auto()
     OUTPUT = auto()
     CONSTANT = auto()
+
+
+class ModelOpType(Enum):
+    """Operators beyond the reference's (``molten_b200/decode.py``)."""
+    MATVEC_Q4 = auto()
+    ROTATE_POSITIONS = auto()
+    WINDOW_ATTENTION = auto()
+    SAMPLE = auto()
 
 
 ELEMENTWISE_OPS = frozenset({
@@ -178,7 +190,8 @@ class DataflowGraph:
         return self.mul(div_id, weight, f"{name}_scale")
 
     def rope(self, x: int, freqs: int, name: str = "", sin: Optional[int] = None,
-             style: Optional[str] = None) -> int:
+             style: Optional[str] = None, positions: Optional[int] = None,
+             sections: Optional[list] = None) -> int:
         """ROTATE: rotary position embedding of x [..., seq, heads, head_dim].
 
         ``rope(x, freqs)`` is the reference's builder (``ir.py:175-176``);
@@ -187,10 +200,76 @@ class DataflowGraph:
         ``sin`` given, ``freqs`` is the cos table and both are
         [seq, head_dim/2] -- the form of ``benchmarks/ops.py:24-35``.
         ``style``: "interleaved" pairs (2i, 2i+1) as in ops.py (default) or
-        "half" pairs (i, i + head_dim/2).  The result has x's dtype."""
+        "half" pairs (i, i + head_dim/2).  The result has x's dtype.
+
+        ``positions`` (int32, [axes, ..., seq], or [..., seq] for one axis)
+        gives every token's row of the table instead of its own index; the
+        tables may then have any number of rows.  With several axes (time,
+        height, width ...) ``sections`` counts the pairs each axis turns, in
+        order (they sum to head_dim/2; at most 4).  A negative position marks
+        padding, whose pairs are left as they are; a position past the table
+        sets a bit of the status word and leaves them too."""
         inputs = [x, freqs] + ([sin] if sin is not None else [])
         attrs = {"style": style} if style else {}
+        if positions is not None:
+            attrs["sections"] = [int(v) for v in sections] if sections is not None else None
+            attrs["packed"] = sin is None
+            return self.add_op(ModelOpType.ROTATE_POSITIONS, inputs + [positions], name, **attrs)
+        if sections is not None:
+            raise ValueError("rope: sections need positions")
         return self.add_op(OpType.ROTATE, inputs, name, **attrs)
+
+    def matvec_q4(self, x: int, qweight: int, scales: int, zeros: Optional[int] = None,
+                  name: str = "") -> int:
+        """x [..., K] times 4-bit weights: y[..., n] = sum_k x[..., k]
+        (q[n, k] - zeros[n, k // G]) * scales[n, k // G].
+
+        ``qweight`` is uint8 [N, K/2], the even k in the low nibble;
+        ``scales`` and ``zeros`` are [N, K/G] floats with G = 32, 64 or 128;
+        without ``zeros`` the zero point is 8.  At most 32 rows of x; the
+        result has x's dtype."""
+        return self.add_op(ModelOpType.MATVEC_Q4,
+                           [x, qweight, scales] + ([zeros] if zeros is not None else []), name)
+
+    def window_attention(self, q: int, k: int, v: int, lengths: Optional[int] = None,
+                         window: Optional[int] = None, sinks: int = 0,
+                         scale: Optional[float] = None, name: str = "") -> int:
+        """Causal attention over a sliding window and the first ``sinks``
+        keys: q [batch, new, heads, d], k and v [batch, cache, kv_heads, d]
+        (heads a multiple of kv_heads; bf16 or fp16, d <= 128).
+
+        ``lengths`` (int32 [batch], default ``cache``) counts each request's
+        valid keys, its new tokens the last of them: query i stands at
+        p = length - new + i and sees key j iff j <= p, j < length and
+        (j > p - window or j < sinks).  ``window=None``: every earlier key.
+        A query that sees no key gets zeros.  ``scale`` defaults to
+        1/sqrt(d).  Keys that no query sees are never used, whatever they
+        hold."""
+        return self.add_op(ModelOpType.WINDOW_ATTENTION,
+                           [q, k, v] + ([lengths] if lengths is not None else []), name,
+                           window=None if window is None else int(window), sinks=int(sinks),
+                           scale=None if scale is None else float(scale))
+
+    def sample(self, logits: int, u: int, temperature: Optional[int] = None,
+               top_k: Optional[int] = None, top_p: Optional[int] = None,
+               min_p: Optional[int] = None, name: str = "") -> int:
+        """One token per row of logits [..., V] (int32 [...]), drawn with the
+        given random numbers u in [0, 1).
+
+        Every parameter is a vector with one value per row (float32; top_k
+        int32) or a scalar constant.  In order: w = exp((x - max) /
+        temperature); keep the ``top_k`` largest (<= 0: all); of those the
+        smallest set of largest ones whose weight is at least ``top_p`` of
+        theirs (>= 1: all); of those the ones with w >= ``min_p`` (the largest
+        w is 1).  Equal logits count by index, the lowest first.  The token is
+        the first, by index, at which the running weight of the kept tokens
+        exceeds u times their sum.  ``temperature`` <= 0 takes the largest
+        logit.  NaN logits and -inf are never drawn; a row of nothing else
+        gives -1.  Decisions are made in 64 bits."""
+        params = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+        given = [k for k, v in params.items() if v is not None]
+        return self.add_op(ModelOpType.SAMPLE, [logits, u] + [params[k] for k in given], name,
+                           params=given)
 
     def transpose(self, x: int, name: str = "") -> int:
         """TRANSPOSE of the last two dims (a matrix [N, K] -> [K, N]).  As

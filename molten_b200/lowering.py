@@ -25,7 +25,7 @@ from __future__ import annotations
 from dataclasses import dataclass, field
 from typing import Optional
 
-from .ir import DataflowGraph, OpType, ELEMENTWISE_OPS, REDUCTION_OPS
+from .ir import DataflowGraph, ModelOpType, OpType, ELEMENTWISE_OPS, REDUCTION_OPS
 
 
 class LoweringError(NotImplementedError):
@@ -38,7 +38,8 @@ _DTYPE_ALIASES = {
     "bfloat16": "bfloat16", "bf16": "bfloat16",
     "float16": "float16", "half": "float16", "fp16": "float16", "f16": "float16",
 }
-DTYPE_SIZE = {"float32": 4, "bfloat16": 2, "float16": 2}
+DTYPE_SIZE = {"float32": 4, "bfloat16": 2, "float16": 2, "int32": 4, "uint8": 1}
+INT_DTYPES = ("int32", "uint8")   # positions, lengths, packed weights, tokens
 DTYPE_CTYPE = {"float32": "float", "bfloat16": "bf16", "float16": "f16"}
 
 
@@ -47,6 +48,12 @@ def canon_dtype(d) -> str:
     if s not in _DTYPE_ALIASES:
         raise LoweringError(f"unsupported dtype {d!r} (float32, bfloat16, float16)")
     return _DTYPE_ALIASES[s]
+
+
+def canon_tensor_dtype(d) -> str:
+    """``canon_dtype`` plus the integer types of tensors that are not computed with."""
+    s = str(d).replace("torch.", "")
+    return s if s in INT_DTYPES else canon_dtype(d)
 
 
 def promote(dtypes) -> str:
@@ -116,6 +123,9 @@ def infer_shapes(graph: DataflowGraph, op_ids, known: dict) -> dict:
         elif t == OpType.ROTATE:
             s = ins[0]
             check_rope_shapes(op, ins)
+        elif isinstance(t, ModelOpType):
+            from .decode import infer_shape
+            s = infer_shape(op, ins)
         elif t == OpType.TRANSPOSE:
             if len(ins[0]) < 2:
                 raise LoweringError("TRANSPOSE needs rank >= 2")
@@ -231,6 +241,7 @@ class GroupPlan:
     output_shapes: list
     kernels: list         # [SubKernel]
     temps: dict           # op id -> (shape, dtype) of intermediates
+    key: str = ""         # what tells plans of the same source apart (sizes passed at launch)
 
 
 # ------------------------------------------------------------ group split
@@ -355,16 +366,18 @@ def split_group(graph: DataflowGraph, ordered: list, outs=(), fuse_prologue: boo
     ROTATE (RoPE) reads each element's pair partner, so it runs as a
     sub-kernel of its own between what it depends on and what follows (the
     fusion rules put it in any group: it is neither elementwise nor a
-    reduction, ``fusion.py:65``)."""
+    reduction, ``fusion.py:65``).  So does every ``ModelOpType``."""
     if fuse_attention and attention_pattern(graph, ordered, set(outs)):
         return [("attn", list(ordered))]
-    rot = [i for i in ordered if graph.ops[i].op_type == OpType.ROTATE]
+    rot = [i for i in ordered if graph.ops[i].op_type == OpType.ROTATE
+           or isinstance(graph.ops[i].op_type, ModelOpType)]
     if rot:
         r = rot[0]
+        family = "rope" if graph.ops[r].op_type == OpType.ROTATE else "model"
         pre_set = _deps_within(graph, r, set(ordered))
         pre = [i for i in ordered if i in pre_set]
         rest = [i for i in ordered if i not in pre_set and i != r]
-        return ((split_group(graph, pre, outs, fuse_prologue) if pre else []) + [("rope", [r])]
+        return ((split_group(graph, pre, outs, fuse_prologue) if pre else []) + [(family, [r])]
                 + (split_group(graph, rest, outs, fuse_prologue) if rest else []))
     mm = [i for i in ordered if graph.ops[i].op_type == OpType.MATMUL]
     if not mm:

@@ -4,10 +4,10 @@ from __future__ import annotations
 
 from typing import Optional
 
-from .ir import DataflowGraph, OpType, TensorShape
+from .ir import DataflowGraph, ModelOpType, OpType, TensorShape
 from .lowering import (
     DTYPE_SIZE, GroupPlan, LoweringError, Operand, OutputSpec, SubKernel,
-    broadcast_shapes, build_dag, canon_dtype, choose_ew_config,
+    INT_DTYPES, broadcast_shapes, build_dag, canon_tensor_dtype, choose_ew_config,
     choose_row_config, choose_row_tma_config, choose_rope_config, classify_operand,
     rms_prologue, attention_pattern,
     group_boundary, infer_shapes,
@@ -50,6 +50,9 @@ def _op_dtypes(graph, ordered, dtypes: dict) -> dict:
         if op.op_type == OpType.ROTATE:
             out[oid] = out[op.inputs[0]]          # out.to(x.dtype), ops.py:35
             continue
+        if isinstance(op.op_type, ModelOpType):
+            out[oid] = "int32" if op.op_type == ModelOpType.SAMPLE else out[op.inputs[0]]
+            continue
         out[oid] = promote(ds) if ds else "float32"
     return out
 
@@ -74,7 +77,7 @@ def plan_group(graph: DataflowGraph, group_op_ids, input_shapes: dict,
         if graph.ops[i].op_type == OpType.CONSTANT:
             known[i] = ()
     shapes = infer_shapes(graph, ordered, known)
-    dts = {i: canon_dtype(input_dtypes[i]) for i in inputs}
+    dts = {i: canon_tensor_dtype(input_dtypes[i]) for i in inputs}
     dts = _op_dtypes(graph, ordered, dts)
 
     # {"gemm": {"prologue": True}} runs RMSNorm -> GEMM as one GEMM that
@@ -88,8 +91,10 @@ def plan_group(graph: DataflowGraph, group_op_ids, input_shapes: dict,
                         fuse_attention=(tune.get("attn") or {}).get("fused", True))
     # intermediates between the sub-kernels of one group are stored in fp32,
     # so a split group still rounds once (at its outputs); a MATMUL operand
-    # keeps its 16-bit type because the tensor cores read it
+    # keeps its 16-bit type because the tensor cores read it, and so does an
+    # operand of a model operator
     mm_operands = {i for o in ordered if graph.ops[o].op_type == OpType.MATMUL
+                   or isinstance(graph.ops[o].op_type, ModelOpType)
                    for i in graph.ops[o].inputs}
     storage = dict(dts)
     produced_by = {}
@@ -114,7 +119,7 @@ def plan_group(graph: DataflowGraph, group_op_ids, input_shapes: dict,
         sk_outs = [o for o in ops if o in out_set or o in later]
         for o in sk_outs:
             if o not in out_set:
-                if o not in mm_operands:
+                if o not in mm_operands and storage[o] not in INT_DTYPES:
                     storage[o] = "float32"
                 temps[o] = (shapes[o], storage[o])
         sub = _plan_sub(graph, family, ops, sk_ext, sk_outs, shapes, storage, tune)
@@ -138,7 +143,9 @@ def plan_group(graph: DataflowGraph, group_op_ids, input_shapes: dict,
         input_shapes=[known[i] for i in inputs],
         outputs=list(outs), output_dtypes=[dts[o] for o in outs],
         output_shapes=[shapes[o] for o in outs],
-        kernels=kernels, temps=temps)
+        kernels=kernels, temps=temps,
+        key=repr([(sk.op_ids, sk.config) for sk in kernels if sk.family == "model"])
+        if any(sk.family == "model" for sk in kernels) else "")
 
 
 SPLIT3_BLOCK = 256
@@ -236,6 +243,12 @@ def _plan_causal_softmax(graph, ops, ext, outs, shapes, dts, tune) -> Optional[S
 
 
 def _plan_sub(graph, family, ops, ext, outs, shapes, dts, tune) -> SubKernel:
+    if family == "model":
+        from .decode import plan_model_op
+        return plan_model_op(graph, ops[0], outs, shapes, dts, tune)
+    for j in ext:
+        if dts.get(j) in INT_DTYPES:
+            raise LoweringError(f"op {j} is {dts[j]}: only floats are computed with")
     if family in ("row", "ew"):
         cs = _plan_causal_softmax(graph, ops, ext, outs, shapes, dts, tune)
         if cs is not None:

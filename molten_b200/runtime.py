@@ -34,7 +34,8 @@ from typing import Optional
 from . import _capi
 from .build import build_cubin, default_cache_dir
 from .codegen import CodeGenerator, GeneratedKernel, KernelConfig, kernel_entry
-from .lowering import DTYPE_SIZE, LoweringError, canon_dtype
+from .decode_launch import STRIDED, launch_model_op
+from .lowering import DTYPE_SIZE, LoweringError, canon_tensor_dtype
 
 _TORCH_DTYPES = None
 
@@ -45,12 +46,13 @@ def _torch():
 
 
 def _dtype_name(t) -> str:
-    return canon_dtype(str(t.dtype))
+    return canon_tensor_dtype(str(t.dtype))
 
 
 def _torch_dtype(name: str):
     torch = _torch()
-    return {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}[name]
+    return {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16,
+            "int32": torch.int32, "uint8": torch.uint8}[name]
 
 
 _TMA_CODE = {"bfloat16": _capi.DT_BF16, "float16": _capi.DT_F16, "float32": _capi.DT_F32}
@@ -274,10 +276,35 @@ class _Spec:
         env.update(zip(plan.outputs, outs))
         if all(o.numel() == 0 for o in outs):
             return outs                      # empty outputs (no rows or no columns): no launch
+        if stream != torch._C._cuda_getCurrentRawStream(di):
+            # a stream other than the caller's current one: intermediates and
+            # workspaces belong to it, or they would be reused while it runs
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=dev)):
+                self._launch(env, dev, di, stream, row_offset)
+        elif torch.cuda.current_device() != di:
+            with torch.cuda.device(di):         # the launches make di current
+                self._launch(env, dev, di, stream, row_offset)
+        else:
+            self._launch(env, dev, di, stream, row_offset)
+        if DEBUG:
+            torch.cuda.synchronize(di)
+            bits = _capi.read_status(di, True)
+            if bits:
+                raise _capi.MoltenError(f"{self.gk.name}: a bounded wait ran out on device {di} "
+                                        f"(status word {bits:#x})")
+        return outs
+
+    def _launch(self, env: dict, dev, di: int, stream: int, row_offset: int) -> None:
+        """Launch every sub-kernel of the plan over the tensors of ``env``."""
+        torch = _torch()
+        plan = self.plan
         for op_id, (s, d) in self.temp_specs.items():
             env[op_id] = torch.empty(s, dtype=d, device=dev)
         mod = self.module(di)
         for i, sk in enumerate(plan.kernels):
+            if sk.family == "model":
+                launch_model_op(self, i, env, di, stream)
+                continue
             cfg = self.launch_cfg(i, di)
             if sk.family == "attn":
                 a = self._attn_args(sk, env, di)
@@ -341,13 +368,6 @@ class _Spec:
                                             f"as kernel {self.entries[i].decode()} requires")
                 outp[o.index] = p
             mod.launch(self.entries[i], cfg, a, stream)
-        if DEBUG:
-            torch.cuda.synchronize(di)
-            bits = _capi.read_status(di, True)
-            if bits:
-                raise _capi.MoltenError(f"{self.gk.name}: a bounded wait ran out on device {di} "
-                                        f"(status word {bits:#x})")
-        return outs
 
 
 def _empty_outputs(gk: GeneratedKernel) -> bool:
@@ -367,6 +387,8 @@ def _alignment_rules(sk):
     16 for TMA sources and for 16-byte vector slots, the slot size for
     narrower slots, the element size for per-row scalars."""
     c = sk.config
+    if sk.family == "model":
+        return [], []                    # checked at the launch (decode_launch.py)
     if sk.family == "attn":
         # TMA sources; P is written by TMA (16) or element by element (2)
         return [16, 16], [16 if c["rows_aligned"] else 2]
@@ -508,8 +530,13 @@ class CompiledKernel:
     @staticmethod
     def _conform(spec: _Spec, tensors):
         plan = spec.plan
-        gemm_b = set()
+        gemm_b, strided = set(), None
         for sk in plan.kernels:
+            # what a model operator alone reads may stay strided
+            takes = {o.op_id for o in sk.operands
+                     if sk.family == "model" and o.index in STRIDED[sk.config["op"]]}
+            leaves = {o.op_id for o in sk.operands} - takes
+            strided = (takes if strided is None else strided | takes) - leaves
             if sk.family == "gemm" and not sk.config.get("split3"):
                 # (an fp32 B is read whole by its split kernel: contiguous)
                 gemm_b.add(sk.operands[sk.b_operand].op_id)
@@ -518,6 +545,8 @@ class CompiledKernel:
             if op_id in gemm_b and t.dim() == 2 and t.stride(1) == 1 \
                     and (t.stride(0) * t.element_size()) % 16 == 0:
                 out.append(t)              # a column slice of B is fine for TMA
+            elif op_id in strided:
+                out.append(t)
             else:
                 out.append(t.contiguous())
         return out
@@ -683,7 +712,9 @@ class MoltenRuntime:
         _capi.load_library()           # fail loudly when the runtime is missing
 
     def compile(self, kernel: GeneratedKernel) -> CompiledKernel:
-        key = hashlib.sha256(kernel.source.encode()).hexdigest()[:16]
+        # (the sources of model operators leave sizes to the launch: plan.key)
+        text = kernel.source + (kernel.plan.key if kernel.plan is not None else "")
+        key = hashlib.sha256(text.encode()).hexdigest()[:16]
         ck = self._compiled.get(key)
         if ck is not None:
             return ck

@@ -1,0 +1,262 @@
+"""The operators of a decode step on a B200, against plain 64-bit forms."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from molten_b200 import _capi, graphs
+from molten_b200.codegen import compile_graph
+from molten_b200.ir import DataflowGraph, TensorShape as TS
+from molten_b200.lowering import LoweringError
+from molten_b200.runtime import MoltenRuntime
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+DT = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def rt():
+    return MoltenRuntime()
+
+
+def gen_of(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def compiled(rt, g, dtype):
+    ks = compile_graph(g, dtype=dtype)
+    assert len(ks) == 1
+    return rt.compile(ks[0])
+
+
+def half_step(dtype):
+    return torch.finfo(DT[dtype]).eps / 2
+
+
+# ------------------------------------------------------------- 4-bit products
+def q4_inputs(m, n, k, group, dtype, zeros, seed=0):
+    g = gen_of(seed)
+    x = torch.randn(m, k, generator=g, device=DEV).to(DT[dtype])
+    q = torch.randint(0, 256, (n, k // 2), generator=g, device=DEV, dtype=torch.uint8)
+    s = ((0.5 + torch.rand(n, k // group, generator=g, device=DEV)) / k ** 0.5).to(DT[dtype])
+    z = (16 * torch.rand(n, k // group, generator=g, device=DEV)).to(DT[dtype]) if zeros else None
+    return x, q, s, z
+
+
+def q4_reference(x, q, s, z):
+    """(y, sum of |terms|) in 64 bits."""
+    n, k = q.shape[0], q.shape[1] * 2
+    w = torch.stack((q & 15, q >> 4), -1).view(n, s.shape[1], -1).double()
+    zp = z.double()[:, :, None] if z is not None else 8.0
+    sd = s.double()[:, :, None]
+    mag = ((w - 8).abs() + (zp - 8.0 if z is None else (zp - 8.0).abs())) * sd
+    w = ((w - zp) * sd).view(n, k)
+    return x.double() @ w.t(), x.double().abs() @ mag.view(n, k).t()
+
+
+def check_q4(y, x, q, s, z, dtype):
+    ref, mag = q4_reference(x, q, s, z)
+    # one output rounding; at most 24 MMAs a group, each off by at most one
+    # step (2^-23) of the magnitudes it sums, and the fp32 sum over groups
+    tol = half_step(dtype) * ref.abs() + 2.0 ** -18 * mag
+    err = (y.double() - ref).abs()
+    assert bool((err <= tol).all()), f"max error {err.max().item():.3e}"
+    # the errors are not systematic: the fp32 result as a whole is near
+    if dtype == "float32":
+        assert err.norm() <= 1e-6 * ref.norm()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("m,n,k,group", [
+    (1, 1, 32, 32), (1, 16, 128, 128), (1, 17, 64, 64), (2, 33, 96, 32), (3, 100, 192, 64),
+    (8, 257, 1152, 128), (9, 48, 4096, 32), (16, 640, 512, 64), (17, 31, 2176, 128),
+    (32, 1000, 1024, 32), (5, 4099, 160, 32)])
+def test_matvec_q4(rt, m, n, k, group, dtype, zeros):
+    x, q, s, z = q4_inputs(m, n, k, group, dtype, zeros, seed=m + n)
+    ck = compiled(rt, graphs.matvec_q4(m, n, k, group, dtype=dtype, zeros=zeros), dtype)
+    args = [x, q, s] + ([z] if zeros else [])
+    y = ck(*args)
+    assert y.shape == (m, n) and y.dtype == DT[dtype]
+    check_q4(y, x, q, s, z, dtype)
+    assert torch.equal(y, ck(*args))
+
+
+@pytest.mark.parametrize("warps,warps_n,ksplit", [
+    (8, 1, 1), (8, 1, 8), (8, 2, 2), (16, 4, 4), (8, 8, 1), (16, 8, 8), (16, 16, 1), (16, 1, 2)])
+def test_matvec_q4_splits(rt, warps, warps_n, ksplit):
+    m, n, k, group = 4, 200, 8192, 128
+    tuned = MoltenRuntime(tune={"q4": {"warps": warps, "warps_n": warps_n, "ksplit": ksplit}})
+    ck = compiled(tuned, graphs.matvec_q4(m, n, k, group, zeros=True), "bfloat16")
+    # (another shape than the declared one: the runtime's tune applies)
+    x2, q2, s2, z2 = q4_inputs(m, n + 1, k, group, "bfloat16", True, seed=4)
+    check_q4(ck(x2, q2, s2, z2), x2, q2, s2, z2, "bfloat16")
+
+
+@pytest.mark.parametrize("m,n,k,group,dtype", [
+    (32, 700, 14336, 32, "bfloat16"), (20, 3000, 5120, 64, "float32"), (2, 40000, 256, 128, "float16"),
+    (1, 5000, 60000 // 32 * 32, 32, "float32"), (7, 130, 32768, 128, "bfloat16")])
+def test_matvec_q4_chunks_and_many_tiles(rt, m, n, k, group, dtype):
+    """x staged in several chunks of k; CTAs that walk over many tiles."""
+    x, q, s, z = q4_inputs(m, n, k, group, dtype, True, seed=5)
+    ck = compiled(rt, graphs.matvec_q4(m, n, k, group, dtype=dtype, zeros=True), dtype)
+    check_q4(ck(x, q, s, z), x, q, s, z, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_matvec_q4_range_of_x(rt, dtype):
+    """Rows and groups of very different size, zeros, and the largest values."""
+    m, n, k, group = 5, 64, 512, 64
+    x, q, s, z = q4_inputs(m, n, k, group, dtype, True, seed=6)
+    power = torch.tensor([0, 100, -100, 60, -60, 20, 119, -10], device=DEV).repeat_interleave(group)
+    x = (x.double() * torch.exp2(power.double())).to(DT[dtype])
+    x[1] = 0
+    x[2, ::2] = 0
+    x[3, :group] *= 2.0 ** -30
+    ck = compiled(rt, graphs.matvec_q4(m, n, k, group, dtype=dtype, zeros=True), dtype)
+    check_q4(ck(x, q, s, z), x, q, s, z, dtype)
+
+
+def test_matvec_q4_mixed_types_rank_and_strides(rt):
+    """bf16 x with fp32 scales, x [2, 2, K] out of a wider tensor."""
+    k, n, group = 256, 70, 64
+    _, q, s, z = q4_inputs(1, n, k, group, "float32", True, seed=5)
+    wide = torch.randn(2, 2, 3 * k, generator=gen_of(6), device=DEV).to(torch.bfloat16)
+    x = wide[..., k:2 * k]
+    g = DataflowGraph("q4")
+    ids = [g.add_input("x", TS([2, 2, k])), g.add_input("q", TS([n, k // 2]), dtype="uint8"),
+           g.add_input("s", TS([n, k // group]), dtype="float32"),
+           g.add_input("z", TS([n, k // group]), dtype="float32")]
+    g.add_output(g.matvec_q4(ids[0], ids[1], ids[2], zeros=ids[3]))
+    ck = compiled(rt, g, "bfloat16")
+    y = ck(x, q, s, z)
+    assert y.shape == (2, 2, n)
+    check_q4(y.view(4, n), x.reshape(4, k), q, s, z, "bfloat16")
+
+
+def test_matvec_q4_in_a_group(rt):
+    """RMSNorm -> 4-bit product -> + bias -> SiLU as one graph."""
+    m, n, k, group = 4, 192, 512, 128
+    x, q, s, _ = q4_inputs(m, n, k, group, "bfloat16", False, seed=7)
+    w = (1 + 0.1 * torch.randn(k, generator=gen_of(8), device=DEV)).to(torch.bfloat16)
+    b = torch.randn(n, generator=gen_of(9), device=DEV).to(torch.bfloat16)
+    g = DataflowGraph("norm_q4")
+    xi, wi = g.add_input("x", TS([m, k])), g.add_input("w", TS([k]))
+    qi = g.add_input("q", TS([n, k // 2]), dtype="uint8")
+    si, bi = g.add_input("s", TS([n, k // group]), dtype="bfloat16"), g.add_input("b", TS([n]))
+    y = g.matvec_q4(g.rms_norm(xi, wi, "norm"), qi, si)
+    g.add_output(g.silu(g.add(y, bi)))
+    out = compiled(rt, g, "bfloat16")(x, w, q, s, b)
+    xd = x.double()
+    h = xd / (xd.pow(2).mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+    ref, _ = q4_reference(h, q, s, None)
+    _, mag = q4_reference(h, q, s, None)
+    ref = ref + b.double()
+    # the normalised rows are rounded to bf16 once, the result once; SiLU's
+    # slope is at most 1.1
+    tol = 2.0 ** -8 * 1.1 * mag + 2.0 ** -8 * ref.abs() + 1e-4
+    assert bool(((out.double() - torch.nn.functional.silu(ref)).abs() <= tol).all())
+
+
+def test_matvec_q4_refuses_unaligned_pointers(rt):
+    x, q, s, _ = q4_inputs(1, 16, 128, 128, "bfloat16", False)
+    ck = compiled(rt, graphs.matvec_q4(1, 16, 128, 128), "bfloat16")
+    raw = torch.empty(16 * 64 + 1, dtype=torch.uint8, device=DEV)
+    with pytest.raises(_capi.MoltenError, match="aligned"):
+        ck(x, raw[1:].view(16, 64), s)
+    with pytest.raises(LoweringError):
+        ck(x.float().int(), q, s)
+
+
+# ------------------------------------------------------ rotary at positions
+def rope_reference(x, cos, sin, pos, sections, style):
+    half = x.shape[-1] // 2
+    axis = torch.repeat_interleave(torch.arange(len(sections)), torch.tensor(sections)).to(DEV)
+    rows = pos.long().view(len(sections), *x.shape[:-2])[axis].movedim(0, -1)     # [.., seq, pair]
+    pair = torch.arange(half, device=DEV)
+    pad = rows < 0
+    c = cos.double()[rows.clamp(min=0), pair].masked_fill(pad, 1.0)[..., None, :]
+    s = sin.double()[rows.clamp(min=0), pair].masked_fill(pad, 0.0)[..., None, :]
+    xd = x.double()
+    a, b = (xd[..., :half], xd[..., half:]) if style == "half" else (xd[..., 0::2], xd[..., 1::2])
+    r0, r1 = a * c - b * s, a * s + b * c
+    mag = (a * c).abs() + (b * s).abs() + (a * s).abs() + (b * c).abs()
+    if style == "half":
+        return torch.cat((r0, r1), -1), torch.cat((mag, mag), -1)
+    return torch.stack((r0, r1), -1).flatten(-2), torch.stack((mag, mag), -1).flatten(-2)
+
+
+def check_rope(out, x, cos, sin, pos, sections, style, dtype):
+    ref, mag = rope_reference(x, cos, sin, pos, sections, style)
+    # one rounding; two fp32 products and a sum before it
+    tol = half_step(dtype) * ref.abs() + 2 * 2.0 ** -24 * mag + 2.0 ** -24 * ref.abs()
+    assert bool(((out.double() - ref).abs() <= tol).all())
+
+
+def tables(rows, half, seed=1, dtype=torch.float32):
+    a = torch.rand(rows, half, generator=gen_of(seed), device=DEV, dtype=torch.float64) * 6.3
+    return torch.cos(a).to(dtype), torch.sin(a).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("style", ["half", "interleaved"])
+@pytest.mark.parametrize("batch,seq,heads,dim,sections", [
+    (1, 1, 1, 2, [1]), (3, 1, 40, 128, [64]), (2, 5, 7, 128, [16, 24, 24]), (1, 33, 4, 80, [13, 27]),
+    (2, 9, 3, 6, [1, 1, 1]), (1, 300, 5, 96, [0, 48]), (1, 4, 2, 64, [5, 7, 9, 11]),
+    (1, 3, 2, 1024, [512])])
+def test_rope_positions(rt, batch, seq, heads, dim, sections, style, dtype):
+    rows = 57
+    x = torch.randn(batch, seq, heads, dim, generator=gen_of(2), device=DEV).to(DT[dtype])
+    cos, sin = tables(rows, dim // 2)
+    pos = torch.randint(-2, rows, (len(sections), batch, seq), generator=gen_of(3), device=DEV,
+                        dtype=torch.int32)
+    g = graphs.rope_positions(batch, seq, heads, dim, rows, sections, dtype=dtype, style=style)
+    out = compiled(rt, g, dtype)(x, cos, sin, pos)
+    check_rope(out, x, cos, sin, pos, sections, style, dtype)
+    assert MoltenRuntime.read_status(0) == 0
+    # padding: both halves of a pair are left bit for bit
+    skip = (pos < 0).all(0)
+    assert torch.equal(out[skip], x[skip])
+
+
+@pytest.mark.parametrize("style", ["half", "interleaved"])
+def test_rope_positions_many_heads_per_thread(rt, style):
+    """Many tokens, more heads than a CTA takes at once."""
+    x = torch.randn(2, 4700, 22, 128, generator=gen_of(2), device=DEV).to(torch.bfloat16)
+    cos, sin = tables(4096, 64)
+    pos = torch.randint(0, 4096, (2, 4700), generator=gen_of(3), device=DEV, dtype=torch.int32)
+    ck = compiled(rt, graphs.rope_positions(2, 4700, 22, 128, 4096, style=style), "bfloat16")
+    check_rope(ck(x, cos, sin, pos), x, cos, sin, pos, [64], style, "bfloat16")
+
+
+def test_rope_positions_views_tables_and_alignment(rt):
+    """x out of a fused q, k, v tensor; 16-bit and packed tables; pointers
+    that are not 16-byte aligned."""
+    b, s, h, d, rows = 2, 6, 3, 64, 40
+    fused = torch.randn(b, s, 3 * h, d, generator=gen_of(4), device=DEV).to(torch.float16)
+    x = fused[:, :, h:2 * h]
+    cos, sin = tables(rows, d // 2, dtype=torch.bfloat16)
+    pos = torch.randint(0, rows, (b, s), generator=gen_of(5), device=DEV, dtype=torch.int32)
+    ck = compiled(rt, graphs.rope_positions(b, s, h, d, rows, dtype="float16",
+                                            table_dtype="bfloat16"), "float16")
+    check_rope(ck(x, cos, sin, pos), x, cos, sin, pos, [32], "half", "float16")
+    packed = torch.stack((cos, sin), -1).flatten(1).float()
+    g = graphs.rope_positions(b, s, h, d, rows, dtype="float16", packed=True, style="interleaved")
+    check_rope(compiled(rt, g, "float16")(x, packed, pos), x, cos, sin, pos, [32], "interleaved",
+               "float16")
+    odd = torch.empty(x.numel() + 1, dtype=torch.float16, device=DEV)[1:].view(x.shape)
+    odd.copy_(x)
+    check_rope(ck(odd, cos, sin, pos), x, cos, sin, pos, [32], "half", "float16")
+
+
+def test_rope_position_past_the_table_is_reported(rt):
+    x = torch.randn(1, 3, 2, 8, generator=gen_of(6), device=DEV)
+    cos, sin = tables(5, 4)
+    pos = torch.tensor([[0, 5, 4]], dtype=torch.int32, device=DEV)
+    out = compiled(rt, graphs.rope_positions(1, 3, 2, 8, 5, dtype="float32"), "float32")(x, cos, sin, pos)
+    assert torch.equal(out[:, 1], x[:, 1])
+    assert MoltenRuntime.read_status(0) == 1024 and MoltenRuntime.read_status(0) == 0
