@@ -129,6 +129,26 @@ typedef struct molten_q4_args {
   int reserved;
 } molten_q4_args;
 
+/* Parameter block of the window-attention kernels for few query rows
+ * (device side: molten::WindowArgs in molten/window_decode.cuh).  Strides
+ * are in elements and, like the pointers of q, k and v, multiples of 16 bytes.
+ * With parts > 1 the kernel "<name>_join" follows with the same block and
+ * `part` holds batch * kv_heads * parts * (nq * per) * (dim + 2) floats. */
+typedef struct molten_window_args {
+  const void* q;                 /* [batch, nq, kv_heads * per, dim] */
+  const void* k;                 /* [batch, cache, kv_heads, dim] */
+  const void* v;
+  const int* lengths;            /* [batch] valid keys, or null: cache */
+  void* out;                     /* [batch, nq, heads, dim] contiguous */
+  float* part;
+  long long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h;
+  int batch, nq, cache, kv_heads, per, dim;
+  int window, sinks;             /* window < 0: every earlier key */
+  float scale_log2;              /* scale * log2(e) */
+  int ranks, parts;              /* CTAs of the cluster; clusters per item */
+  int reserved;
+} molten_window_args;
+
 /* Version of this ABI (major * 100 + minor). */
 int molten_version(void);
 

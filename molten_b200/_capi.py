@@ -99,6 +99,18 @@ class Q4Args(ctypes.Structure):
                 ("teams", ctypes.c_int), ("reserved", ctypes.c_int)]
 
 
+class WindowArgs(ctypes.Structure):
+    """molten_window_args / molten::WindowArgs."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "lengths", "out", "part")]
+                + [(n, ctypes.c_longlong) for n in ("q_b", "q_s", "q_h", "k_b", "k_s", "k_h",
+                                                     "v_b", "v_s", "v_h")]
+                + [(n, ctypes.c_int) for n in ("batch", "nq", "cache", "kv_heads", "per", "dim",
+                                               "window", "sinks")]
+                + [("scale_log2", ctypes.c_float), ("ranks", ctypes.c_int),
+                   ("parts", ctypes.c_int), ("reserved", ctypes.c_int)])
+
+
+assert ctypes.sizeof(WindowArgs) == 168
 assert ctypes.sizeof(RopePosArgs) == 120
 assert ctypes.sizeof(Q4Args) == 88
 assert ctypes.sizeof(RowArgs) == 160

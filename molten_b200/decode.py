@@ -33,6 +33,10 @@ Q4_SUMS_BYTES = 16 * 1024         # sums of a CTA's tiles, where they are kept
 SMEM_LIMIT = 227 * 1024           # shared memory of a CTA, and of an SM
 SMEM_SM = 228 * 1024
 
+WINDOW_MAX_DIM = 128
+WINDOW_FEW_ROWS = 32              # rows of a key head up to which the few-row kernel runs
+WINDOW_WARPS, WINDOW_STAGES, WINDOW_TILE = 4, 3, 16
+
 ROPE_MAX_AXES = 4
 ROPE_MAX_DIM = 1024
 
@@ -86,7 +90,24 @@ def _rope_shape(op, ins):
     return x
 
 
-_SHAPES = {ModelOpType.MATVEC_Q4: _q4_shape, ModelOpType.ROTATE_POSITIONS: _rope_shape}
+def _window_shape(op, ins):
+    _need(len(ins) in (3, 4), "window_attention takes (q, k, v[, lengths])")
+    q, k, v = ins[:3]
+    _need(len(q) == 4 and len(k) == 4 and k == v and q[0] == k[0] and q[3] == k[3],
+          "window_attention needs q [batch, new, heads, d] and k, v [batch, cache, kv_heads, d]: "
+          f"{q}, {k}, {v}")
+    _need(k[2] > 0 and q[2] % k[2] == 0, f"window_attention: {q[2]} heads over {k[2]} key heads")
+    _need(0 < q[3] <= WINDOW_MAX_DIM and q[3] % 8 == 0,
+          f"window_attention: head dim {q[3]} must be a multiple of 8, at most {WINDOW_MAX_DIM}")
+    _need(len(ins) == 3 or ins[3] == q[:1], f"window_attention: lengths {ins[-1]}, expected {q[:1]}")
+    w, s = op.attrs.get("window"), op.attrs.get("sinks") or 0
+    _need(w is None or w >= 1, f"window_attention: window {w} must be at least 1 (None: no limit)")
+    _need(s >= 0, f"window_attention: {s} sinks")
+    return q
+
+
+_SHAPES = {ModelOpType.MATVEC_Q4: _q4_shape, ModelOpType.ROTATE_POSITIONS: _rope_shape,
+           ModelOpType.WINDOW_ATTENTION: _window_shape}
 
 
 # -------------------------------------------------------------------- types
@@ -260,7 +281,51 @@ def _plan_rope(op, sk, tune) -> dict:
             "flops": 3 * tokens * heads * d}
 
 
-_PLANS = {ModelOpType.MATVEC_Q4: _plan_q4, ModelOpType.ROTATE_POSITIONS: _plan_rope}
+def _plan_window(op, sk, tune) -> dict:
+    q, k, v = sk.operands[:3]
+    _need(q.dtype == k.dtype == v.dtype and q.dtype in ("bfloat16", "float16"),
+          f"window_attention takes bf16 or fp16 q, k and v of one type, got {q.dtype}, {k.dtype}, "
+          f"{v.dtype}")
+    batch, new, heads, dim = q.shape
+    cache, kv_heads = k.shape[1], k.shape[2]
+    per = heads // kv_heads
+    rows, items = new * per, batch * kv_heads
+    _need(max(cache, new) < 2 ** 30 and items < 2 ** 24 and rows < 2 ** 30,
+          "window_attention: sizes beyond the kernel's range")
+    window, sinks = op.attrs.get("window"), op.attrs.get("sinks") or 0
+    window = -1 if window is None or window >= cache + new else window
+    sinks = min(sinks, cache)
+    scale = op.attrs.get("scale")
+    scale = dim ** -0.5 if scale is None else scale
+    o = tune.get("window") or {}
+    c = {"batch": batch, "new": new, "cache": cache, "kv_heads": kv_heads, "per": per, "dim": dim,
+         "window": window, "sinks": sinks, "scale": scale, "dp": 64 if dim <= 64 else 128}
+    # most keys a row can see, and most keys any row of a request sees
+    seen = cache if window < 0 else min(cache, window + sinks)
+    span = cache if window < 0 else min(cache, window + sinks + new)
+    c["flops"] = 4 * batch * heads * new * seen * dim
+    _need(rows <= WINDOW_FEW_ROWS, "window_attention: too many rows")
+    tiles = -(-span // WINDOW_TILE) + 1
+    # two CTAs an SM: split the keys of an item over a cluster, and past that
+    # over parts joined by a second kernel, as far as every warp has a tile
+    want = max(1, min(-(-2 * SMS // max(1, items)), tiles // WINDOW_WARPS))
+    ranks = 1
+    while ranks < 8 and 2 * ranks <= want:
+        ranks *= 2
+    parts = max(1, want // ranks) if ranks == 8 else 1
+    ranks, parts = int(o.get("ranks") or ranks), int(o.get("parts") or parts)
+    mt = 1 if rows <= 16 else 2
+    warps, stages = int(o.get("warps") or WINDOW_WARPS), int(o.get("stages") or WINDOW_STAGES)
+    ring = warps * stages * 2 * WINDOW_TILE * c["dp"] * 2
+    area = warps * 16 * mt * (c["dp"] + 4) * 4
+    smem = max(ring, area) + warps * 16 * mt * (8 + WINDOW_TILE * 4)
+    c.update(kind="few", mt=mt, ranks=ranks, parts=parts, items=items, rows=rows, warps=warps,
+             stages=stages, block=32 * warps, smem=smem)
+    return c
+
+
+_PLANS = {ModelOpType.MATVEC_Q4: _plan_q4, ModelOpType.ROTATE_POSITIONS: _plan_rope,
+          ModelOpType.WINDOW_ATTENTION: _plan_window}
 
 
 def launch_record(sk: SubKernel) -> dict:
@@ -270,6 +335,9 @@ def launch_record(sk: SubKernel) -> dict:
         rec.update(grid=c["teams"] * c["ksplit"], cluster=c["ksplit"], warps_n=c["warps_n"])
     elif c["op"] == ModelOpType.ROTATE_POSITIONS:
         rec.update(head_lanes=c["head_lanes"], tokens_per_cta=c["tokens_per_cta"])
+    elif c["op"] == ModelOpType.WINDOW_ATTENTION:
+        rec.update(kind=c["kind"], cluster=c["ranks"], parts=c["parts"],
+                   grid=c["items"] * c["parts"] * c["ranks"])
     return rec
 
 
@@ -317,4 +385,30 @@ extern "C" __global__ void __launch_bounds__(1024) {name}(const __grid_constant_
 """
 
 
-_EMIT = {ModelOpType.MATVEC_Q4: _emit_q4, ModelOpType.ROTATE_POSITIONS: _emit_rope}
+def _emit_window(sk, name):
+    c = sk.config
+    t, ot = DTYPE_CTYPE[sk.operands[0].dtype], DTYPE_CTYPE[sk.outputs[0].dtype]
+    lay = f"{c['dp']}, {c['mt']}, {c['warps']}, {c['stages']}"
+    return f"""// Molten sm_100a window attention, few query rows: {name}
+// {sk.operands[0].dtype}, head dim up to {c['dp']}, up to {16 * c['mt']} rows
+#include "molten/window_decode.cuh"
+
+using namespace molten;
+
+static_assert(WindowDecodeLayout<{lay}>::SMEM == {c['smem']}, "the launch's dynamic shared memory");
+
+extern "C" __global__ void __launch_bounds__({c['block']}, 2) {name}(const __grid_constant__ WindowArgs args) {{
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  pdl_enter();
+  window_decode<{t}, {ot}, {lay}>(args, smem_raw);
+}}
+
+extern "C" __global__ void __launch_bounds__(128) {name}_join(const __grid_constant__ WindowArgs args) {{
+  pdl_enter();
+  window_join<{ot}>(args);
+}}
+"""
+
+
+_EMIT = {ModelOpType.MATVEC_Q4: _emit_q4, ModelOpType.ROTATE_POSITIONS: _emit_rope,
+         ModelOpType.WINDOW_ATTENTION: _emit_window}

@@ -8,11 +8,14 @@ and captured graphs never share one.
 
 from __future__ import annotations
 
-import ctypes
+import math
 
 from . import _capi
 from .ir import ModelOpType
 from .lowering import DTYPE_SIZE
+
+
+LOG2E = math.log2(math.e)
 
 
 def _merged(t, keep: int):
@@ -106,7 +109,43 @@ def _launch_rope(spec, sk, entry, ins, out, device, stream):
     spec.module(device).launch(entry, _cfg(grid, c["block"]), a, stream)
 
 
-_LAUNCH = {ModelOpType.MATVEC_Q4: _launch_q4, ModelOpType.ROTATE_POSITIONS: _launch_rope}
+def _launch_window(spec, sk, entry, ins, out, device, stream):
+    c = sk.config
+    a = _capi.WindowArgs()
+    qkv = []
+    for j in range(3):
+        t = ins[j]
+        # 16-byte rows: the last dim contiguous, every other stride a multiple
+        # of 8 elements
+        if (t.stride(3) != 1 and t.shape[3] > 1) or not _aligned(t, 16, t.stride()[:3]):
+            t = t.contiguous()
+        _check_aligned(sk.operands[j].name, entry, t, 16)
+        qkv.append(t)
+    q, k, v = qkv
+    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.lengths = ins[3].data_ptr() if 3 in ins else None
+    a.q_b, a.q_s, a.q_h = q.stride()[:3]
+    a.k_b, a.k_s, a.k_h = k.stride()[:3]
+    a.v_b, a.v_s, a.v_h = v.stride()[:3]
+    a.batch, a.nq, a.cache, a.kv_heads = c["batch"], c["new"], c["cache"], c["kv_heads"]
+    a.per, a.dim, a.window, a.sinks = c["per"], c["dim"], c["window"], c["sinks"]
+    a.scale_log2 = c["scale"] * LOG2E
+    a.ranks, a.parts = c["ranks"], c["parts"]
+    mod = spec.module(device)
+    grid = c["items"] * c["parts"] * c["ranks"]
+    part = None
+    if c["parts"] > 1:
+        import torch
+        part = torch.empty(c["items"] * c["parts"] * c["rows"] * (c["dim"] + 2),
+                           dtype=torch.float32, device=q.device)
+        a.part = part.data_ptr()
+    mod.launch(entry, _cfg(grid, c["block"], c["ranks"], c["smem"]), a, stream)
+    if part is not None:
+        mod.launch(entry + b"_join", _cfg(-(-c["items"] * c["rows"] // 4), 128), a, stream)
+
+
+_LAUNCH = {ModelOpType.MATVEC_Q4: _launch_q4, ModelOpType.ROTATE_POSITIONS: _launch_rope,
+           ModelOpType.WINDOW_ATTENTION: _launch_window}
 
 # operands a kernel takes as strided views; the rest are made contiguous
 STRIDED = {ModelOpType.MATVEC_Q4: (0,), ModelOpType.ROTATE_POSITIONS: (0,),

@@ -260,3 +260,143 @@ def test_rope_position_past_the_table_is_reported(rt):
     out = compiled(rt, graphs.rope_positions(1, 3, 2, 8, 5, dtype="float32"), "float32")(x, cos, sin, pos)
     assert torch.equal(out[:, 1], x[:, 1])
     assert MoltenRuntime.read_status(0) == 1024 and MoltenRuntime.read_status(0) == 0
+
+
+# --------------------------------------------------------- window attention
+def seen_mask(lengths, new, cache, window, sinks):
+    """[batch, new, cache]: query i sees key j."""
+    n = lengths.long().clamp(0, cache)[:, None, None]
+    p = n - new + torch.arange(new, device=DEV)[:, None]
+    j = torch.arange(cache, device=DEV)
+    near = torch.ones_like(j, dtype=torch.bool) if window is None else (j > p - window) | (j < sinks)
+    return (j <= p) & (j < n) & near
+
+
+def attention_reference(q, k, v, lengths, window, sinks, scale=None):
+    """(o, sum p |v|, largest |score|) in 64 bits; unseen keys are left out."""
+    b, new, heads, d = q.shape
+    cache, kv = k.shape[1:3]
+    scale = d ** -0.5 if scale is None else scale
+    seen = seen_mask(lengths, new, cache, window, sinks)[:, None, None]            # b 1 1 new cache
+    used = seen.any(3)[:, 0, 0]                                                    # b cache
+    kd = torch.where(used[:, :, None, None], k.double(), 0.0)
+    vd = torch.where(used[:, :, None, None], v.double(), 0.0)
+    qd = q.double().view(b, new, kv, heads // kv, d)
+    s = torch.einsum("bnkgd,bckd->bkgnc", qd, kd) * scale
+    s = torch.where(seen, s, -torch.inf)
+    top = s.amax(-1, keepdim=True)
+    p = torch.where(seen, torch.exp(s - torch.where(top == -torch.inf, 0.0, top)), 0.0)
+    p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+    o = torch.einsum("bkgnc,bckd->bnkgd", p, vd)
+    mag = torch.einsum("bkgnc,bckd->bnkgd", p, vd.abs())
+    big = torch.where(seen, s, 0.0).abs().amax(-1)                                  # b kv per new
+    big = big.permute(0, 3, 1, 2)[..., None]
+    return (t.expand(b, new, kv, heads // kv, d).reshape(b, new, heads, d) for t in (o, mag, big))
+
+
+def check_attention(out, q, k, v, lengths, window, sinks, dtype, p_half, scale=None):
+    ref, mag, big = attention_reference(q, k, v, lengths, window, sinks, scale)
+    # one output rounding; P rounded to `p_half` of itself; scores summed in
+    # fp32 (d products, 2^-23 each of the largest score, and the exponential's
+    # argument again) and exponentials within 2^-20, in P and in its sum
+    tol = half_step(dtype) * ref.abs() + (p_half + 2.0 ** -19 + 2.0 ** -21 * (1 + big)) * mag
+    # subnormal outputs and weights of fp16
+    tol = tol + (2.0 ** -24 if dtype == "float16" else 0.0)
+    err = (out.double() - ref).abs()
+    assert bool((err <= tol).all()), f"max error {err.max().item():.3e}"
+
+
+def attention_inputs(b, new, cache, heads, kv, d, dtype, seed=0, spread=1.0):
+    g = gen_of(seed)
+    q = (spread * torch.randn(b, new, heads, d, generator=g, device=DEV)).to(DT[dtype])
+    k = torch.randn(b, cache, kv, d, generator=g, device=DEV).to(DT[dtype])
+    v = torch.randn(b, cache, kv, d, generator=g, device=DEV).to(DT[dtype])
+    return q, k, v
+
+
+def window_kernel(rt, b, new, cache, heads, kv, d, window, sinks, dtype, lengths=True, scale=None):
+    g = graphs.window_attention(b, new, cache, heads, kv, d, window=window, sinks=sinks, dtype=dtype,
+                                lengths=lengths, scale=scale)
+    return compiled(rt, g, dtype)
+
+
+FEW = [  # b, new, cache, heads, kv, d, window, sinks, lengths
+    (1, 1, 1, 1, 1, 64, 1, 0, [1]),
+    (3, 1, 40, 4, 2, 64, 7, 2, [40, 3, 0]),
+    (2, 1, 300, 8, 2, 128, 100, 4, [300, 150]),
+    (2, 1, 1000, 12, 4, 80, None, 0, [1000, 999]),
+    (4, 1, 515, 16, 1, 128, 64, 33, [515, 64, 65, 17]),
+    (2, 2, 130, 10, 2, 8, 16, 1, [130, 1]),
+    (1, 4, 2500, 32, 8, 128, 1024, 16, [2333]),
+    (2, 3, 77, 20, 2, 96, 30, 0, [77, 2]),
+    (1, 32, 200, 4, 4, 64, 50, 5, [180]),
+    (5, 1, 33, 7, 7, 24, 1, 3, [33, 32, 31, 5, -4]),
+    (1, 1, 9000, 8, 1, 128, None, 0, [9001]),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("case", FEW)
+def test_window_attention_few_rows(rt, case, dtype):
+    b, new, cache, heads, kv, d, window, sinks, lens = case
+    q, k, v = attention_inputs(b, new, cache, heads, kv, d, dtype, seed=cache)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    ck = window_kernel(rt, b, new, cache, heads, kv, d, window, sinks, dtype)
+    out = ck(q, k, v, lengths)
+    assert out.shape == q.shape and out.dtype == q.dtype
+    check_attention(out, q, k, v, lengths, window, sinks, dtype, 2.0 ** -16)
+    assert torch.equal(out, ck(q, k, v, lengths))
+
+
+@pytest.mark.parametrize("ranks,parts", [(1, 1), (2, 1), (8, 1), (1, 3), (4, 5), (8, 7)])
+def test_window_attention_splits(ranks, parts):
+    """Clusters and parts, with requests shorter than the split."""
+    b, new, cache, heads, kv, d = 3, 2, 700, 8, 2, 64
+    tuned = MoltenRuntime(tune={"window": {"ranks": ranks, "parts": parts}})
+    ck = window_kernel(tuned, 1, 1, 16, heads, kv, d, 300, 4, "bfloat16")
+    q, k, v = attention_inputs(b, new, cache, heads, kv, d, "bfloat16", seed=1)
+    lengths = torch.tensor([700, 20, 0], dtype=torch.int32, device=DEV)
+    check_attention(ck(q, k, v, lengths), q, k, v, lengths, 300, 4, "bfloat16", 2.0 ** -16)
+
+
+@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), torch.finfo(torch.bfloat16).min])
+def test_window_attention_ignores_unseen_keys(rt, new, bad):
+    """Whatever stands behind a request's length, before its window, or ahead
+    of a query does not reach it."""
+    b, cache, heads, kv, d, window, sinks = 2, 120, 8, 2, 64, 40, 3
+    q, k, v = attention_inputs(b, new, cache, heads, kv, d, "bfloat16", seed=2)
+    lengths = torch.tensor([97, 60], dtype=torch.int32, device=DEV)
+    seen = seen_mask(lengths, new, cache, window, sinks)
+    unseen = ~seen.any(1)
+    k[unseen], v[unseen] = bad, bad
+    ck = window_kernel(rt, b, new, cache, heads, kv, d, window, sinks, "bfloat16")
+    out = ck(q, k, v, lengths)
+    check_attention(out, q, k, v, lengths, window, sinks, "bfloat16", 2.0 ** -16)
+    if new > 1:
+        # the newest value: only the last query may notice
+        v2 = v.clone()
+        v2[torch.arange(b, device=DEV), lengths.long() - 1] = bad
+        got = ck(q, k, v2, lengths)
+        # (the same sums in another order for the rows that share the tile)
+        check_attention(got[:, :-1], q[:, :-1], k, v, lengths - 1, window, sinks, "bfloat16", 2.0 ** -16)
+        if bad != bad or bad == float("inf"):
+            assert not bool(torch.isfinite(got[:, -1]).any())
+
+
+def test_window_attention_views_and_scale(rt):
+    """q, k, v out of one fused tensor; caches laid out [batch, heads, seq, d];
+    a given scale; large scores."""
+    b, new, heads, kv, d, cache = 2, 2, 8, 4, 64, 90
+    fused = torch.randn(b, new, heads + 2 * kv, d, generator=gen_of(3), device=DEV).to(torch.float16)
+    q = fused[:, :, :heads] * 4
+    kc = torch.randn(b, kv, cache + 6, d, generator=gen_of(4), device=DEV).to(torch.float16)
+    vc = torch.randn(b, kv, cache + 6, d, generator=gen_of(5), device=DEV).to(torch.float16)
+    k, v = kc[:, :, 6:].transpose(1, 2), vc[:, :, 6:].transpose(1, 2)
+    lengths = torch.tensor([90, 31], dtype=torch.int32, device=DEV)
+    ck = window_kernel(rt, b, new, cache, heads, kv, d, 25, 1, "float16", scale=1.5)
+    out = ck(fused[:, :, :heads] * 4, k, v, lengths)
+    check_attention(out, q, k, v, lengths, 25, 1, "float16", 2.0 ** -16, scale=1.5)
+    full = torch.full((b,), cache, dtype=torch.int32, device=DEV)
+    none = window_kernel(rt, b, new, cache, heads, kv, d, None, 0, "float16", lengths=False)
+    check_attention(none(q, k, v), q, k, v, full, None, 0, "float16", 2.0 ** -16)
