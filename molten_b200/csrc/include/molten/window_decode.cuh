@@ -5,12 +5,15 @@
 //   over the keys it sees, 0 if it sees none.
 //
 // For single tokens and a few speculated ones: the rows of a key head (nq
-// queries times the heads that share it, at most 16 MT) fit one or two MMA
-// row tiles, and each key and value is used only that often.  Bound by HBM:
-// the keys and values that any query sees, read once.  So loads decide and
-// the products run on mma.sync m16n8k16, whose S accumulators are the A
-// operand of P V as they stand (tcgen05 would want 128 rows and P written
-// back to TMEM for a result that is mostly padding).
+// queries times the heads that share it) number 8 NB at most, and each key
+// and value is used only that often.  Bound by HBM: the keys and values that
+// any query sees, read once.  The products run on mma.sync m16n8k16 (tcgen05
+// would want 128 rows, and P written back to TMEM, for a result that is
+// mostly padding) in the orientation whose narrow side is the rows: S^T = K
+// Q^T and O^T = V^T P^T, with keys and head dims as the 16-row operands.  (With
+// the rows as the 16-row operand half of every MMA was padding, and MMAs, not
+// loads, bounded a warp: 1.0 us a tile.)  The S^T accumulators become the P^T
+// operand by an 8 x 8 transposition (movmatrix).
 //
 // A warp owns tiles of 16 keys: it copies them with 16-byte cp.async into a
 // ring of its own (no barrier between warps; STAGES - 1 tiles in flight),
@@ -123,10 +126,47 @@ struct WindowSpan {
   }
 };
 
-// DP: dim padded to 64 or 128.
-template <int DP, int MT, int WARPS, int STAGES>
+// z: (x, y, maximum, sum) of one share of a row's keys, joined with another's.
+__device__ __forceinline__ void wd_join(float4& z, const float4& w) {
+  if (w.z == -INFINITY && w.w == 0.0f) return;       // saw no key
+  const float mn = fmaxf(z.z, w.z);
+  const float f0 = fast_exp2(z.z - mn), f1 = fast_exp2(w.z - mn);
+  z.w = z.w * f0 + w.w * f1;
+  z.x = z.x * f0 + w.x * f1;
+  z.y = z.y * f0 + w.y * f1;
+  z.z = mn;
+}
+
+// Columns d and d + 1 of row r: the output, or the part's share of it.
+template <typename OT>
+__device__ __forceinline__ void window_store(const WindowArgs& a, int b, int h, int item, int part,
+                                             int rows, int r, int d, const float4& z) {
+  if (a.parts == 1) {
+    const float inv = z.w == 0.0f ? 0.0f : 1.0f / z.w;
+    const int q = r / a.per, hd = h * a.per + r % a.per;
+    OT* dst = static_cast<OT*>(a.out) +
+              (((long long)b * a.nq + q) * (a.kv_heads * a.per) + hd) * a.dim + d;
+    Slot<OT, 2> so;
+    const float f[2] = {z.x * inv, z.y * inv};
+    pack_slot<OT, 2>(so, f);
+    *reinterpret_cast<Slot<OT, 2>*>(dst) = so;
+  } else {
+    float* dst = a.part + (((long long)item * a.parts + part) * rows + r) * (a.dim + 2);
+    *reinterpret_cast<float2*>(dst + d) = make_float2(z.x, z.y);
+    if (d == 0) *reinterpret_cast<float2*>(dst + a.dim) = make_float2(z.z, z.w);
+  }
+}
+
+__device__ __forceinline__ uint32_t wd_transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// DP: dim padded to 64 or 128.  NB: blocks of 8 rows.
+template <int DP, int NB, int WARPS, int STAGES>
 struct WindowDecodeLayout {
-  static constexpr int TILE = 16, ROWS = 16 * MT;
+  static constexpr int TILE = 16, ROWS = 8 * NB;
   static constexpr int KV_BYTES = TILE * DP * 2;     // one tile of K or V
   static constexpr int RING = WARPS * STAGES * 2 * KV_BYTES;
   static constexpr int OUT = WARPS * ROWS * (DP + 4) * 4;       // merge area (over the ring)
@@ -135,10 +175,10 @@ struct WindowDecodeLayout {
   static constexpr int SMEM = (RING > OUT ? RING : OUT) + STAT + PROB;
 };
 
-template <typename T, typename OT, int DP, int MT, int WARPS, int STAGES>
+template <typename T, typename OT, int DP, int NB, int WARPS, int STAGES>
 __device__ __forceinline__ void window_decode(const WindowArgs& a, uint8_t* raw) {
-  typedef WindowDecodeLayout<DP, MT, WARPS, STAGES> L;
-  constexpr int TILE = L::TILE, ROWS = L::ROWS, NK = DP / 16, ND = DP / 8, PITCH = DP * 2;
+  typedef WindowDecodeLayout<DP, NB, WARPS, STAGES> L;
+  constexpr int TILE = L::TILE, ROWS = L::ROWS, NK = DP / 16, PITCH = DP * 2;
   constexpr int CHUNKS = DP / 8;                     // 16-byte chunks of a row
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int g = lane / 4, t = lane % 4;
@@ -146,7 +186,35 @@ __device__ __forceinline__ void window_decode(const WindowArgs& a, uint8_t* raw)
   const int part = rest0 % a.parts, item = rest0 / a.parts;
   const int b = item / a.kv_heads, h = item - b * a.kv_heads;
   const int rows = a.nq * a.per;
+  if (a.ranks > 1)                                   // every CTA of the cluster has started: waited
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");     // for before the merge
+
+  // Q^T as B operands (row n of a block is lane group g); row r is query
+  // r / per, head r % per.  A lane keeps statistics of rows 2 t, 2 t + 1.
+  uint32_t qb[NB][NK][2];
+  int pos[NB][2];                                    // where those two rows stand
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = n * 8 + 2 * t + e;
+      pos[n][e] = r < rows ? r / a.per : -0x40000000;
+    }
+    const int r = n * 8 + g, i = min(r / a.per, a.nq - 1);
+    const T* src = static_cast<const T*>(a.q) + b * a.q_b + (long long)i * a.q_s
+                   + (long long)(h * a.per + r % a.per) * a.q_h;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int d = k * 16 + c * 8 + 2 * t;
+        qb[n][k][c] = r < rows && d < a.dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+      }
+    }
+  }
   const WindowSpan span = WindowSpan::of<TILE>(a, b);
+#pragma unroll
+  for (int n = 0; n < NB; ++n) { pos[n][0] += span.first; pos[n][1] += span.first; }
   // tiles of this CTA: an equal share of the item's, in order
   const int shares = a.ranks * a.parts, share = part * a.ranks + rank;
   const int t0 = (int)((long long)span.tiles * share / shares);
@@ -159,20 +227,30 @@ __device__ __forceinline__ void window_decode(const WindowArgs& a, uint8_t* raw)
   float* stat = reinterpret_cast<float*>(raw + (L::RING > L::OUT ? L::RING : L::OUT));
   float* prob = stat + WARPS * ROWS * 2 + warp * ROWS * TILE;
 
+  // a lane copies chunk cc of every RSTEP-th row of a tile
+  constexpr int RSTEP = 32 / CHUNKS;
+  const int cc = lane % CHUNKS, cr = lane / CHUNKS;
+  const bool col = cc * 8 < a.dim;                   // chunks past the head dim are zero-filled
+  const T* kl = kb + (col ? cc * 8 : 0);
+  const T* vl = vb + (col ? cc * 8 : 0);
   auto copy_tile = [&](int tile, int stage) {
     if (tile < t1) {
-      const int key0 = span.key0<TILE>(tile);
+      const int key0 = span.key0<TILE>(tile) + cr;
       const uint32_t dst = ring_s + stage * (2 * L::KV_BYTES);
+      const T* ks = kl + (long long)key0 * a.k_s;
+      const T* vs = vl + (long long)key0 * a.v_s;
+      const int last = key0 - cr + TILE - 1;
+      const bool full = last < span.len && (key0 - cr >= span.start || last < a.sinks);
 #pragma unroll
-      for (int i = 0; i < TILE * CHUNKS / 32; ++i) {
-        const int c = (i * 32 + lane) % CHUNKS, r = (i * 32 + lane) / CHUNKS;
-        const int j = key0 + r;
-        const bool in = span.any(a, j) && c * 8 < a.dim;
-        const long long jj = in ? j : 0;
-        const int cc = in ? c * 8 : 0;
-        const uint32_t off = r * PITCH + ((c ^ (r & 7)) << 4);
-        wd_copy16(dst + off, kb + jj * a.k_s + cc, in);
-        wd_copy16(dst + L::KV_BYTES + off, vb + jj * a.v_s + cc, in);
+      for (int i = 0; i < TILE / RSTEP; ++i) {
+        const int r = cr + i * RSTEP;
+        const bool in = col && (full || span.any(a, key0 + i * RSTEP));
+        const uint32_t off = r * PITCH + ((cc ^ (r & 7)) << 4);
+        // (nothing is read where nothing is wanted; the address stays valid)
+        wd_copy16(dst + off, in ? ks : kb, in);
+        wd_copy16(dst + L::KV_BYTES + off, in ? vs : vb, in);
+        ks += RSTEP * a.k_s;
+        vs += RSTEP * a.v_s;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -180,38 +258,15 @@ __device__ __forceinline__ void window_decode(const WindowArgs& a, uint8_t* raw)
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) copy_tile(t0 + warp + s * WARPS, s);
 
-  // the rows of q as A operands; row r is query r / per, head r % per
-  uint32_t qa[MT][NK][4];
-  int pos[MT][2];                                    // where rows g and g + 8 stand
+  float o[NB][NK][4], mx[NB][2], sum[NB][2];         // O^T: dims 16 i + g, + 8; rows 2 t, 2 t + 1
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int n = 0; n < NB; ++n) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = m * 16 + e * 8 + g;
-      const int i = r / a.per;
-      pos[m][e] = r < rows ? span.first + i : -1;
-      const T* src = static_cast<const T*>(a.q) + b * a.q_b + (long long)min(i, a.nq - 1) * a.q_s
-                     + (long long)(h * a.per + r % a.per) * a.q_h;
+    for (int e = 0; e < 2; ++e) { mx[n][e] = -INFINITY; sum[n][e] = 0.0f; }
 #pragma unroll
-      for (int k = 0; k < NK; ++k) {
+    for (int i = 0; i < NK; ++i)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int d = k * 16 + c * 8 + 2 * t;
-          qa[m][k][c * 2 + e] = r < rows && d < a.dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
-        }
-      }
-    }
-  }
-
-  float o[MT][ND][4], mx[MT][2], sum[MT][2];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) { mx[m][e] = -INFINITY; sum[m][e] = 0.0f; }
-#pragma unroll
-    for (int n = 0; n < ND; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[m][n][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
   }
 
   int stage = 0;
@@ -226,121 +281,116 @@ __device__ __forceinline__ void window_decode(const WindowArgs& a, uint8_t* raw)
     __syncwarp();
     const int key0 = span.key0<TILE>(tile);
     const uint32_t ks = ring_s + stage * (2 * L::KV_BYTES), vs = ks + L::KV_BYTES;
-    const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
+    const uint8_t* vt = ring + stage * (2 * L::KV_BYTES) + L::KV_BYTES;
 
-    float s[MT][2][4];
+    // S^T: keys g, g + 8; rows 2 t, 2 t + 1; even and odd steps in chains of their own
+    float s[NB][4], s2[NB][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[m][n][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) { s[n][e] = 0.0f; s2[n][e] = 0.0f; }
+    const int kr = (lane & 7) + (((lane >> 3) & 1) << 3), kc = lane >> 4;
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
       uint32_t kf[4];
       wd_ldmatrix<false>(ks + kr * PITCH + (((2 * k + kc) ^ (kr & 7)) << 4), kf);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        wd_mma<T>(s[m][0], qa[m][k], kf[0], kf[1]);
-        wd_mma<T>(s[m][1], qa[m][k], kf[2], kf[3]);
-      }
+      for (int n = 0; n < NB; ++n) wd_mma<T>(k % 2 ? s2[n] : s[n], kf, qb[n][k][0], qb[n][k][1]);
     }
 
     // keys that every query sees need no mask
     const bool whole = key0 + TILE - 1 <= span.first &&
                        (a.window < 0 || key0 > span.last - a.window || key0 + TILE <= a.sinks);
-    uint32_t ph[MT][4], pl[MT][4];
+    uint32_t ph[NB][2], pl[NB][2];
+    float fix[NB][2];
+    bool moved = false;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    for (int n = 0; n < NB; ++n) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {                  // rows g, g + 8
-        float x[4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int j = key0 + n * 8 + 2 * t + c;
-            const float v = s[m][n][e * 2 + c] * a.scale_log2;
-            x[n * 2 + c] = whole || span.sees(a, pos[m][e], j) ? v : -INFINITY;
-          }
-        float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float mn = fmaxf(mx[m][e], top);
+      for (int e = 0; e < 2; ++e) {                  // rows 2 t, 2 t + 1
+        float x0 = (s[n][e] + s2[n][e]) * a.scale_log2;
+        float x1 = (s[n][e + 2] + s2[n][e + 2]) * a.scale_log2;
+        if (!whole) {
+          if (!span.sees(a, pos[n][e], key0 + g)) x0 = -INFINITY;
+          if (!span.sees(a, pos[n][e], key0 + g + 8)) x1 = -INFINITY;
+        }
+        float top = fmaxf(x0, x1);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const float mn = fmaxf(mx[n][e], top);
         const float base = mn == -INFINITY ? 0.0f : mn;
-        const float fix = fast_exp2(mx[m][e] - base);
-        if (__any_sync(0xffffffffu, mn != mx[m][e])) {
-          sum[m][e] *= fix;
-#pragma unroll
-          for (int n = 0; n < ND; ++n) { o[m][n][e * 2] *= fix; o[m][n][e * 2 + 1] *= fix; }
-        }
-        mx[m][e] = mn;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          x[q] = fast_exp2(x[q] - base);
-          sum[m][e] += x[q];
-          s[m][q / 2][e * 2 + q % 2] = x[q];
-        }
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint32_t hi = wd_pack<T>(x[2 * n], x[2 * n + 1]);
-          const float2 hf = wd_unpack<T>(hi);
-          ph[m][n * 2 + e] = hi;
-          pl[m][n * 2 + e] = wd_pack<T>(x[2 * n] - hf.x, x[2 * n + 1] - hf.y);
-        }
+        fix[n][e] = fast_exp2(mx[n][e] - base);
+        moved |= mn != mx[n][e];
+        mx[n][e] = mn;
+        x0 = fast_exp2(x0 - base);
+        x1 = fast_exp2(x1 - base);
+        sum[n][e] = sum[n][e] * fix[n][e] + (x0 + x1);
+        s[n][e] = x0;
+        s[n][e + 2] = x1;
       }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {                  // keys 0..7, 8..15
+        const uint32_t hi = wd_pack<T>(s[n][2 * c], s[n][2 * c + 1]);
+        const float2 hf = wd_unpack<T>(hi);
+        ph[n][c] = wd_transpose(hi);
+        pl[n][c] = wd_transpose(wd_pack<T>(s[n][2 * c] - hf.x, s[n][2 * c + 1] - hf.y));
+      }
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          o[n][i][0] *= fix[n][0]; o[n][i][1] *= fix[n][1];
+          o[n][i][2] *= fix[n][0]; o[n][i][3] *= fix[n][1];
+        }
     }
 
     bool odd = false;                                // an infinity or NaN that P = 0 would meet
     if (a.nq > 1 && !whole) {
 #pragma unroll 1
       for (int i = lane; i < L::KV_BYTES / 4; i += 32) {
-        const uint32_t u = *reinterpret_cast<const uint32_t*>(ring + stage * (2 * L::KV_BYTES) +
-                                                              L::KV_BYTES + 4 * i);
-        const float2 f = wd_unpack<T>(u);
+        const float2 f = wd_unpack<T>(*reinterpret_cast<const uint32_t*>(vt + 4 * i));
         odd |= !isfinite(f.x) || !isfinite(f.y);
       }
       odd = __any_sync(0xffffffffu, odd);
     }
     if (!odd) {
-      const int vr = (lane & 7) + (((lane >> 3) & 1) << 3), vc = lane >> 4;
+      const int vm = lane >> 3, vr = (lane & 7) + ((vm >> 1) << 3), vc = vm & 1;
 #pragma unroll
-      for (int n = 0; n < ND / 2; ++n) {
+      for (int i = 0; i < NK; ++i) {
         uint32_t vf[4];
-        wd_ldmatrix<true>(vs + vr * PITCH + (((2 * n + vc) ^ (vr & 7)) << 4), vf);
+        wd_ldmatrix<true>(vs + vr * PITCH + (((2 * i + vc) ^ (vr & 7)) << 4), vf);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          wd_mma<T>(o[m][2 * n], ph[m], vf[0], vf[1]);
-          wd_mma<T>(o[m][2 * n + 1], ph[m], vf[2], vf[3]);
-          wd_mma<T>(o[m][2 * n], pl[m], vf[0], vf[1]);
-          wd_mma<T>(o[m][2 * n + 1], pl[m], vf[2], vf[3]);
+        for (int n = 0; n < NB; ++n) {
+          wd_mma<T>(o[n][i], vf, ph[n][0], ph[n][1]);
+          wd_mma<T>(o[n][i], vf, pl[n][0], pl[n][1]);
         }
       }
     } else {
       // row by row, over the keys each row sees
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            prob[(m * 16 + g + (e >> 1) * 8) * TILE + n * 8 + 2 * t + (e & 1)] = s[m][n][e];
+        for (int e = 0; e < 4; ++e)
+          prob[(n * 8 + 2 * t + (e & 1)) * TILE + g + (e >> 1) * 8] = s[n][e];
       __syncwarp();
 #pragma unroll 1
       for (int kk = 0; kk < TILE; ++kk) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        for (int i = 0; i < NK; ++i) {
+          const T* row = reinterpret_cast<const T*>(vt + kk * PITCH);
+          const float v0 = to_f32(row[(((2 * i) ^ (kk & 7)) << 3) + g]);
+          const float v1 = to_f32(row[(((2 * i + 1) ^ (kk & 7)) << 3) + g]);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float p = prob[(m * 16 + g + e * 8) * TILE + kk];
-            if (!span.sees(a, pos[m][e], key0 + kk)) continue;
+          for (int n = 0; n < NB; ++n) {
 #pragma unroll
-            for (int n = 0; n < ND; ++n) {
-              const uint32_t u = *reinterpret_cast<const uint32_t*>(
-                  ring + stage * (2 * L::KV_BYTES) + L::KV_BYTES + kk * PITCH + ((n ^ (kk & 7)) << 4) + 4 * t);
-              const float2 f = wd_unpack<T>(u);
-              o[m][n][e * 2] += p * f.x;
-              o[m][n][e * 2 + 1] += p * f.y;
+            for (int e = 0; e < 2; ++e) {
+              if (!span.sees(a, pos[n][e], key0 + kk)) continue;
+              const float p = prob[(n * 8 + 2 * t + e) * TILE + kk];
+              o[n][i][e] += p * v0;
+              o[n][i][e + 2] += p * v1;
             }
           }
         }
@@ -356,74 +406,72 @@ __device__ __forceinline__ void window_decode(const WindowArgs& a, uint8_t* raw)
   float* area = reinterpret_cast<float*>(raw);
   constexpr int OP = DP + 4;                         // pitch (rows on different banks)
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int n = 0; n < NB; ++n) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float total = sum[m][e];
-      total += __shfl_xor_sync(0xffffffffu, total, 1);
-      total += __shfl_xor_sync(0xffffffffu, total, 2);
-      const int r = m * 16 + e * 8 + g;
-      if (t == 0) {
-        stat[(warp * ROWS + r) * 2] = mx[m][e];
+      float total = sum[n][e];
+      total += __shfl_xor_sync(0xffffffffu, total, 4);
+      total += __shfl_xor_sync(0xffffffffu, total, 8);
+      total += __shfl_xor_sync(0xffffffffu, total, 16);
+      const int r = n * 8 + 2 * t + e;
+      if (r >= rows) continue;
+      if (g == 0) {
+        stat[(warp * ROWS + r) * 2] = mx[n][e];
         stat[(warp * ROWS + r) * 2 + 1] = total;
       }
 #pragma unroll
-      for (int n = 0; n < ND; ++n)
-        *reinterpret_cast<float2*>(&area[(warp * ROWS + r) * OP + n * 8 + 2 * t]) =
-            make_float2(o[m][n][e * 2], o[m][n][e * 2 + 1]);
+      for (int i = 0; i < NK; ++i) {
+        area[(warp * ROWS + r) * OP + i * 16 + g] = o[n][i][e];
+        area[(warp * ROWS + r) * OP + i * 16 + g + 8] = o[n][i][e + 2];
+      }
     }
   }
-  if (a.ranks > 1)
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  else
-    __syncthreads();
+  __syncthreads();
 
-  // the ranks share the (row, 2 columns) pairs; each joins every warp of
-  // every rank, in order
-  const uint32_t area_s = wd_smem(area), stat_s = wd_smem(stat);
+  // a (row, 2 columns) pair a thread: join the CTA's warps in order; with a
+  // cluster, push the result to the rank that owns the pair
   const int pairs = a.dim / 2, total = rows * pairs;
-  for (int i = rank * (WARPS * 32) + threadIdx.x; i < total; i += a.ranks * (WARPS * 32)) {
+  const int own = (total + a.ranks - 1) / a.ranks;   // pairs of one rank
+  float4* inbox = reinterpret_cast<float4*>(raw + L::SMEM);      // [rank][own]
+  if (a.ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+#pragma unroll 1
+  for (int i = threadIdx.x; i < total; i += WARPS * 32) {
     const int r = i / pairs, d = (i - r * pairs) * 2;
-    float M = -INFINITY, S = 0.0f, x = 0.0f, y = 0.0f;
-    for (int c = 0; c < a.ranks; ++c) {
-      uint32_t area_c = area_s, stat_c = stat_s;
-      if (a.ranks > 1) {
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(area_c) : "r"(area_s), "r"(c));
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(stat_c) : "r"(stat_s), "r"(c));
-      }
+    float2 ms[WARPS], v[WARPS];
+    float4 z = make_float4(0.0f, 0.0f, -INFINITY, 0.0f);
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        float2 ms, v;
-        asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];"
-                     : "=f"(ms.x), "=f"(ms.y) : "r"(stat_c + 8u * (uint32_t)(w * ROWS + r)));
-        asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];"
-                     : "=f"(v.x), "=f"(v.y) : "r"(area_c + 4u * (uint32_t)((w * ROWS + r) * OP + d)));
-        if (ms.x == -INFINITY && ms.y == 0.0f) continue;         // saw no key
-        const float mn = fmaxf(M, ms.x);
-        const float f0 = fast_exp2(M - mn), f1 = fast_exp2(ms.x - mn);
-        S = S * f0 + ms.y * f1;
-        x = x * f0 + v.x * f1;
-        y = y * f0 + v.y * f1;
-        M = mn;
-      }
+    for (int w = 0; w < WARPS; ++w) {
+      ms[w] = *reinterpret_cast<const float2*>(&stat[(w * ROWS + r) * 2]);
+      v[w] = *reinterpret_cast<const float2*>(&area[(w * ROWS + r) * OP + d]);
     }
-    if (a.parts == 1) {
-      const float inv = S == 0.0f ? 0.0f : 1.0f / S;
-      const int q = r / a.per, hd = h * a.per + r % a.per;
-      OT* dst = static_cast<OT*>(a.out) +
-                (((long long)b * a.nq + q) * (a.kv_heads * a.per) + hd) * a.dim + d;
-      Slot<OT, 2> so;
-      const float f[2] = {x * inv, y * inv};
-      pack_slot<OT, 2>(so, f);
-      *reinterpret_cast<Slot<OT, 2>*>(dst) = so;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) wd_join(z, make_float4(v[w].x, v[w].y, ms[w].x, ms[w].y));
+    if (a.ranks == 1) {
+      window_store<OT>(a, b, h, item, part, rows, r, d, z);
     } else {
-      float* dst = a.part + (((long long)item * a.parts + part) * rows + r) * (a.dim + 2);
-      *reinterpret_cast<float2*>(dst + d) = make_float2(x, y);
-      if (d == 0) *reinterpret_cast<float2*>(dst + a.dim) = make_float2(M, S);
+      const int owner = i / own;
+      uint32_t at = wd_smem(inbox + rank * own + (i - owner * own));
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(at), "r"(owner));
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};"
+                   :: "r"(at), "f"(z.x), "f"(z.y), "f"(z.z), "f"(z.w) : "memory");
     }
   }
-  if (a.ranks > 1)                                   // peers may still read this CTA's rows
+  if (a.ranks > 1) {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+#pragma unroll 1
+    for (int i = threadIdx.x; i < own && rank * own + i < total; i += WARPS * 32) {
+      float4 x[8];                                   // at most 8 ranks
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < a.ranks) x[c] = inbox[c * own + i];
+      float4 z = make_float4(0.0f, 0.0f, -INFINITY, 0.0f);
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < a.ranks) wd_join(z, x[c]);
+      const int at = rank * own + i, r = at / pairs, d = (at - r * pairs) * 2;
+      window_store<OT>(a, b, h, item, part, rows, r, d, z);
+    }
+  }
 }
 
 // Join the parts of every row: a warp per (item, row).

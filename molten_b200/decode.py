@@ -35,7 +35,7 @@ SMEM_SM = 228 * 1024
 
 WINDOW_MAX_DIM = 128
 WINDOW_FEW_ROWS = 32              # rows of a key head up to which the few-row kernel runs
-WINDOW_WARPS, WINDOW_STAGES, WINDOW_TILE = 4, 3, 16
+WINDOW_STAGES, WINDOW_TILE = 3, 16
 
 ROPE_MAX_AXES = 4
 ROPE_MAX_DIM = 1024
@@ -281,6 +281,33 @@ def _plan_rope(op, sk, tune) -> dict:
             "flops": 3 * tokens * heads * d}
 
 
+def _split_window(items: int, tiles: int, most_warps: int):
+    """(ranks, parts, warps): how the keys of an item (``tiles`` tiles of 16)
+    are spread over the CTAs of a cluster, over clusters, and over the warps
+    of a CTA.  An SM holds 8 warps; a CTA costs about 4 us to fill and drain
+    and 1.4 us per tile of each warp, a join of parts 2.5 us and more
+    (measured with head dim 128, 4 rows: 8 items of 66 tiles 6.6 us on 8 CTAs
+    of 8 warps each, 12-17 us on one or two; 512 items of 257 tiles 154 us on
+    one CTA of 4 warps each, 170 of 2, 161 of 8; 8 items of 4096 tiles 54 us
+    on 4 x 8 CTAs of 4 warps, 114 on 8; 1 item of 512 tiles 11.5 us on 4 x 8
+    CTAs, 18 on 8).  CTAs of 8 warps in large numbers leave SMs without a
+    place for a whole cluster."""
+    best = None
+    for warps in (4, 8, 2):
+        slots = SMS * (8 // warps)
+        for ranks in (1, 2, 4, 8):
+            for parts in (1, 2, 4) if ranks == 8 else (1,):
+                ctas = items * ranks * parts
+                if warps > most_warps or warps == 8 and ranks > 1 and ctas > 64:
+                    continue
+                per_warp = -(-tiles // (ranks * parts * warps))
+                waves = 1.0 if ctas <= slots else ctas / slots + 0.15
+                cost = waves * (4.0 + 1.4 * per_warp) + (2.5 + 0.2 * parts if parts > 1 else 0.0)
+                if best is None or cost < best[0] - 1e-9:
+                    best = (cost, ranks, parts, warps)
+    return best[1:]
+
+
 def _plan_window(op, sk, tune) -> dict:
     q, k, v = sk.operands[:3]
     _need(q.dtype == k.dtype == v.dtype and q.dtype in ("bfloat16", "float16"),
@@ -306,21 +333,25 @@ def _plan_window(op, sk, tune) -> dict:
     c["flops"] = 4 * batch * heads * new * seen * dim
     _need(rows <= WINDOW_FEW_ROWS, "window_attention: too many rows")
     tiles = -(-span // WINDOW_TILE) + 1
-    # two CTAs an SM: split the keys of an item over a cluster, and past that
-    # over parts joined by a second kernel, as far as every warp has a tile
-    want = max(1, min(-(-2 * SMS // max(1, items)), tiles // WINDOW_WARPS))
-    ranks = 1
-    while ranks < 8 and 2 * ranks <= want:
-        ranks *= 2
-    parts = max(1, want // ranks) if ranks == 8 else 1
+    nb = 1 if rows <= 8 else 2 if rows <= 16 else 4
+    ranks, parts, warps = _split_window(items, tiles, 8 if nb == 1 else 4)
     ranks, parts = int(o.get("ranks") or ranks), int(o.get("parts") or parts)
-    mt = 1 if rows <= 16 else 2
-    warps, stages = int(o.get("warps") or WINDOW_WARPS), int(o.get("stages") or WINDOW_STAGES)
-    ring = warps * stages * 2 * WINDOW_TILE * c["dp"] * 2
-    area = warps * 16 * mt * (c["dp"] + 4) * 4
-    smem = max(ring, area) + warps * 16 * mt * (8 + WINDOW_TILE * 4)
-    c.update(kind="few", mt=mt, ranks=ranks, parts=parts, items=items, rows=rows, warps=warps,
-             stages=stages, block=32 * warps, smem=smem)
+    warps = int(o.get("warps") or warps)
+    # what the ranks of a cluster send one another: 16 bytes per 2 columns
+    inbox = -(-rows * (dim // 2) // ranks) * ranks * 16 if ranks > 1 else 0
+    area = warps * 8 * nb * (c["dp"] + 4) * 4
+    # 8 warps an SM, twice that where a tile is half as wide; a third stage
+    # where the SM's shared memory holds it
+    min_ctas = max(1, min(4, 8 // warps)) * (2 if c["dp"] == 64 and nb < 4 else 1)
+    for stages in (WINDOW_STAGES, WINDOW_STAGES - 1):
+        stages = int(o.get("stages") or stages)
+        ring = warps * stages * 2 * WINDOW_TILE * c["dp"] * 2
+        smem = max(ring, area) + warps * 8 * nb * (8 + WINDOW_TILE * 4)
+        if (smem + inbox + 1024) * min_ctas <= SMEM_SM:
+            break
+    _need(smem + inbox <= SMEM_LIMIT, "window_attention: the tile does not fit shared memory")
+    c.update(kind="few", nb=nb, ranks=ranks, parts=parts, items=items, rows=rows, warps=warps,
+             stages=stages, min_ctas=min_ctas, block=32 * warps, smem=smem, smem_launch=smem + inbox)
     return c
 
 
@@ -388,16 +419,16 @@ extern "C" __global__ void __launch_bounds__(1024) {name}(const __grid_constant_
 def _emit_window(sk, name):
     c = sk.config
     t, ot = DTYPE_CTYPE[sk.operands[0].dtype], DTYPE_CTYPE[sk.outputs[0].dtype]
-    lay = f"{c['dp']}, {c['mt']}, {c['warps']}, {c['stages']}"
+    lay = f"{c['dp']}, {c['nb']}, {c['warps']}, {c['stages']}"
     return f"""// Molten sm_100a window attention, few query rows: {name}
-// {sk.operands[0].dtype}, head dim up to {c['dp']}, up to {16 * c['mt']} rows
+// {sk.operands[0].dtype}, head dim up to {c['dp']}, up to {8 * c['nb']} rows
 #include "molten/window_decode.cuh"
 
 using namespace molten;
 
 static_assert(WindowDecodeLayout<{lay}>::SMEM == {c['smem']}, "the launch's dynamic shared memory");
 
-extern "C" __global__ void __launch_bounds__({c['block']}, 2) {name}(const __grid_constant__ WindowArgs args) {{
+extern "C" __global__ void __launch_bounds__({c['block']}, {c['min_ctas']}) {name}(const __grid_constant__ WindowArgs args) {{
   extern __shared__ __align__(128) uint8_t smem_raw[];
   pdl_enter();
   window_decode<{t}, {ot}, {lay}>(args, smem_raw);

@@ -139,7 +139,7 @@ def _launch_window(spec, sk, entry, ins, out, device, stream):
         part = torch.empty(c["items"] * c["parts"] * c["rows"] * (c["dim"] + 2),
                            dtype=torch.float32, device=q.device)
         a.part = part.data_ptr()
-    mod.launch(entry, _cfg(grid, c["block"], c["ranks"], c["smem"]), a, stream)
+    mod.launch(entry, _cfg(grid, c["block"], c["ranks"], c["smem_launch"]), a, stream)
     if part is not None:
         mod.launch(entry + b"_join", _cfg(-(-c["items"] * c["rows"] // 4), 128), a, stream)
 
