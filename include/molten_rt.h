@@ -149,6 +149,27 @@ typedef struct molten_window_args {
   int reserved;
 } molten_window_args;
 
+/* Parameter block of the window-attention kernels for many query rows
+ * (device side: molten::WindowTcArgs in molten/window_sm100.cuh).  Tensor maps
+ * from molten_encode_tma_4d: q [dim, heads, nq, batch] in boxes of {64, per,
+ * positions, 1}, k and v [dim, kv_heads, cache, batch] in boxes of {64, 1, 128,
+ * 1}.  positions = 128 / per; blocks = ceil(nq / (2 positions)); the grid is
+ * at most one CTA per SM. */
+typedef struct molten_window_tc_args {
+  MOLTEN_ALIGN64 unsigned char tmap_q[128];
+  MOLTEN_ALIGN64 unsigned char tmap_k[128];
+  MOLTEN_ALIGN64 unsigned char tmap_v[128];
+  const void* v;
+  const int* lengths;            /* [batch] valid keys, or null: cache */
+  void* out;                     /* [batch, nq, heads, dim] contiguous */
+  int* status;
+  long long v_b, v_s, v_h;       /* strides of v in elements */
+  int batch, nq, cache, kv_heads, per, dim;
+  int window, sinks;             /* window < 0: every earlier key */
+  float scale_log2;              /* scale * log2(e), positive */
+  int positions, blocks, reserved;
+} molten_window_tc_args;
+
 /* Version of this ABI (major * 100 + minor). */
 int molten_version(void);
 
@@ -207,6 +228,13 @@ int molten_launch(void* mod, const char* kernel, const molten_launch_cfg* cfg,
 int molten_encode_tma_2d(void* tmap, int dtype, const void* base,
                          uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
                          uint32_t box_inner, uint32_t box_outer, int swizzle);
+
+/* Encode a 4-D TMA descriptor (16-bit elements, 128-byte swizzle) for a
+ * tensor of dims[0] contiguous elements and dims[1..3] at strides_bytes[0..2]
+ * (multiples of 16 bytes, not 0), copied in boxes of box[0..3] elements
+ * (box[0] at most 64).  Out-of-range box elements read as zero. */
+int molten_encode_tma_4d(void* tmap, int dtype, const void* base, const uint64_t* dims,
+                         const uint64_t* strides_bytes, const uint32_t* box);
 
 /* Per-device error word that kernels with bounded waits set bits in
  * (allocated on first use, then reused). */

@@ -33,6 +33,8 @@ SIGNATURES = {
     "molten_encode_tma_2d": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_void_p, _c.c_uint64,
                                         _c.c_uint64, _c.c_uint64, _c.c_uint32, _c.c_uint32,
                                         _c.c_int]),
+    "molten_encode_tma_4d": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_void_p, _c.c_void_p,
+                                        _c.c_void_p, _c.c_void_p]),
     "molten_status_word": (_c.c_int, [_c.c_int, _c.POINTER(_c.c_void_p)]),
     "molten_read_status": (_c.c_int, [_c.c_int, _c.POINTER(_c.c_int), _c.c_int]),
     "molten_scores_softmax_bf16_noalloc": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p,
@@ -110,6 +112,20 @@ class WindowArgs(ctypes.Structure):
                    ("parts", ctypes.c_int), ("reserved", ctypes.c_int)])
 
 
+class WindowTcArgs(ctypes.Structure):
+    """molten_window_tc_args / molten::WindowTcArgs (512 bytes, 64-byte aligned
+    on the device side)."""
+    _fields_ = ([(n, ctypes.c_ubyte * 128) for n in ("tmap_q", "tmap_k", "tmap_v")]
+                + [(n, ctypes.c_void_p) for n in ("v", "lengths", "out", "status")]
+                + [(n, ctypes.c_longlong) for n in ("v_b", "v_s", "v_h")]
+                + [(n, ctypes.c_int) for n in ("batch", "nq", "cache", "kv_heads", "per", "dim",
+                                               "window", "sinks")]
+                + [("scale_log2", ctypes.c_float)]
+                + [(n, ctypes.c_int) for n in ("positions", "blocks", "reserved")]
+                + [("tail_", ctypes.c_ubyte * 24)])
+
+
+assert ctypes.sizeof(WindowTcArgs) == 512
 assert ctypes.sizeof(WindowArgs) == 168
 assert ctypes.sizeof(RopePosArgs) == 120
 assert ctypes.sizeof(Q4Args) == 88
@@ -211,6 +227,19 @@ def encode_tma_2d(dtype_code: int, base: int, inner: int, outer: int, row_stride
                                    inner, outer, row_stride_bytes, box_inner, box_outer,
                                    int(swizzle)),
           "encoding a TMA descriptor")
+    return ctypes.string_at(aligned, 128)
+
+
+def encode_tma_4d(dtype_code: int, base: int, dims, strides_bytes, box) -> bytes:
+    """128-byte TMA descriptor of a 4-D tensor of 16-bit elements (128-byte
+    swizzle); ``dims`` from the contiguous one out, ``strides_bytes`` of the
+    other three."""
+    buf = ctypes.create_string_buffer(128 + 64)
+    aligned = (ctypes.addressof(buf) + 63) & ~63
+    check(load_library().molten_encode_tma_4d(
+        ctypes.c_void_p(aligned), dtype_code, ctypes.c_void_p(base),
+        (ctypes.c_uint64 * 4)(*dims), (ctypes.c_uint64 * 3)(*strides_bytes),
+        (ctypes.c_uint32 * 4)(*box)), "encoding a TMA descriptor")
     return ctypes.string_at(aligned, 128)
 
 

@@ -1,0 +1,647 @@
+// Attention over a sliding window and the first keys, many query rows
+// (prompts and chunks), on tcgen05:
+//
+//   query i of request b stands at p = len_b - nq + i and sees key j iff
+//   j <= p and (j > p - window or j < sinks);  o = softmax(q k^T scale) v
+//   over the keys it sees, 0 if it sees none.
+//
+// A work item is a key head of a request and two Q tiles of up to 128 rows;
+// a row is (position, head that shares the key head), so grouped heads fill a
+// tile with fewer positions and the window's edges cost fewer masked
+// products.  The item's key tiles of 128 are those that some row sees: the
+// sinks' and the window's.  Each Q tile has its own S and O in TMEM (S0, S1,
+// O0, O1: 512 columns at head dim 128), P over S:
+//
+//   warp 0       TMA: the Q tiles, then K and V tiles through one ring;
+//   warp 1       TMEM owner, MMA issuer: S = Q K^T (both operands in shared
+//                memory), O += P V with P as the TMEM operand; the two Q tiles
+//                alternate, so one's products run under the other's softmax;
+//   warps 2, 3   clean the V tiles that not every row sees all of (below);
+//   warps 4..7   softmax of Q tile 0 (a thread owns a row), warps 8..11 of
+//                tile 1: S from TMEM, running maximum and sum in fp32, P
+//                rounded to the type of V (the tensor core takes operands of
+//                one type; relative 2^-9 or 2^-12 a weight) back to TMEM.
+//
+// Bound by the tensor core (4 D operations a visible pair) and, next to it, by
+// the EX2 unit: a 128 x 128 tile takes some 1024 cycles of either.  O is
+// rescaled only when a row's maximum has grown by more than 2^8 since the last
+// time: the weights stay below 2^8 and O and the sum share the factor, so
+// nothing is lost, and most rescales (each a round trip of O through
+// registers) never happen.
+//
+// P = 0 times an infinity or NaN is NaN, so V rows that no query of the item
+// sees (behind the length, before the window) are zeroed in shared memory
+// before their MMA, and so are infinities and NaN in rows that only some
+// queries see; an item that had one of those adds it, from global memory, to
+// the outputs of the rows that do see it.
+//
+// Every mbarrier wait is bounded; on timeout the CTA sets a status bit, stops,
+// drains its copies, frees TMEM and returns.
+#pragma once
+
+#include "molten/attn_sm100.cuh"
+
+namespace molten {
+
+struct alignas(64) WindowTcArgs {
+  CUtensorMap tmap_q;              // q [batch, nq, heads, dim], box {64, per, positions, 1}
+  CUtensorMap tmap_k;              // k [batch, cache, kv_heads, dim], box {64, 1, 128, 1}
+  CUtensorMap tmap_v;
+  const void* v;
+  const int* lengths;              // [batch] valid keys, or null: cache
+  void* out;                       // [batch, nq, heads, dim] contiguous
+  int* status;
+  long long v_b, v_s, v_h;         // strides of v in elements
+  int batch, nq, cache, kv_heads, per, dim;
+  int window, sinks;               // window < 0: every earlier key
+  float scale_log2;                // scale * log2(e), positive
+  int positions;                   // positions of one Q tile
+  int blocks;                      // pairs of Q tiles of a request
+  int reserved;
+};
+
+enum WindowTcStatus { kWindowTimeout = 2048 };
+
+// DP: dim padded to 64 or 128.
+template <int DP_, int STAGES_>
+struct WindowTcLayout {
+  static constexpr int DP = DP_, STAGES = STAGES_, DCH = DP / 64, BN = 128;
+  static constexpr int CHUNK = 128 * 128;            // 128 rows of 128 bytes
+  static constexpr int Q_BYTES = DCH * CHUNK;        // one Q tile
+  static constexpr int STAGE_BYTES = DCH * CHUNK;    // one K or V tile
+  static constexpr int RING_OFFSET = 2 * Q_BYTES;
+  static constexpr int BAR_OFFSET = RING_OFFSET + STAGES * STAGE_BYTES;
+  // full[S] empty[S] clean[S] q_full[2] q_empty[2] s_full[2] p_full[2] o_full[2] o_free[2] done
+  static constexpr int NUM_BARS = 3 * STAGES + 13;
+  static constexpr int SMEM_BYTES = BAR_OFFSET + NUM_BARS * 8 + 8 + 8 * 4 + 8 + 1024;
+  static constexpr int THREADS = 384;
+  static constexpr uint32_t TM_S = 0, TM_O = 256;    // + 128 for Q tile 1
+};
+
+template <class L> struct WindowTcBars {
+  uint32_t base;
+  __device__ __forceinline__ uint32_t full(int i) const { return base + 8u * i; }
+  __device__ __forceinline__ uint32_t empty(int i) const { return base + 8u * (L::STAGES + i); }
+  __device__ __forceinline__ uint32_t clean(int i) const { return base + 8u * (2 * L::STAGES + i); }
+  __device__ __forceinline__ uint32_t q_full(int t) const { return base + 8u * (3 * L::STAGES + t); }
+  __device__ __forceinline__ uint32_t q_empty(int t) const { return base + 8u * (3 * L::STAGES + 2 + t); }
+  __device__ __forceinline__ uint32_t s_full(int t) const { return base + 8u * (3 * L::STAGES + 4 + t); }
+  __device__ __forceinline__ uint32_t p_full(int t) const { return base + 8u * (3 * L::STAGES + 6 + t); }
+  __device__ __forceinline__ uint32_t o_full(int t) const { return base + 8u * (3 * L::STAGES + 8 + t); }
+  __device__ __forceinline__ uint32_t o_free(int t) const { return base + 8u * (3 * L::STAGES + 10 + t); }
+  __device__ __forceinline__ uint32_t done() const { return base + 8u * (3 * L::STAGES + 12); }
+};
+
+struct WindowTcShared {
+  uint8_t* q;                      // 1024-aligned
+  uint8_t* ring;
+  uint32_t bars;
+  uint32_t* tmem_slot;
+  volatile int* abort_flag;
+  volatile int* dirty;             // [8] item number + 1 of an item with cleaned infinities or NaN
+};
+
+template <class L>
+__device__ __forceinline__ WindowTcShared window_tc_carve(uint8_t* raw) {
+  WindowTcShared s;
+  const uintptr_t base = (reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023);
+  s.q = reinterpret_cast<uint8_t*>(base);
+  s.ring = s.q + L::RING_OFFSET;
+  s.bars = smem_u32(s.q + L::BAR_OFFSET);
+  s.tmem_slot = reinterpret_cast<uint32_t*>(s.q + L::BAR_OFFSET + L::NUM_BARS * 8);
+  s.abort_flag = reinterpret_cast<volatile int*>(s.tmem_slot + 1);
+  s.dirty = s.abort_flag + 1;
+  return s;
+}
+
+__device__ __forceinline__ void window_tc_fail(const WindowTcShared& s, const WindowTcArgs& args) {
+  *s.abort_flag = 1;
+  if (args.status) atomicOr(args.status, kWindowTimeout);
+}
+
+// The key tiles of a work item: [0, sink) and [start, end) in ascending order;
+// of these Q tile t needs those below need_sink[t] and in [lo[t], hi[t]).
+struct WindowItem {
+  int b, h, first, len;            // first: position of query 0
+  int i0;                          // first query of the item
+  int sink, start, end, tiles;
+  int lo[2], hi[2], need_sink[2];
+  int pa[2], pb[2];                // positions of the Q tiles' first and last rows; pb < pa: none
+  __device__ __forceinline__ WindowItem(const WindowTcArgs& a, int item) {
+    const int block = item % a.blocks, rest = item / a.blocks;
+    h = rest % a.kv_heads;
+    b = rest / a.kv_heads;
+    int n = a.lengths ? a.lengths[b] : a.cache;
+    n = n < 0 ? 0 : (n > a.cache ? a.cache : n);
+    len = n;
+    first = n - a.nq;
+    i0 = block * 2 * a.positions;
+    start = 0x7fffffff;
+    end = 0;
+    sink = 0x7fffffff;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int ia = i0 + t * a.positions, ib = min(ia + a.positions, a.nq) - 1;
+      pa[t] = max(first + ia, 0);                    // rows before the first key see nothing
+      pb[t] = first + ib;
+      if (ib < ia || pb[t] < 0) {
+        pa[t] = 0; pb[t] = -1; lo[t] = 0; hi[t] = 0; need_sink[t] = 0;
+        continue;
+      }
+      lo[t] = (a.window < 0 || pa[t] < a.window ? 0 : pa[t] - a.window + 1) / 128;
+      hi[t] = pb[t] / 128 + 1;
+      need_sink[t] = min((a.sinks + 127) / 128, hi[t]);
+      start = min(start, lo[t]);
+      end = max(end, hi[t]);
+      sink = min(sink, min(need_sink[t], lo[t]));
+    }
+    // (a later Q tile's sinks may reach past the earlier one's window start:
+    // they are inside [start, end) then)
+    if (end == 0) { sink = 0; start = 0; }
+    else if (pb[0] >= pa[0] && pb[1] >= pa[1]) sink = min(max(need_sink[0], need_sink[1]), start);
+    else sink = min(sink, start);
+    tiles = sink + end - start;
+  }
+  __device__ __forceinline__ int tile(int u) const { return u < sink ? u : u - sink + start; }
+  __device__ __forceinline__ bool need(int t, int j) const {
+    return pb[t] >= pa[t] && (j < need_sink[t] || (j >= lo[t] && j < hi[t]));
+  }
+  // every row of Q tile t sees all of key tile j
+  __device__ __forceinline__ bool whole(const WindowTcArgs& a, int t, int j) const {
+    const int k = j * 128;
+    return k + 127 <= pa[t] && first + i0 + t * a.positions >= 0 &&
+           (a.window < 0 || k > pb[t] - a.window || k + 128 <= a.sinks);
+  }
+  // V needs no cleaning: whole for each Q tile that needs it, and both do
+  __device__ __forceinline__ bool clean(const WindowTcArgs& a, int j) const {
+    return (!need(0, j) || whole(a, 0, j)) && (!need(1, j) || whole(a, 1, j));
+  }
+};
+
+// The positions of the rows are one run from pa to pb, so the keys some row
+// sees are one run (and the sinks).
+__device__ __forceinline__ bool window_tc_any(const WindowTcArgs& a, int pa, int pb, int j) {
+  return j <= pb && (a.window < 0 || j > pa - a.window || j < a.sinks);
+}
+__device__ __forceinline__ bool window_tc_sees(const WindowTcArgs& a, int p, int j) {
+  return j <= p && (a.window < 0 || j > p - a.window || j < a.sinks);
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+               " [%0], [%1, {%3, %4, %5, %6}], [%2];"
+               :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// D (+)= A B with A in TMEM (two 16-bit values a column)
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\t"
+               "setp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               :: "r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// A warp's 32 lanes x 128 columns -> 128 registers a thread (the wait inside:
+// no use of them can move before it).
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&u)[128]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+               "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+               "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+               "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
+               "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+               "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+               "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+               "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127"
+               "}, [%128];\n\t"
+               "tcgen05.wait::ld.sync.aligned;"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
+                 "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]),
+                 "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]),
+                 "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31]),
+                 "=r"(u[32]), "=r"(u[33]), "=r"(u[34]), "=r"(u[35]), "=r"(u[36]), "=r"(u[37]), "=r"(u[38]), "=r"(u[39]),
+                 "=r"(u[40]), "=r"(u[41]), "=r"(u[42]), "=r"(u[43]), "=r"(u[44]), "=r"(u[45]), "=r"(u[46]), "=r"(u[47]),
+                 "=r"(u[48]), "=r"(u[49]), "=r"(u[50]), "=r"(u[51]), "=r"(u[52]), "=r"(u[53]), "=r"(u[54]), "=r"(u[55]),
+                 "=r"(u[56]), "=r"(u[57]), "=r"(u[58]), "=r"(u[59]), "=r"(u[60]), "=r"(u[61]), "=r"(u[62]), "=r"(u[63]),
+                 "=r"(u[64]), "=r"(u[65]), "=r"(u[66]), "=r"(u[67]), "=r"(u[68]), "=r"(u[69]), "=r"(u[70]), "=r"(u[71]),
+                 "=r"(u[72]), "=r"(u[73]), "=r"(u[74]), "=r"(u[75]), "=r"(u[76]), "=r"(u[77]), "=r"(u[78]), "=r"(u[79]),
+                 "=r"(u[80]), "=r"(u[81]), "=r"(u[82]), "=r"(u[83]), "=r"(u[84]), "=r"(u[85]), "=r"(u[86]), "=r"(u[87]),
+                 "=r"(u[88]), "=r"(u[89]), "=r"(u[90]), "=r"(u[91]), "=r"(u[92]), "=r"(u[93]), "=r"(u[94]), "=r"(u[95]),
+                 "=r"(u[96]), "=r"(u[97]), "=r"(u[98]), "=r"(u[99]), "=r"(u[100]), "=r"(u[101]), "=r"(u[102]), "=r"(u[103]),
+                 "=r"(u[104]), "=r"(u[105]), "=r"(u[106]), "=r"(u[107]), "=r"(u[108]), "=r"(u[109]), "=r"(u[110]), "=r"(u[111]),
+                 "=r"(u[112]), "=r"(u[113]), "=r"(u[114]), "=r"(u[115]), "=r"(u[116]), "=r"(u[117]), "=r"(u[118]), "=r"(u[119]),
+                 "=r"(u[120]), "=r"(u[121]), "=r"(u[122]), "=r"(u[123]), "=r"(u[124]), "=r"(u[125]), "=r"(u[126]), "=r"(u[127])
+               : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* u) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+               "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+               "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32"
+               "};"
+               :: "r"(taddr),
+                 "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]),
+                 "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]),
+                 "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]),
+                 "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+template <class L>
+__device__ __forceinline__ void window_tc_init(const WindowTcShared& s, const WindowTcArgs& args) {
+  const int tid = threadIdx.x, warp = tid / 32;
+  if (tid == 0) {
+    const WindowTcBars<L> b{s.bars};
+    for (int i = 0; i < L::STAGES; ++i) {
+      mbar_init(b.full(i), 1);
+      mbar_init(b.empty(i), 1);
+      mbar_init(b.clean(i), 2);                      // the two cleaning warps
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(b.q_full(t), 1);
+      mbar_init(b.q_empty(t), 1);
+      mbar_init(b.s_full(t), 1);
+      mbar_init(b.p_full(t), 4);                     // the Q tile's softmax warps
+      mbar_init(b.o_full(t), 1);
+      mbar_init(b.o_free(t), 4);
+    }
+    mbar_init(b.done(), 1);
+    *s.abort_flag = 0;
+    for (int i = 0; i < 8; ++i) s.dirty[i] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" :: "l"(&args.tmap_q) : "memory");
+    asm volatile("prefetch.tensormap [%0];" :: "l"(&args.tmap_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" :: "l"(&args.tmap_v) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_u32(s.tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+}
+
+// Infinities and NaN of V that were cleaned away, added to columns c .. c + 31
+// of the row at position p, from the keys it sees (any weight above 0 carries
+// them into the sum).
+template <typename T>
+__device__ __noinline__ void window_tc_add_dirty(const WindowTcArgs& args, const WindowItem& w, int p,
+                                                 int c, float (&o)[32]) {
+  for (int u = 0; u < w.tiles; ++u) {
+    const int j = w.tile(u);
+    if (w.clean(args, j)) continue;
+    for (int key = j * 128; key < j * 128 + 128 && key < w.len; ++key) {
+      if (!window_tc_sees(args, p, key)) continue;
+      const T* v = static_cast<const T*>(args.v) + w.b * args.v_b + key * args.v_s + w.h * args.v_h + c;
+      for (int q = 0; q < 32 && c + q < args.dim; ++q) {
+        const float x = to_f32(v[q]);
+        if (!isfinite(x)) o[q] += x;
+      }
+    }
+  }
+}
+
+template <class L, typename T, typename OT, int POLY>
+__device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const WindowTcArgs& args) {
+  constexpr bool F16IN = std::is_same<T, f16>::value;
+  constexpr uint32_t S = L::STAGES;
+  tc_fence_after();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t tmem = *s.tmem_slot;
+  const WindowTcBars<L> bar{s.bars};
+  const int items = args.batch * args.kv_heads * args.blocks;
+  // ring entries in order K, V, K, V ...: entry e lies in stage e % S, and the
+  // barriers of its e / S-th use have that parity; V tile e / 2 is passed on by
+  // the cleaning warps through barrier clean(e / 2 % S)
+  bool ok = true;
+  auto wait = [&](uint32_t b, uint32_t parity) {
+    if (ok && !attn_wait(b, parity & 1u)) { window_tc_fail(s, args); ok = false; }
+    if (*s.abort_flag) ok = false;
+    return ok;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------- TMA producer
+    if (lane == 0) {
+      const uint32_t q_bytes = (uint32_t)(L::DCH * 128 * args.per * args.positions);
+      uint32_t entry = 0, qn[2] = {0, 0};
+      auto load = [&](const CUtensorMap* map, const WindowItem& w, int j) {
+        const uint32_t st = entry % S;
+        if (!wait(bar.empty(st), entry / S + 1u)) return;
+        mbar_expect_tx(bar.full(st), (uint32_t)L::STAGE_BYTES);
+#pragma unroll
+        for (int c = 0; c < L::DCH; ++c)
+          tma_load_4d(smem_u32(s.ring + st * L::STAGE_BYTES + c * L::CHUNK), map, bar.full(st),
+                      c * 64, w.h, j * 128, w.b);
+        ++entry;
+      };
+      for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
+        const WindowItem w(args, it);
+        for (int t = 0; t < 2; ++t) {
+          if (w.pb[t] < w.pa[t]) continue;
+          if (!wait(bar.q_empty(t), qn[t] + 1u)) break;
+          ++qn[t];
+          mbar_expect_tx(bar.q_full(t), q_bytes);
+#pragma unroll
+          for (int c = 0; c < L::DCH; ++c)
+            tma_load_4d(smem_u32(s.q + t * L::Q_BYTES + c * L::CHUNK), &args.tmap_q, bar.q_full(t),
+                        c * 64, w.h * args.per, w.i0 + t * args.positions, w.b);
+        }
+        for (int u = 0; u < w.tiles && ok; ++u) {
+          load(&args.tmap_k, w, w.tile(u));
+          if (ok) load(&args.tmap_v, w, w.tile(u));
+        }
+      }
+      if (!ok) {
+        // let the copies this thread issued land before the CTA can exit
+        bool landed = true;
+        for (uint32_t i = 0; i < S && i < entry; ++i) {
+          const uint32_t e = entry - 1u - i;
+          landed &= attn_wait(bar.full(e % S), (e / S) & 1u);
+        }
+        for (int t = 0; t < 2; ++t)
+          if (qn[t]) landed &= attn_wait(bar.q_full(t), (qn[t] + 1u) & 1u);
+        if (!landed && args.status) atomicOr(args.status, kWindowTimeout);
+      }
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t IDESC_S = umma_idesc<128, 128, F16IN, true>();
+      constexpr uint32_t IDESC_O = umma_idesc<128, L::DP, F16IN, false>();
+      uint32_t n = 0;                                // key tiles done
+      uint32_t qn[2] = {0, 0}, pn[2] = {0, 0}, on[2] = {0, 0};   // Q tiles, P tiles, items of O
+      for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
+        const WindowItem w(args, it);
+        bool begun[2] = {false, false};              // O_t holds this item's sums
+        // step u: P V of tile u - 1 and S of tile u, for either Q tile in turn
+        for (int u = 0; u <= w.tiles && w.tiles > 0 && ok; ++u) {
+          const int j = u < w.tiles ? w.tile(u) : -1, prev = u > 0 ? w.tile(u - 1) : -1;
+          const uint32_t ke = 2u * (n + u), ve = ke - 1u;        // ring entries of K_u, V_u-1
+          if (j >= 0 && !wait(bar.full(ke % S), ke / S)) break;
+          if (prev >= 0) {
+            if (!wait(bar.full(ve % S), ve / S) || !wait(bar.clean(ve / 2u % S), ve / 2u / S)) break;
+          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (prev >= 0 && w.need(t, prev)) {
+              if (!begun[t] && !wait(bar.o_free(t), on[t]++ + 1u)) break;
+              if (!wait(bar.p_full(t), pn[t]++)) break;
+              tc_fence_after();
+              const uint32_t v_base = smem_u32(s.ring + (ve % S) * L::STAGE_BYTES);
+              const uint32_t d = tmem + L::TM_O + 128u * t, p = tmem + L::TM_S + 128u * t;
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk)
+                umma_f16_ts(d, p + 8u * kk, umma_desc(v_base + 2048u * kk, (uint32_t)L::CHUNK, 1024u),
+                            IDESC_O, begun[t] || kk != 0 ? 1u : 0u);
+              umma_commit(bar.o_full(t));
+              begun[t] = true;
+            }
+            if (j >= 0 && w.need(t, j)) {
+              // (S_t is free: its last P has been used, and MMAs run in order)
+              if (!(qn[t] & 0x80000000u)) {
+                if (!wait(bar.q_full(t), qn[t])) break;
+                qn[t] |= 0x80000000u;                // waited for in this item
+              }
+              tc_fence_after();
+              const uint32_t d = tmem + L::TM_S + 128u * t;
+              const uint32_t a_base = smem_u32(s.q + t * L::Q_BYTES);
+              const uint32_t b_base = smem_u32(s.ring + (ke % S) * L::STAGE_BYTES);
+#pragma unroll
+              for (int c = 0; c < L::DCH; ++c)
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                  umma_f16(d, umma_desc(a_base + c * L::CHUNK + 32u * kk, 16u, 1024u),
+                           umma_desc(b_base + c * L::CHUNK + 32u * kk, 16u, 1024u), IDESC_S,
+                           (c | kk) != 0 ? 1u : 0u);
+              umma_commit(bar.s_full(t));
+            }
+          }
+          if (!ok) break;
+          if (prev >= 0) umma_commit(bar.empty(ve % S));
+          if (j >= 0) umma_commit(bar.empty(ke % S));
+          if (u == w.tiles - 1) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              if (qn[t] & 0x80000000u) {             // the item's last S: Q_t is free
+                umma_commit(bar.q_empty(t));
+                qn[t] = (qn[t] & 0x7fffffffu) + 1u;
+              }
+          }
+        }
+        n += (uint32_t)w.tiles;
+      }
+      // all MMAs this thread issued must finish before TMEM is released
+      umma_commit(bar.done());
+      if (!attn_wait(bar.done(), 0u)) { if (args.status) atomicOr(args.status, kWindowTimeout); }
+    }
+  } else if (warp < 4) {
+    // ----------------------------------------------------------- cleaning
+    // (every V tile is seen and passed on, so that the parities of a stage's
+    // barriers cannot run ahead of these warps)
+    uint32_t n = 0, seq = 0;
+    for (int it = blockIdx.x; it < items && ok; it += gridDim.x, ++seq) {
+      const WindowItem w(args, it);
+      const bool v0 = w.pb[0] >= w.pa[0], v1 = w.pb[1] >= w.pa[1];
+      const int pa = v0 ? w.pa[0] : w.pa[1], pb = v1 ? w.pb[1] : w.pb[0];
+      for (int u = 0; u < w.tiles && ok; ++u) {
+        const int j = w.tile(u);
+        const uint32_t e = 2u * (n + u) + 1u;
+        const bool got = attn_wait(bar.full(e % S), (e / S) & 1u);
+        if (!__all_sync(0xffffffffu, got && !*s.abort_flag)) {
+          if (lane == 0) window_tc_fail(s, args);
+          ok = false;
+          break;
+        }
+        bool found = false;
+#pragma unroll 1
+        for (int r = (warp - 2) * 32 + lane; r < 128 && !w.clean(args, j); r += 64) {
+          const int key = j * 128 + r;
+          const bool any = key < w.len && window_tc_any(args, pa, pb, key);
+          const bool all = key <= pa && (args.window < 0 || key > pb - args.window || key < args.sinks);
+          if (any && all) continue;
+          uint8_t* row = s.ring + (e % S) * L::STAGE_BYTES + r * 128;
+#pragma unroll 1
+          for (int q = 0; q < L::DCH * 8; ++q) {     // 16-byte chunks, the lanes' on different banks
+            uint4* at = reinterpret_cast<uint4*>(row + (q >> 3) * L::CHUNK + (((q + lane) & 7) << 4));
+            if (!any) { *at = make_uint4(0u, 0u, 0u, 0u); continue; }
+            uint4 x = *at;
+            uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              constexpr uint32_t EXP = F16IN ? 0x7C00u : 0x7F80u;
+              if ((xs[i] & EXP) == EXP) { xs[i] &= 0xFFFF0000u; bad = true; }
+              if ((xs[i] >> 16 & EXP) == EXP) { xs[i] &= 0x0000FFFFu; bad = true; }
+            }
+            if (bad) { *at = x; found = true; }
+          }
+        }
+        if (found) s.dirty[seq & 7u] = (int)seq + 1;
+        // the writes come before the tensor core's reads
+        fence_async_shared();
+        __threadfence_block();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar.clean(e / 2u % S));
+      }
+      n += (uint32_t)w.tiles;
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int t = (warp - 4) / 4, quarter = warp % 4;
+    const int r = quarter * 32 + lane;               // row of the Q tile = TMEM lane
+    const uint32_t lane_at = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_at = tmem + lane_at + L::TM_S + 128u * t;
+    const uint32_t o_at = tmem + lane_at + L::TM_O + 128u * t;
+    const float C2 = args.scale_log2;
+    const float slack = 8.0f / C2;                   // growth of the maximum left in the weights
+    uint32_t sn = 0, seq = 0;
+    for (int it = blockIdx.x; it < items && ok; it += gridDim.x, ++seq) {
+      const WindowItem w(args, it);
+      const int i = w.i0 + t * args.positions + r / args.per;    // this row's query
+      const bool real = r < args.per * args.positions && i < args.nq;
+      const int p = w.first + i;
+      float mref = -INFINITY, sum = 0.0f;            // maximum the weights are taken from; their sum
+      const bool run = w.pb[t] >= w.pa[t];
+      if (run) {
+        bool begun = false;
+        for (int u = 0; u < w.tiles; ++u) {
+          const int j = w.tile(u);
+          if (!w.need(t, j)) continue;
+          const bool got = attn_wait(bar.s_full(t), sn & 1u);
+          if (!__all_sync(0xffffffffu, got && !*s.abort_flag)) {
+            if (lane == 0) window_tc_fail(s, args);
+            ok = false;
+            break;
+          }
+          ++sn;
+          tc_fence_after();
+          uint32_t x[128];
+          tmem_ld128(s_at, x);
+          const bool whole = w.whole(args, t, j);
+          if (!whole) {
+            // columns from c0 on (or below cs) and up to c1 are seen
+            const int c1 = p - j * 128;
+            const int c0 = args.window < 0 ? -1 : p - args.window - j * 128;
+            const int cs = args.sinks - j * 128;
+#pragma unroll
+            for (int c = 0; c < 128; ++c)
+              if (!(c <= c1 && (c > c0 || c < cs))) x[c] = 0xFF800000u;          // -inf
+          }
+          float top[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) top[q] = __uint_as_float(x[q]);
+#pragma unroll
+          for (int c = 4; c < 128; ++c) top[c % 4] = fmaxf(top[c % 4], __uint_as_float(x[c]));
+          const float mn = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), mref);
+          if (!begun) {
+            mref = mn;
+          } else if (__any_sync(0xffffffffu, real && mn > mref + slack)) {
+            // rescale O once P V of the last tile is done
+            const bool done = attn_wait(bar.o_full(t), sn & 1u);         // (its number is sn - 2)
+            if (!__all_sync(0xffffffffu, done ? 1 : 0)) {
+              if (lane == 0) window_tc_fail(s, args);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            // (each row by its own maximum: no row's result depends on another's)
+            const bool grown = real && mn > mref + slack;
+            const float fix = !grown ? 1.0f : mref == -INFINITY ? 0.0f : fast_exp2((mref - mn) * C2);
+            sum *= fix;
+            if (grown) mref = mn;
+#pragma unroll 1
+            for (int c = 0; c < L::DP; c += 32) {
+              float o[32];
+              tmem_ld32(o_at + c, o);
+              uint32_t y[32];
+#pragma unroll
+              for (int q = 0; q < 32; ++q) y[q] = __float_as_uint(o[q] * fix);
+              tmem_st32(o_at + c, y);
+            }
+          }
+          begun = true;
+          const float off = mref == -INFINITY ? 0.0f : -mref * C2;
+          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (whole) {
+#pragma unroll
+            for (int c = 0; c < 128; ++c) {
+              const float e = attn_exp2<POLY>(c, fmaf(__uint_as_float(x[c]), C2, off));
+              part[c % 4] += e;
+              x[c] = __float_as_uint(e);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 128; ++c) {
+              const float e = fast_exp2(fmaf(__uint_as_float(x[c]), C2, off));
+              part[c % 4] += e;
+              x[c] = __float_as_uint(e);
+            }
+          }
+          sum += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+          for (int c = 0; c < 64; ++c) {
+            Slot<T, 2> two;
+            const float f[2] = {__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])};
+            pack_slot<T, 2>(two, f);
+            x[c] = *reinterpret_cast<const uint32_t*>(&two);
+          }
+          tmem_st32(s_at, x);
+          tmem_st32(s_at + 32, x + 32);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar.p_full(t));
+        }
+        if (!ok) break;
+        const bool done = attn_wait(bar.o_full(t), (sn + 1u) & 1u);
+        if (!__all_sync(0xffffffffu, done && !*s.abort_flag)) {
+          if (lane == 0) window_tc_fail(s, args);
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+      }
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const bool dirty = s.dirty[seq & 7u] == (int)seq + 1;
+      OT* dst = static_cast<OT*>(args.out) +
+                (((long long)w.b * args.nq + i) * args.kv_heads * args.per + w.h * args.per + r % args.per) *
+                    (long long)args.dim;
+#pragma unroll 1
+      for (int c = 0; c < L::DP; c += 32) {
+        float o[32];
+        if (run) tmem_ld32(o_at + c, o);             // (the whole warp)
+        if (c >= args.dim) continue;
+#pragma unroll
+        for (int q = 0; q < 32; ++q) o[q] = sum == 0.0f ? 0.0f : o[q] * inv;
+        if (dirty && real) window_tc_add_dirty<T>(args, w, p, c, o);
+        if (real) {
+#pragma unroll
+          for (int q = 0; q < 32; q += 8) {
+            if (c + q >= args.dim) break;
+            Slot<OT, 8> so;
+            pack_slot<OT, 8>(so, *reinterpret_cast<const float(*)[8]>(&o[q]));
+            store_slot<kStoreDefault, OT, 8>(dst + c + q, so);
+          }
+        }
+      }
+      if (run) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar.o_free(t));
+      }
+    }
+  }
+}
+
+template <class L>
+__device__ __forceinline__ void window_tc_teardown(const WindowTcShared& s) {
+  if (threadIdx.x / 32 == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
+                 :: "r"(*s.tmem_slot), "r"(512u) : "memory");
+  }
+}
+
+}  // namespace molten

@@ -439,6 +439,40 @@ int molten_encode_tma_2d(void* tmap, int dtype, const void* base, uint64_t inner
   return MOLTEN_OK;
 }
 
+int molten_encode_tma_4d(void* tmap, int dtype, const void* base, const uint64_t* dims,
+                         const uint64_t* strides_bytes, const uint32_t* box) {
+  if (!tmap || !base || !dims || !strides_bytes || !box)
+    return fail(MOLTEN_ERR_INVALID, "null tensor map, base pointer, dims, strides or box");
+  if (reinterpret_cast<uintptr_t>(tmap) % 64)
+    return fail(MOLTEN_ERR_INVALID, "tensor map storage must be 64-byte aligned");
+  if (reinterpret_cast<uintptr_t>(base) % 16)
+    return fail(MOLTEN_ERR_INVALID, "TMA base address must be 16-byte aligned");
+  if (dtype != MOLTEN_DT_BF16 && dtype != MOLTEN_DT_F16)
+    return fail(MOLTEN_ERR_INVALID, "4-D TMA maps take 16-bit element types");
+  for (int i = 0; i < 4; ++i)
+    if (!dims[i] || dims[i] > (1ull << 32) || !box[i] || box[i] > 256)
+      return fail(MOLTEN_ERR_INVALID, "bad TMA extents or box");
+  for (int i = 0; i < 3; ++i)
+    if (!strides_bytes[i] || strides_bytes[i] % 16 || strides_bytes[i] >= (1ull << 40))
+      return fail(MOLTEN_ERR_INVALID, "TMA strides must be multiples of 16 bytes below 2^40");
+  if (box[0] * 2 > 128 || box[0] % 8)
+    return fail(MOLTEN_ERR_INVALID, "a 128-byte swizzled box row takes up to 64 elements, in eights");
+  int rc = need_driver();
+  if (rc) return rc;
+  cuuint64_t d[4], st[3];
+  cuuint32_t b[4], estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) { d[i] = dims[i]; b[i] = box[i]; }
+  for (int i = 0; i < 3; ++i) st[i] = strides_bytes[i];
+  CUresult r = driver().tensor_map_encode_tiled(
+      static_cast<CUtensorMap*>(tmap),
+      dtype == MOLTEN_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+      const_cast<void*>(base), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return drv_fail(r, "cuTensorMapEncodeTiled");
+  return MOLTEN_OK;
+}
+
 int molten_status_word(int device, int** dev_ptr) {
   if (!dev_ptr || device < 0) return fail(MOLTEN_ERR_INVALID, "bad device or null output");
   std::lock_guard<std::mutex> lock(g_status_mu);

@@ -36,6 +36,7 @@ SMEM_SM = 228 * 1024
 WINDOW_MAX_DIM = 128
 WINDOW_FEW_ROWS = 32              # rows of a key head up to which the few-row kernel runs
 WINDOW_STAGES, WINDOW_TILE = 3, 16
+WINDOW_POLY = 0                   # exponentials of every 32 on the FMA pipe
 
 ROPE_MAX_AXES = 4
 ROPE_MAX_DIM = 1024
@@ -96,10 +97,13 @@ def _window_shape(op, ins):
     _need(len(q) == 4 and len(k) == 4 and k == v and q[0] == k[0] and q[3] == k[3],
           "window_attention needs q [batch, new, heads, d] and k, v [batch, cache, kv_heads, d]: "
           f"{q}, {k}, {v}")
+    _need(k[1] > 0, "window_attention needs a cache of at least one key")
     _need(k[2] > 0 and q[2] % k[2] == 0, f"window_attention: {q[2]} heads over {k[2]} key heads")
     _need(0 < q[3] <= WINDOW_MAX_DIM and q[3] % 8 == 0,
           f"window_attention: head dim {q[3]} must be a multiple of 8, at most {WINDOW_MAX_DIM}")
     _need(len(ins) == 3 or ins[3] == q[:1], f"window_attention: lengths {ins[-1]}, expected {q[:1]}")
+    scale = op.attrs.get("scale")
+    _need(scale is None or 0 < scale < float("inf"), f"window_attention: scale {scale} must be positive")
     w, s = op.attrs.get("window"), op.attrs.get("sinks") or 0
     _need(w is None or w >= 1, f"window_attention: window {w} must be at least 1 (None: no limit)")
     _need(s >= 0, f"window_attention: {s} sinks")
@@ -331,7 +335,8 @@ def _plan_window(op, sk, tune) -> dict:
     seen = cache if window < 0 else min(cache, window + sinks)
     span = cache if window < 0 else min(cache, window + sinks + new)
     c["flops"] = 4 * batch * heads * new * seen * dim
-    _need(rows <= WINDOW_FEW_ROWS, "window_attention: too many rows")
+    if o.get("kind") == "tiles" or (o.get("kind") is None and rows > WINDOW_FEW_ROWS):
+        return _plan_window_tiles(c, o)
     tiles = -(-span // WINDOW_TILE) + 1
     nb = 1 if rows <= 8 else 2 if rows <= 16 else 4
     ranks, parts, warps = _split_window(items, tiles, 8 if nb == 1 else 4)
@@ -355,6 +360,25 @@ def _plan_window(op, sk, tune) -> dict:
     return c
 
 
+def _plan_window_tiles(c: dict, o: dict) -> dict:
+    """The tcgen05 kernel: pairs of Q tiles of up to 128 (position, head) rows."""
+    per, dp = c["per"], c["dp"]
+    _need(per <= 128, f"window_attention: {per} heads over one key head; at most 128")
+    positions = 128 // per
+    blocks = -(-c["new"] // (2 * positions))
+    items = c["batch"] * c["kv_heads"] * blocks
+    _need(items < 2 ** 31, "window_attention: sizes beyond the kernel's range")
+    dch = dp // 64
+    stages = int(o.get("stages") or (5 if dp == 128 else 10))
+    bars = 3 * stages + 13
+    smem = 2 * dch * 16384 + stages * dch * 16384 + bars * 8 + 48 + 1024
+    _need(smem <= SMEM_LIMIT, f"window_attention: {stages} stages need {smem} bytes")
+    poly = int(o.get("poly", WINDOW_POLY))
+    c.update(kind="tiles", positions=positions, blocks=blocks, items=items, stages=stages,
+             smem=smem, block=384, poly=poly, ranks=1, parts=1)
+    return c
+
+
 _PLANS = {ModelOpType.MATVEC_Q4: _plan_q4, ModelOpType.ROTATE_POSITIONS: _plan_rope,
           ModelOpType.WINDOW_ATTENTION: _plan_window}
 
@@ -367,8 +391,11 @@ def launch_record(sk: SubKernel) -> dict:
     elif c["op"] == ModelOpType.ROTATE_POSITIONS:
         rec.update(head_lanes=c["head_lanes"], tokens_per_cta=c["tokens_per_cta"])
     elif c["op"] == ModelOpType.WINDOW_ATTENTION:
-        rec.update(kind=c["kind"], cluster=c["ranks"], parts=c["parts"],
-                   grid=c["items"] * c["parts"] * c["ranks"])
+        if c["kind"] == "tiles":
+            rec.update(kind="tiles", positions=c["positions"], blocks=c["blocks"], items=c["items"])
+        else:
+            rec.update(kind="few", cluster=c["ranks"], parts=c["parts"], smem=c["smem_launch"],
+                       grid=c["items"] * c["parts"] * c["ranks"])
     return rec
 
 
@@ -419,6 +446,29 @@ extern "C" __global__ void __launch_bounds__(1024) {name}(const __grid_constant_
 def _emit_window(sk, name):
     c = sk.config
     t, ot = DTYPE_CTYPE[sk.operands[0].dtype], DTYPE_CTYPE[sk.outputs[0].dtype]
+    if c["kind"] == "tiles":
+        return f"""// Molten sm_100a window attention: {name}
+// {sk.operands[0].dtype}, head dim up to {c['dp']}
+#include "molten/window_sm100.cuh"
+
+using namespace molten;
+
+typedef WindowTcLayout<{c['dp']}, {c['stages']}> Layout_{name};
+static_assert(Layout_{name}::SMEM_BYTES == {c['smem']}, "the launch's dynamic shared memory");
+static_assert(Layout_{name}::THREADS == {c['block']}, "block size");
+
+extern "C" __global__ void __launch_bounds__({c['block']}, 1) {name}(const __grid_constant__ WindowTcArgs args) {{
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const WindowTcShared sh = window_tc_carve<Layout_{name}>(smem_raw);
+  window_tc_init<Layout_{name}>(sh, args);     // mbarriers + TMEM allocation
+  pdl_enter();                                 // no global access before this
+  __syncthreads();
+  window_tc_roles<Layout_{name}, {t}, {ot}, {c['poly']}>(sh, args);
+  tc_fence_before();
+  __syncthreads();
+  window_tc_teardown<Layout_{name}>(sh);       // TMEM release
+}}
+"""
     lay = f"{c['dp']}, {c['nb']}, {c['warps']}, {c['stages']}"
     return f"""// Molten sm_100a window attention, few query rows: {name}
 // {sk.operands[0].dtype}, head dim up to {c['dp']}, up to {8 * c['nb']} rows

@@ -8,9 +8,11 @@ and captured graphs never share one.
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 from . import _capi
+from .decode import SMS
 from .ir import ModelOpType
 from .lowering import DTYPE_SIZE
 
@@ -109,6 +111,33 @@ def _launch_rope(spec, sk, entry, ins, out, device, stream):
     spec.module(device).launch(entry, _cfg(grid, c["block"]), a, stream)
 
 
+def _tma_4d(t, dtype: str, box) -> bytes:
+    """TMA descriptor of t [b, s, h, d]; the stride of a dim of one element
+    (any number in torch) is replaced by one that the encoder takes."""
+    b, s, h, d = t.shape
+    size = t.element_size()
+    strides = [t.stride(2) if h > 1 else 8, t.stride(1) if s > 1 else 8, t.stride(0) if b > 1 else 8]
+    return _capi.encode_tma_4d(_capi.DT_BF16 if dtype == "bfloat16" else _capi.DT_F16, t.data_ptr(),
+                               (d, h, s, b), [x * size for x in strides], box)
+
+
+def _launch_window_tiles(spec, sk, entry, q, k, v, lengths, out, device, stream):
+    c = sk.config
+    dt = sk.operands[0].dtype
+    a = _capi.WindowTcArgs()
+    ctypes.memmove(a.tmap_q, _tma_4d(q, dt, (64, c["per"], c["positions"], 1)), 128)
+    ctypes.memmove(a.tmap_k, _tma_4d(k, dt, (64, 1, 128, 1)), 128)
+    ctypes.memmove(a.tmap_v, _tma_4d(v, dt, (64, 1, 128, 1)), 128)
+    a.v, a.out = v.data_ptr(), out.data_ptr()
+    a.lengths = lengths.data_ptr() if lengths is not None else None
+    a.status = _capi.status_word(device)
+    a.v_b, a.v_s, a.v_h = v.stride()[:3]
+    a.batch, a.nq, a.cache, a.kv_heads = c["batch"], c["new"], c["cache"], c["kv_heads"]
+    a.per, a.dim, a.window, a.sinks = c["per"], c["dim"], c["window"], c["sinks"]
+    a.scale_log2, a.positions, a.blocks = c["scale"] * LOG2E, c["positions"], c["blocks"]
+    spec.module(device).launch(entry, _cfg(min(c["items"], SMS), c["block"], 1, c["smem"]), a, stream)
+
+
 def _launch_window(spec, sk, entry, ins, out, device, stream):
     c = sk.config
     a = _capi.WindowArgs()
@@ -116,12 +145,17 @@ def _launch_window(spec, sk, entry, ins, out, device, stream):
     for j in range(3):
         t = ins[j]
         # 16-byte rows: the last dim contiguous, every other stride a multiple
-        # of 8 elements
-        if (t.stride(3) != 1 and t.shape[3] > 1) or not _aligned(t, 16, t.stride()[:3]):
+        # of 8 elements (and not 0 where the tiles are copied by TMA)
+        if ((t.stride(3) != 1 and t.shape[3] > 1) or not _aligned(t, 16, t.stride()[:3])
+                or (c["kind"] == "tiles" and any(n > 1 and x == 0 for n, x in zip(t.shape, t.stride())))):
             t = t.contiguous()
         _check_aligned(sk.operands[j].name, entry, t, 16)
         qkv.append(t)
     q, k, v = qkv
+    _check_aligned("output", entry, out, 16)
+    if c["kind"] == "tiles":
+        _launch_window_tiles(spec, sk, entry, q, k, v, ins.get(3), out, device, stream)
+        return
     a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     a.lengths = ins[3].data_ptr() if 3 in ins else None
     a.q_b, a.q_s, a.q_h = q.stride()[:3]

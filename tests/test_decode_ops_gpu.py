@@ -400,3 +400,87 @@ def test_window_attention_views_and_scale(rt):
     full = torch.full((b,), cache, dtype=torch.int32, device=DEV)
     none = window_kernel(rt, b, new, cache, heads, kv, d, None, 0, "float16", lengths=False)
     check_attention(none(q, k, v), q, k, v, full, None, 0, "float16", 2.0 ** -16)
+
+
+MANY = [  # b, new, cache, heads, kv, d, window, sinks, lengths
+    (1, 40, 40, 2, 2, 64, None, 0, [40]),
+    (1, 128, 128, 1, 1, 128, None, 0, [128]),
+    (1, 257, 257, 1, 1, 64, 100, 3, [257]),
+    (2, 300, 300, 4, 2, 128, 128, 4, [300, 170]),
+    (2, 130, 900, 8, 2, 128, 200, 130, [900, 411]),
+    (1, 700, 1500, 5, 1, 80, 333, 16, [1500]),
+    (3, 65, 400, 14, 2, 96, 1, 0, [400, 65, 30]),
+    (2, 90, 500, 8, 8, 24, 50, 1, [0, 499]),
+    (1, 2000, 2000, 2, 1, 128, 512, 129, [2000]),
+    (1, 33, 3000, 128, 1, 64, 700, 5, [2999]),
+    (2, 600, 700, 6, 2, 128, 2000, 0, [700, 644]),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("case", MANY)
+def test_window_attention_many_rows(rt, case, dtype):
+    b, new, cache, heads, kv, d, window, sinks, lens = case
+    q, k, v = attention_inputs(b, new, cache, heads, kv, d, dtype, seed=cache + new)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    ck = window_kernel(rt, b, new, cache, heads, kv, d, window, sinks, dtype)
+    assert ck.specialization(q, k, v, lengths).plan.kernels[0].config["kind"] == "tiles"
+    out = ck(q, k, v, lengths)
+    assert MoltenRuntime.read_status(0) == 0
+    check_attention(out, q, k, v, lengths, window, sinks, dtype, half_step(dtype))
+    assert torch.equal(out, ck(q, k, v, lengths))
+
+
+@pytest.mark.parametrize("spread", [8.0, 60.0])
+def test_window_attention_growing_maxima(rt, spread):
+    """Scores whose maxima grow along the keys: O is rescaled, and large
+    differences leave single keys."""
+    b, new, cache, heads, kv, d = 1, 200, 1200, 4, 2, 64
+    q, k, v = attention_inputs(b, new, cache, heads, kv, d, "bfloat16", seed=7, spread=spread)
+    k = (k * torch.linspace(0.05, 1.0, cache, device=DEV)[None, :, None, None]).to(torch.bfloat16)
+    lengths = torch.tensor([cache], dtype=torch.int32, device=DEV)
+    ck = window_kernel(rt, b, new, cache, heads, kv, d, None, 0, "bfloat16")
+    out = ck(q, k, v, lengths)
+    check_attention(out, q, k, v, lengths, None, 0, "bfloat16", 2.0 ** -8)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), torch.finfo(torch.bfloat16).min])
+def test_window_attention_many_rows_ignores_unseen_keys(rt, bad):
+    b, new, cache, heads, kv, d, window, sinks = 2, 150, 900, 4, 2, 128, 130, 3
+    q, k, v = attention_inputs(b, new, cache, heads, kv, d, "bfloat16", seed=8)
+    lengths = torch.tensor([811, 120], dtype=torch.int32, device=DEV)
+    unseen = ~seen_mask(lengths, new, cache, window, sinks).any(1)
+    k[unseen], v[unseen] = bad, bad
+    ck = window_kernel(rt, b, new, cache, heads, kv, d, window, sinks, "bfloat16")
+    check_attention(ck(q, k, v, lengths), q, k, v, lengths, window, sinks, "bfloat16", 2.0 ** -8)
+    if bad != bad or bad == float("inf"):
+        # one value that only the last 10 queries see, one that only the first do
+        v2 = v.clone()
+        v2[0, 801, 0, 5] = bad
+        v2[0, 811 - 150 - 100, 1, 7] = bad
+        got = ck(q, k, v2, lengths)
+        v2[0, 801, 0, 5] = 0
+        v2[0, 811 - 150 - 100, 1, 7] = 0
+        ref, _, _ = attention_reference(q, k, v2, lengths, window, sinks)
+        seen = seen_mask(lengths, new, cache, window, sinks)[0]
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[0, :, :2, 5] = seen[:, 801][:, None]
+        hit[0, :, 2:, 7] = seen[:, 811 - 150 - 100][:, None]
+        assert int(hit.sum()) > 0 and torch.equal(~torch.isfinite(got), hit)
+        assert bool(((got.double() - ref).abs() <= 0.05)[~hit].all())
+
+
+def test_window_attention_many_rows_views(rt):
+    b, new, heads, kv, d, cache = 2, 100, 8, 4, 64, 333
+    fused = torch.randn(b, new, heads + 2 * kv, d, generator=gen_of(3), device=DEV).to(torch.float16)
+    q = fused[:, :, :heads]
+    kc = torch.randn(b, kv, cache + 6, d, generator=gen_of(4), device=DEV).to(torch.float16)
+    vc = torch.randn(1, cache, kv, d, generator=gen_of(5), device=DEV).to(torch.float16)
+    k, v = kc[:, :, 6:].transpose(1, 2), vc.expand(b, cache, kv, d)
+    lengths = torch.tensor([cache, 131], dtype=torch.int32, device=DEV)
+    ck = window_kernel(rt, b, new, cache, heads, kv, d, 90, 1, "float16", scale=0.3)
+    check_attention(ck(q, k, v, lengths), q, k, v, lengths, 90, 1, "float16", 2.0 ** -11, scale=0.3)
+    # the same through the few-row kernel's form of the parameters: one row at a time
+    one = window_kernel(rt, b, 1, cache, heads, kv, d, 90, 1, "float16", scale=0.3)
+    got = one(q[:, -1:], k, v, lengths)
+    check_attention(got, q[:, -1:], k, v, lengths, 90, 1, "float16", 2.0 ** -16, scale=0.3)
