@@ -170,6 +170,25 @@ typedef struct molten_window_tc_args {
   int positions, blocks, reserved;
 } molten_window_tc_args;
 
+/* Parameter block of the sampling kernels (device side: molten::SampleArgs in
+ * molten/sample.cuh).  A parameter's vector may be null: its scalar is used
+ * then (temperature 1, top_k 0, top_p 1 and min_p 0 leave every token).
+ * Grid rows * ranks in clusters of `ranks`, run = ceil(vocab / (256 ranks)),
+ * made odd. */
+typedef struct molten_sample_args {
+  const void* logits;            /* [rows, vocab], rows row_stride elements apart */
+  const float* u;                /* [rows] in [0, 1) */
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  int* out;                      /* [rows]; -1: nothing can be drawn */
+  long long row_stride;
+  int rows, vocab, run, ranks;
+  float temperature_all, top_p_all, min_p_all;
+  int top_k_all;
+} molten_sample_args;
+
 /* Version of this ABI (major * 100 + minor). */
 int molten_version(void);
 

@@ -125,6 +125,17 @@ class WindowTcArgs(ctypes.Structure):
                 + [("tail_", ctypes.c_ubyte * 24)])
 
 
+class SampleArgs(ctypes.Structure):
+    """molten_sample_args / molten::SampleArgs."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "u", "temperature", "top_k", "top_p",
+                                                "min_p", "out")]
+                + [("row_stride", ctypes.c_longlong)]
+                + [(n, ctypes.c_int) for n in ("rows", "vocab", "run", "ranks")]
+                + [(n, ctypes.c_float) for n in ("temperature_all", "top_p_all", "min_p_all")]
+                + [("top_k_all", ctypes.c_int)])
+
+
+assert ctypes.sizeof(SampleArgs) == 96
 assert ctypes.sizeof(WindowTcArgs) == 512
 assert ctypes.sizeof(WindowArgs) == 168
 assert ctypes.sizeof(RopePosArgs) == 120

@@ -38,6 +38,9 @@ WINDOW_FEW_ROWS = 32              # rows of a key head up to which the few-row k
 WINDOW_STAGES, WINDOW_TILE = 3, 16
 WINDOW_POLY = 0                   # exponentials of every 32 on the FMA pipe
 
+SAMPLE_THREADS = 256
+SAMPLE_FIXED = 18848              # sizeof(SampleShared) (molten/sample.cuh)
+
 ROPE_MAX_AXES = 4
 ROPE_MAX_DIM = 1024
 
@@ -110,8 +113,18 @@ def _window_shape(op, ins):
     return q
 
 
+def _sample_shape(op, ins):
+    logits, u = ins[:2]
+    _need(len(logits) >= 2 and logits[-1] > 0, f"sample needs logits [..., vocabulary], got {logits}")
+    lead = logits[:-1]
+    _need(u == lead, f"sample: u of shape {u}, expected {lead}")
+    for name, s in zip(op.attrs.get("params", ()), ins[2:]):
+        _need(s in ((), lead), f"sample: {name} of shape {s}, expected {lead} or a constant")
+    return lead
+
+
 _SHAPES = {ModelOpType.MATVEC_Q4: _q4_shape, ModelOpType.ROTATE_POSITIONS: _rope_shape,
-           ModelOpType.WINDOW_ATTENTION: _window_shape}
+           ModelOpType.WINDOW_ATTENTION: _window_shape, ModelOpType.SAMPLE: _sample_shape}
 
 
 # -------------------------------------------------------------------- types
@@ -379,8 +392,34 @@ def _plan_window_tiles(c: dict, o: dict) -> dict:
     return c
 
 
+def _plan_sample(op, sk, tune) -> dict:
+    logits = sk.operands[0]
+    vocab, rows = logits.shape[-1], prod(logits.shape[:-1])
+    _need(rows * 8 < 2 ** 31, "sample: sizes beyond 2^31")
+    o = tune.get("sample") or {}
+
+    def run_of(ranks):
+        # consecutive tokens of a thread, an odd number (no bank conflicts)
+        return -(-vocab // (SAMPLE_THREADS * ranks)) | 1
+
+    def smem_of(ranks):
+        return SAMPLE_FIXED + 4 * SAMPLE_THREADS * run_of(ranks)
+    # the fewest CTAs a row that leave room for three on an SM; more while SMs
+    # would have none
+    ranks = 1
+    while ranks < 8 and (smem_of(ranks) > SMEM_SM // 3 - 1024
+                         or (rows * ranks < SMS and run_of(ranks) > 8)):
+        ranks *= 2
+    ranks = int(o.get("ranks") or ranks)
+    _need(smem_of(ranks) <= SMEM_LIMIT,
+          f"sample: a vocabulary of {vocab} does not fit the shared memory of a cluster")
+    return {"rows": rows, "vocab": vocab, "ranks": ranks, "run": run_of(ranks),
+            "smem": smem_of(ranks), "block": SAMPLE_THREADS, "params": list(op.attrs.get("params", ())),
+            "flops": 2 * rows * vocab}
+
+
 _PLANS = {ModelOpType.MATVEC_Q4: _plan_q4, ModelOpType.ROTATE_POSITIONS: _plan_rope,
-          ModelOpType.WINDOW_ATTENTION: _plan_window}
+          ModelOpType.WINDOW_ATTENTION: _plan_window, ModelOpType.SAMPLE: _plan_sample}
 
 
 def launch_record(sk: SubKernel) -> dict:
@@ -390,6 +429,8 @@ def launch_record(sk: SubKernel) -> dict:
         rec.update(grid=c["teams"] * c["ksplit"], cluster=c["ksplit"], warps_n=c["warps_n"])
     elif c["op"] == ModelOpType.ROTATE_POSITIONS:
         rec.update(head_lanes=c["head_lanes"], tokens_per_cta=c["tokens_per_cta"])
+    elif c["op"] == ModelOpType.SAMPLE:
+        rec.update(grid=c["rows"] * c["ranks"], cluster=c["ranks"])
     elif c["op"] == ModelOpType.WINDOW_ATTENTION:
         if c["kind"] == "tiles":
             rec.update(kind="tiles", positions=c["positions"], blocks=c["blocks"], items=c["items"])
@@ -491,5 +532,24 @@ extern "C" __global__ void __launch_bounds__(128) {name}_join(const __grid_const
 """
 
 
+def _emit_sample(sk, name):
+    t = DTYPE_CTYPE[sk.operands[0].dtype]
+    return f"""// Molten sm_100a sampling: {name}
+// {sk.operands[0].dtype} logits
+#include "molten/sample.cuh"
+
+using namespace molten;
+
+static_assert(sizeof(SampleShared) == {SAMPLE_FIXED} && SAMPLE_THREADS == {SAMPLE_THREADS},
+              "the launch's dynamic shared memory");
+
+extern "C" __global__ void __launch_bounds__({SAMPLE_THREADS}, 3) {name}(const __grid_constant__ SampleArgs args) {{
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  pdl_enter();
+  sample_row<{t}>(args, smem_raw);
+}}
+"""
+
+
 _EMIT = {ModelOpType.MATVEC_Q4: _emit_q4, ModelOpType.ROTATE_POSITIONS: _emit_rope,
-         ModelOpType.WINDOW_ATTENTION: _emit_window}
+         ModelOpType.WINDOW_ATTENTION: _emit_window, ModelOpType.SAMPLE: _emit_sample}

@@ -178,8 +178,27 @@ def _launch_window(spec, sk, entry, ins, out, device, stream):
         mod.launch(entry + b"_join", _cfg(-(-c["items"] * c["rows"] // 4), 128), a, stream)
 
 
+def _launch_sample(spec, sk, entry, ins, out, device, stream):
+    c = sk.config
+    x = _merged(ins[0], 1)
+    _check_aligned(sk.operands[0].name, entry, x, x.element_size())
+    a = _capi.SampleArgs()
+    a.logits, a.u, a.out = x.data_ptr(), ins[1].data_ptr(), out.data_ptr()
+    a.row_stride, a.rows, a.vocab = x.stride(0), c["rows"], c["vocab"]
+    a.run, a.ranks = c["run"], c["ranks"]
+    a.temperature_all, a.top_p_all = 1.0, 1.0        # without a parameter: no limit
+    for i, name in enumerate(c["params"]):
+        if 2 + i in ins:
+            setattr(a, name, ins[2 + i].data_ptr())
+        else:
+            value = c["scalars"][2 + i]
+            setattr(a, name + "_all", int(value) if name == "top_k" else float(value))
+    spec.module(device).launch(entry, _cfg(c["rows"] * c["ranks"], c["block"], c["ranks"], c["smem"]), a,
+                               stream)
+
+
 _LAUNCH = {ModelOpType.MATVEC_Q4: _launch_q4, ModelOpType.ROTATE_POSITIONS: _launch_rope,
-           ModelOpType.WINDOW_ATTENTION: _launch_window}
+           ModelOpType.WINDOW_ATTENTION: _launch_window, ModelOpType.SAMPLE: _launch_sample}
 
 # operands a kernel takes as strided views; the rest are made contiguous
 STRIDED = {ModelOpType.MATVEC_Q4: (0,), ModelOpType.ROTATE_POSITIONS: (0,),

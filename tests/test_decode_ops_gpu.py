@@ -484,3 +484,160 @@ def test_window_attention_many_rows_views(rt):
     one = window_kernel(rt, b, 1, cache, heads, kv, d, 90, 1, "float16", scale=0.3)
     got = one(q[:, -1:], k, v, lengths)
     check_attention(got, q[:, -1:], k, v, lengths, 90, 1, "float16", 2.0 ** -16, scale=0.3)
+
+
+# ------------------------------------------------------------------ sampling
+def sample_reference(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    """(tokens, how near any border came to a decision), in 64 bits."""
+    x_all = logits.double().cpu().numpy()
+    rows = x_all.shape[0]
+
+    def of(v, r, none):
+        return none if v is None else float(v[r]) if torch.is_tensor(v) else float(v)
+    out, near = np.empty(rows, np.int64), np.empty(rows)
+    for r in range(rows):
+        x = np.where(np.isnan(x_all[r]), -np.inf, np.minimum(x_all[r], 3.4028234663852886e38))
+        t, k, p, mp = of(temperature, r, 1.0), of(top_k, r, 0), of(top_p, r, 1.0), of(min_p, r, 0.0)
+        order = np.argsort(-x, kind="stable")
+        near[r] = 1.0
+        if x[order[0]] == -np.inf:
+            out[r] = -1
+            continue
+        if not t > 0:
+            out[r] = order[0]
+            continue
+        count = int(np.sum(x > -np.inf))
+        if k > 0:
+            count = min(count, int(k))
+        w = np.exp((x[order[:count]] - x[order[0]]) / t)
+        if p < 1:
+            reach = np.cumsum(w)
+            goal = max(p, 0.0) * reach[-1]
+            near[r] = min(near[r], np.min(np.abs(reach / reach[-1] - p)) if p > 0 else 1.0)
+            count = max(1, int(np.searchsorted(reach, goal, side="left")) + (1 if goal > 0 else 0))
+            count = min(count, w.size)
+        if mp > 0:
+            near[r] = min(near[r], np.min(np.abs(w[:count] - mp)))
+            count = max(1, int(np.sum(w[:count] >= min(mp, 1.0))))
+        chosen = np.sort(order[:count])
+        reach = np.cumsum(np.exp((x[chosen] - x[order[0]]) / t))
+        goal = float(u[r]) * reach[-1]
+        near[r] = min(near[r], np.min(np.abs(reach - goal)) / reach[-1])
+        out[r] = chosen[min(np.searchsorted(reach, goal, side="right"), chosen.size - 1)]
+    return out, near
+
+
+def check_sample(tokens, logits, u, **params):
+    want, near = sample_reference(logits, u, **params)
+    got = tokens.cpu().numpy()
+    # where a border lies within 1e-10 of the decision, 64 bits do not decide it
+    sure = near > 1e-10
+    assert sure.mean() > 0.9
+    assert np.array_equal(got[sure], want[sure]), np.flatnonzero((got != want) & sure)[:8]
+
+
+def sample_inputs(rows, vocab, dtype, seed=0, spread=3.0):
+    g = gen_of(seed)
+    x = (spread * torch.randn(rows, vocab, generator=g, device=DEV)).to(DT[dtype])
+    return x, torch.rand(rows, generator=g, device=DEV)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (5, 2), (3, 7), (40, 300), (33, 5003), (9, 50257), (4, 131072)])
+@pytest.mark.parametrize("use", ["", "k", "p", "m", "kp", "kpm"])
+def test_sample(rt, rows, vocab, dtype, use):
+    x, u = sample_inputs(rows, vocab, dtype, seed=rows + vocab)
+    g = gen_of(9)
+    params = {"temperature": 0.3 + 1.5 * torch.rand(rows, generator=g, device=DEV)}
+    if "k" in use:
+        params["top_k"] = torch.randint(-1, min(vocab + 2, 3000), (rows,), generator=g, device=DEV,
+                                        dtype=torch.int32)
+    if "p" in use:
+        params["top_p"] = 1.1 * torch.rand(rows, generator=g, device=DEV)
+    if "m" in use:
+        params["min_p"] = 0.3 * torch.rand(rows, generator=g, device=DEV) - 0.05
+    ck = compiled(rt, graphs.sample(rows, vocab, dtype=dtype, top_k="k" in use, top_p="p" in use,
+                                    min_p="m" in use), dtype)
+    tokens = ck(x, u, *params.values())
+    assert tokens.dtype == torch.int32 and tokens.shape == (rows,)
+    check_sample(tokens, x, u, **params)
+    assert torch.equal(tokens, ck(x, u, *params.values()))
+
+
+@pytest.mark.parametrize("ranks", [1, 2, 4, 8])
+@pytest.mark.parametrize("kind", ["ties", "equal", "steps", "narrow", "wide", "one"])
+def test_sample_hard_rows(ranks, kind):
+    """Rows whose borders fall into many equal logits, spread over 40 orders of
+    magnitude or lie a rounding apart."""
+    rows, vocab = 24, 20011
+    tuned = MoltenRuntime(tune={"sample": {"ranks": ranks}})
+    ck = compiled(tuned, graphs.sample(2, 64, top_k=True, top_p=True, min_p=True), "float32")
+    g = gen_of(11)
+    x = torch.randn(rows, vocab, generator=g, device=DEV)
+    if kind == "ties":
+        x = (4 * x).round() / 2
+    elif kind == "equal":
+        x = torch.full_like(x, 3.25)
+    elif kind == "steps":
+        x = torch.arange(vocab, device=DEV).float().expand(rows, vocab) % 97 * 0.01
+    elif kind == "narrow":
+        x = 1000 + x * 1e-4
+    elif kind == "wide":
+        x = x * torch.exp(20 * torch.rand(rows, vocab, generator=g, device=DEV) - 10) * 1e30
+    else:
+        x = torch.full_like(x, -torch.inf)
+        x[torch.arange(rows, device=DEV), torch.randint(0, vocab, (rows,), generator=g, device=DEV)] = 2.0
+    x = x.contiguous()
+    u = torch.rand(rows, generator=g, device=DEV)
+    params = {"temperature": 0.5 + torch.rand(rows, generator=g, device=DEV),
+              "top_k": torch.randint(0, vocab, (rows,), generator=g, device=DEV, dtype=torch.int32),
+              "top_p": 0.3 + 0.8 * torch.rand(rows, generator=g, device=DEV),
+              "min_p": 0.1 * torch.rand(rows, generator=g, device=DEV) - 0.05}
+    if kind == "wide":
+        params["temperature"] *= 1e33
+    check_sample(ck(x, u, *params.values()), x, u, **params)
+
+
+def test_sample_edges(rt):
+    """Greedy rows, rows without a token, infinities and NaN, u at its ends,
+    parameters that keep only the largest token."""
+    vocab = 1000
+    inf, nan = float("inf"), float("nan")
+    base = torch.randn(12, vocab, generator=gen_of(12), device=DEV)
+    x = base.clone()
+    x[0] = -inf
+    x[1] = nan
+    x[2, 5::7] = nan
+    x[3, 100], x[3, 200] = inf, inf
+    x[4, 17], x[4, 9] = 9.0, 9.0
+    x[5, :-1] = -inf
+    u = torch.tensor([.3, .3, .5, .7, .9, .5, 0., 1 - 2.0 ** -24, .5, .5, .5, .5], device=DEV)
+    t = torch.tensor([1, 1, 1, 1, 0, 1, 1, 1, -1, 1e-6, 1e30, 1], device=DEV)
+    k = torch.tensor([0, 5, 50, 0, 3, 2, 0, 0, 1, 0, 0, 1], dtype=torch.int32, device=DEV)
+    p = torch.tensor([.5, .5, .9, .99, .1, .5, 1, 1, 1, 1, .5, 0.], device=DEV)
+    m = torch.tensor([0, 0, 0, 0, 0, .5, 0, 0, 0, 0, 0, 2.], device=DEV)
+    ck = compiled(rt, graphs.sample(12, vocab, top_k=True, top_p=True, min_p=True), "float32")
+    tokens = ck(x, u, t, k, p, m)
+    check_sample(tokens, x, u, temperature=t, top_k=k, top_p=p, min_p=m)
+    assert tokens[0] == -1 and tokens[1] == -1 and tokens[4] == 9 and tokens[5] == vocab - 1
+    assert tokens[3] in (100, 200)
+
+
+def test_sample_constants_views_and_rank(rt):
+    """Scalar parameters, a strided view, two leading dims."""
+    wide = 2 * torch.randn(3, 4, 777, generator=gen_of(13), device=DEV).to(torch.bfloat16)
+    x = wide[..., 5:506]
+    u = torch.rand(3, 4, generator=gen_of(14), device=DEV)
+    g = DataflowGraph("sample")
+    xi, ui = g.add_input("x", TS([3, 4, 501])), g.add_input("u", TS([3, 4]))
+    g.add_output(g.sample(xi, ui, temperature=g.add_constant("t", 0.7), top_k=g.add_constant("k", 40),
+                          top_p=g.add_constant("p", 0.8)))
+    tokens = compiled(rt, g, "bfloat16")(x, u)
+    assert tokens.shape == (3, 4)
+    check_sample(tokens.view(12), x.reshape(12, 501), u.view(12), temperature=0.7, top_k=40, top_p=0.8)
+    # greedy
+    g = DataflowGraph("greedy")
+    xi, ui = g.add_input("x", TS([3, 4, 501])), g.add_input("u", TS([3, 4]))
+    g.add_output(g.sample(xi, ui, temperature=g.add_constant("t", 0.0)))
+    assert torch.equal(compiled(rt, g, "bfloat16")(x, u).long().view(12),
+                       torch.from_numpy(sample_reference(x.reshape(12, 501), u.view(12), 0.0)[0]).to(DEV))
