@@ -241,19 +241,6 @@ def encode_tma_2d(dtype_code: int, base: int, inner: int, outer: int, row_stride
     return ctypes.string_at(aligned, 128)
 
 
-def encode_tma_4d(dtype_code: int, base: int, dims, strides_bytes, box) -> bytes:
-    """128-byte TMA descriptor of a 4-D tensor of 16-bit elements (128-byte
-    swizzle); ``dims`` from the contiguous one out, ``strides_bytes`` of the
-    other three."""
-    buf = ctypes.create_string_buffer(128 + 64)
-    aligned = (ctypes.addressof(buf) + 63) & ~63
-    check(load_library().molten_encode_tma_4d(
-        ctypes.c_void_p(aligned), dtype_code, ctypes.c_void_p(base),
-        (ctypes.c_uint64 * 4)(*dims), (ctypes.c_uint64 * 3)(*strides_bytes),
-        (ctypes.c_uint32 * 4)(*box)), "encoding a TMA descriptor")
-    return ctypes.string_at(aligned, 128)
-
-
 def status_word(device: int) -> int:
     p = ctypes.c_void_p()
     check(load_library().molten_status_word(device, ctypes.byref(p)), "status word")

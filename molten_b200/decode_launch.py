@@ -1,21 +1,29 @@
 """Parameter blocks and launches of the model operators (``decode.py``).
 
-Every call reads pointers, strides and sizes from the tensors it is given;
-nothing is kept from one call for the next.  Workspaces come from torch's
+Every call reads pointers and strides from the tensors it is given; nothing is
+kept from one call for the next but what the shapes decide (the sizes' part of
+the parameter block, the launch geometry).  Workspaces come from torch's
 allocator on the launching stream, one per call, so calls on several streams
 and captured graphs never share one.
+
+A call has two ways in.  ``launch_model_op`` runs a model operator among the
+sub-kernels of any plan and brings operands into a layout the kernel takes.
+``ModelCall`` is the short way for a graph that is one model operator, called
+again with the shapes of its last call: single tokens run for a few
+microseconds, less than the general path's bookkeeping.  It declines
+(``NotImplemented``) whatever is not plain, and the general path takes over.
 """
 
 from __future__ import annotations
 
 import ctypes
 import math
+from struct import Struct
 
 from . import _capi
 from .decode import SMS
 from .ir import ModelOpType
 from .lowering import DTYPE_SIZE
-
 
 LOG2E = math.log2(math.e)
 
@@ -40,166 +48,310 @@ def _aligned(t, nbytes: int, strides) -> bool:
     return t.data_ptr() % nbytes == 0 and all(s * t.element_size() % nbytes == 0 for s in strides)
 
 
-def _check_aligned(name: str, entry: bytes, t, nbytes: int) -> None:
-    if t.data_ptr() % nbytes:
-        raise _capi.MoltenError(f"input {name!r} at {t.data_ptr():#x} is not {nbytes}-byte aligned "
-                                f"as kernel {entry.decode()} requires")
+class _Bound:
+    """One model sub-kernel on one device: its module, launch geometry and the
+    part of its parameter block that the shapes decide."""
+
+    def __init__(self, spec, i: int, device: int):
+        self.sk = spec.plan.kernels[i]
+        self.c = self.sk.config
+        self.entry = spec.entries[i]
+        self.module = spec.module(device)
+        self.device = device
+        self.setup()
+
+    def config(self, grid, block: int, cluster: int = 1, smem: int = 0):
+        from .runtime import PDL
+        cfg = _capi.LaunchCfg()
+        cfg.grid[:] = [grid, 1, 1]
+        cfg.block[:] = [block, 1, 1]
+        cfg.cluster[:] = [cluster, 1, 1]
+        cfg.smem_bytes = smem
+        cfg.flags = _capi.LAUNCH_PDL if PDL else 0
+        return ctypes.byref(cfg), cfg
+
+    def tail(self, args_type, first: str) -> bytes:
+        """The static end of a parameter block, from field ``first`` on, with
+        this kernel's sizes."""
+        a = args_type()
+        self.fill(a)
+        return bytes(a)[getattr(args_type, first).offset:]
+
+    def launch(self, block: bytes, stream: int, cfg=None, entry=None) -> None:
+        entry = entry or self.entry
+        rc = self.module.lib.molten_launch(self.module.handle, entry, cfg or self.cfg[0], block,
+                                           len(block), stream)
+        if rc:
+            raise _capi.MoltenError(f"launching {entry.decode()} failed (code {rc}): "
+                                    f"{_capi.last_error()}")
+
+    def need_aligned(self, j: int, t, nbytes: int) -> None:
+        if t.data_ptr() % nbytes:
+            name = next(o.name for o in self.sk.operands if o.index == j) if j >= 0 else "output"
+            raise _capi.MoltenError(f"{'input ' + repr(name) if j >= 0 else name} at "
+                                    f"{t.data_ptr():#x} is not {nbytes}-byte aligned as kernel "
+                                    f"{self.entry.decode()} requires")
+
+    # per operator: setup(); fill(args); conform(ins) -> ins the kernel takes;
+    # run(ins, out, stream) on such ins
 
 
-def _cfg(grid, block: int, cluster: int = 1, smem: int = 0):
-    from .runtime import PDL
-    cfg = _capi.LaunchCfg()
-    cfg.grid[:] = [grid, 1, 1]
-    cfg.block[:] = [block, 1, 1]
-    cfg.cluster[:] = [cluster, 1, 1]
-    cfg.smem_bytes = smem
-    cfg.flags = _capi.LAUNCH_PDL if PDL else 0
-    return cfg
+class _Q4(_Bound):
+    head = Struct("<5Qq")
 
+    def setup(self):
+        c = self.c
+        self.cfg = self.config(c["teams"] * c["ksplit"], c["block"], c["ksplit"], c["smem"])
+        self.rest = self.tail(_capi.Q4Args, "n")
 
-def launch_model_op(spec, i: int, env: dict, device: int, stream: int) -> None:
-    """Launch sub-kernel ``i`` of ``spec`` on ``stream``."""
-    sk = spec.plan.kernels[i]
-    ins = {o.index: env[o.op_id] for o in sk.operands}
-    _LAUNCH[sk.config["op"]](spec, sk, spec.entries[i], ins, env[sk.outputs[0].op_id], device, stream)
+    def fill(self, a):
+        c = self.c
+        a.n, a.m, a.k = c["n"], c["m"], c["k"]
+        a.warps_n_log, a.ksplit_log = c["warps_n"].bit_length() - 1, c["ksplit"].bit_length() - 1
+        a.chunk, a.tiles, a.teams = c["chunk"], c["tiles"], c["teams"]
 
-
-def _launch_q4(spec, sk, entry, ins, out, device, stream):
-    c = sk.config
-    x, q, scales, zeros = _merged(ins[0], 1), ins[1], ins[2], ins.get(3)
-    if not _aligned(x, 16, x.stride()[:-1]) and x.shape[0] > 1:
-        x = x.contiguous()
-    _check_aligned(sk.operands[0].name, entry, x, 16)
-    _check_aligned(sk.operands[1].name, entry, q, 16)
-    for o, t in zip(sk.operands[2:], (scales, zeros)):
-        _check_aligned(o.name, entry, t, DTYPE_SIZE[o.dtype])
-    a = _capi.Q4Args()
-    a.x, a.q, a.scales, a.out = x.data_ptr(), q.data_ptr(), scales.data_ptr(), out.data_ptr()
-    a.zeros = zeros.data_ptr() if zeros is not None else None
-    a.x_stride, a.n, a.m, a.k = x.stride(0), c["n"], c["m"], c["k"]
-    a.warps_n_log, a.ksplit_log = c["warps_n"].bit_length() - 1, c["ksplit"].bit_length() - 1
-    a.chunk, a.tiles, a.teams = c["chunk"], c["tiles"], c["teams"]
-    cfg = _cfg(c["teams"] * c["ksplit"], c["block"], c["ksplit"], c["smem"])
-    spec.module(device).launch(entry, cfg, a, stream)
-
-
-def _launch_rope(spec, sk, entry, ins, out, device, stream):
-    c = sk.config
-    x = _merged(ins[0], 2)
-    tables, pos = [ins[j] for j in range(1, len(ins) - 1)], ins[len(ins) - 1]
-    if c["xvec"]:
-        slot = min(16, c["vec"] * x.element_size())
-        if not _aligned(x, slot, x.stride()[:-1]):
+    def conform(self, ins):
+        x = _merged(ins[0], 1)
+        if not _aligned(x, 16, x.stride()[:-1]) and x.shape[0] > 1:
             x = x.contiguous()
-        _check_aligned(sk.operands[0].name, entry, x, slot)
-        _check_aligned("output", entry, out, min(16, c["vec"] * out.element_size()))
-    if c["tvec"]:
-        for o, t in zip(sk.operands[1:], tables):
-            _check_aligned(o.name, entry, t, c["table_slot"])
-    a = _capi.RopePosArgs()
-    a.x, a.cos_t, a.pos, a.out = x.data_ptr(), tables[0].data_ptr(), pos.data_ptr(), out.data_ptr()
-    a.sin_t = tables[-1].data_ptr()
-    a.status = _capi.status_word(device)
-    a.tokens, a.x_token, a.x_head = c["tokens"], x.stride(0), x.stride(1)
-    a.table_rows, a.heads, a.dim = c["table_rows"], c["heads"], c["dim"]
-    a.axes, a.head_lanes, a.tokens_per_cta = len(c["sections"]), c["head_lanes"], c["tokens_per_cta"]
-    end = 0
-    for j, width in enumerate(c["sections"]):
-        end += width
-        a.bound[j] = end
-    grid = -(-c["tokens"] // c["tokens_per_cta"])
-    spec.module(device).launch(entry, _cfg(grid, c["block"]), a, stream)
+        self.need_aligned(0, x, 16)
+        self.need_aligned(1, ins[1], 16)
+        for j in range(2, len(ins)):
+            self.need_aligned(j, ins[j], ins[j].element_size())
+        return [x] + ins[1:]
+
+    def run(self, ins, out, stream):
+        x = ins[0]
+        block = self.head.pack(x.data_ptr(), ins[1].data_ptr(), ins[2].data_ptr(),
+                               ins[3].data_ptr() if len(ins) > 3 else 0, out.data_ptr(),
+                               x.stride(-2) if x.dim() > 1 else self.c["k"])
+        self.launch(block + self.rest, stream)
 
 
-def _tma_4d(t, dtype: str, box) -> bytes:
-    """TMA descriptor of t [b, s, h, d]; the stride of a dim of one element
-    (any number in torch) is replaced by one that the encoder takes."""
-    b, s, h, d = t.shape
-    size = t.element_size()
-    strides = [t.stride(2) if h > 1 else 8, t.stride(1) if s > 1 else 8, t.stride(0) if b > 1 else 8]
-    return _capi.encode_tma_4d(_capi.DT_BF16 if dtype == "bfloat16" else _capi.DT_F16, t.data_ptr(),
-                               (d, h, s, b), [x * size for x in strides], box)
+class _Rope(_Bound):
+    head = Struct("<6Q4q")
+
+    def setup(self):
+        c = self.c
+        self.cfg = self.config(-(-c["tokens"] // c["tokens_per_cta"]), c["block"])
+        self.rest = self.tail(_capi.RopePosArgs, "heads")
+        self.status = _capi.status_word(self.device)
+
+    def fill(self, a):
+        c = self.c
+        a.heads, a.dim = c["heads"], c["dim"]
+        a.axes, a.head_lanes, a.tokens_per_cta = len(c["sections"]), c["head_lanes"], c["tokens_per_cta"]
+        end = 0
+        for j, width in enumerate(c["sections"]):
+            end += width
+            a.bound[j] = end
+
+    def conform(self, ins):
+        c = self.c
+        x = _merged(ins[0], 2)
+        if c["xvec"]:
+            slot = min(16, c["vec"] * x.element_size())
+            if not _aligned(x, slot, x.stride()[:-1]):
+                x = x.contiguous()
+            self.need_aligned(0, x, slot)
+        if c["tvec"]:
+            for j in range(1, len(ins) - 1):
+                self.need_aligned(j, ins[j], c["table_slot"])
+        return [x] + ins[1:]
+
+    def run(self, ins, out, stream):
+        c, x = self.c, ins[0]
+        if c["xvec"]:
+            self.need_aligned(-1, out, min(16, c["vec"] * out.element_size()))
+        block = self.head.pack(x.data_ptr(), ins[1].data_ptr(), ins[-2].data_ptr(),
+                               ins[-1].data_ptr(), out.data_ptr(), self.status,
+                               c["tokens"], x.stride(-3), x.stride(-2), c["table_rows"])
+        self.launch(block + self.rest, stream)
 
 
-def _launch_window_tiles(spec, sk, entry, q, k, v, lengths, out, device, stream):
-    c = sk.config
-    dt = sk.operands[0].dtype
-    a = _capi.WindowTcArgs()
-    ctypes.memmove(a.tmap_q, _tma_4d(q, dt, (64, c["per"], c["positions"], 1)), 128)
-    ctypes.memmove(a.tmap_k, _tma_4d(k, dt, (64, 1, 128, 1)), 128)
-    ctypes.memmove(a.tmap_v, _tma_4d(v, dt, (64, 1, 128, 1)), 128)
-    a.v, a.out = v.data_ptr(), out.data_ptr()
-    a.lengths = lengths.data_ptr() if lengths is not None else None
-    a.status = _capi.status_word(device)
-    a.v_b, a.v_s, a.v_h = v.stride()[:3]
-    a.batch, a.nq, a.cache, a.kv_heads = c["batch"], c["new"], c["cache"], c["kv_heads"]
-    a.per, a.dim, a.window, a.sinks = c["per"], c["dim"], c["window"], c["sinks"]
-    a.scale_log2, a.positions, a.blocks = c["scale"] * LOG2E, c["positions"], c["blocks"]
-    spec.module(device).launch(entry, _cfg(min(c["items"], SMS), c["block"], 1, c["smem"]), a, stream)
+class _Window(_Bound):
+    head = Struct("<6Q9q")
+    tiles_head = Struct("<4Q3q")
+    dims, strides, box = Struct("<4Q"), Struct("<3Q"), Struct("<4I")
 
-
-def _launch_window(spec, sk, entry, ins, out, device, stream):
-    c = sk.config
-    a = _capi.WindowArgs()
-    qkv = []
-    for j in range(3):
-        t = ins[j]
-        # 16-byte rows: the last dim contiguous, every other stride a multiple
-        # of 8 elements (and not 0 where the tiles are copied by TMA)
-        if ((t.stride(3) != 1 and t.shape[3] > 1) or not _aligned(t, 16, t.stride()[:3])
-                or (c["kind"] == "tiles" and any(n > 1 and x == 0 for n, x in zip(t.shape, t.stride())))):
-            t = t.contiguous()
-        _check_aligned(sk.operands[j].name, entry, t, 16)
-        qkv.append(t)
-    q, k, v = qkv
-    _check_aligned("output", entry, out, 16)
-    if c["kind"] == "tiles":
-        _launch_window_tiles(spec, sk, entry, q, k, v, ins.get(3), out, device, stream)
-        return
-    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    a.lengths = ins[3].data_ptr() if 3 in ins else None
-    a.q_b, a.q_s, a.q_h = q.stride()[:3]
-    a.k_b, a.k_s, a.k_h = k.stride()[:3]
-    a.v_b, a.v_s, a.v_h = v.stride()[:3]
-    a.batch, a.nq, a.cache, a.kv_heads = c["batch"], c["new"], c["cache"], c["kv_heads"]
-    a.per, a.dim, a.window, a.sinks = c["per"], c["dim"], c["window"], c["sinks"]
-    a.scale_log2 = c["scale"] * LOG2E
-    a.ranks, a.parts = c["ranks"], c["parts"]
-    mod = spec.module(device)
-    grid = c["items"] * c["parts"] * c["ranks"]
-    part = None
-    if c["parts"] > 1:
-        import torch
-        part = torch.empty(c["items"] * c["parts"] * c["rows"] * (c["dim"] + 2),
-                           dtype=torch.float32, device=q.device)
-        a.part = part.data_ptr()
-    mod.launch(entry, _cfg(grid, c["block"], c["ranks"], c["smem_launch"]), a, stream)
-    if part is not None:
-        mod.launch(entry + b"_join", _cfg(-(-c["items"] * c["rows"] // 4), 128), a, stream)
-
-
-def _launch_sample(spec, sk, entry, ins, out, device, stream):
-    c = sk.config
-    x = _merged(ins[0], 1)
-    _check_aligned(sk.operands[0].name, entry, x, x.element_size())
-    a = _capi.SampleArgs()
-    a.logits, a.u, a.out = x.data_ptr(), ins[1].data_ptr(), out.data_ptr()
-    a.row_stride, a.rows, a.vocab = x.stride(0), c["rows"], c["vocab"]
-    a.run, a.ranks = c["run"], c["ranks"]
-    a.temperature_all, a.top_p_all = 1.0, 1.0        # without a parameter: no limit
-    for i, name in enumerate(c["params"]):
-        if 2 + i in ins:
-            setattr(a, name, ins[2 + i].data_ptr())
+    def setup(self):
+        c = self.c
+        if c["kind"] == "tiles":
+            self.cfg = self.config(min(c["items"], SMS), c["block"], 1, c["smem"])
+            self.rest = self.tail(_capi.WindowTcArgs, "batch")
+            self.status = _capi.status_word(self.device)
+            self.code = _capi.DT_BF16 if self.sk.operands[0].dtype == "bfloat16" else _capi.DT_F16
         else:
-            value = c["scalars"][2 + i]
+            self.cfg = self.config(c["items"] * c["parts"] * c["ranks"], c["block"], c["ranks"],
+                                   c["smem_launch"])
+            self.rest = self.tail(_capi.WindowArgs, "batch")
+            self.part = c["items"] * c["parts"] * c["rows"] * (c["dim"] + 2) if c["parts"] > 1 else 0
+            self.join = self.config(-(-c["items"] * c["rows"] // 4), 128)
+
+    def fill(self, a):
+        c = self.c
+        a.batch, a.nq, a.cache, a.kv_heads = c["batch"], c["new"], c["cache"], c["kv_heads"]
+        a.per, a.dim, a.window, a.sinks = c["per"], c["dim"], c["window"], c["sinks"]
+        a.scale_log2 = c["scale"] * LOG2E
+        if c["kind"] == "tiles":
+            a.positions, a.blocks = c["positions"], c["blocks"]
+        else:
+            a.ranks, a.parts = c["ranks"], c["parts"]
+
+    def conform(self, ins):
+        out = list(ins)
+        for j in range(3):
+            t = ins[j]
+            # 16-byte rows: the last dim contiguous, every other stride a
+            # multiple of 8 elements (and not 0 where TMA copies the tiles)
+            if ((t.stride(3) != 1 and t.shape[3] > 1) or not _aligned(t, 16, t.stride()[:3])
+                    or (self.c["kind"] == "tiles"
+                        and any(n > 1 and x == 0 for n, x in zip(t.shape, t.stride())))):
+                t = t.contiguous()
+            self.need_aligned(j, t, 16)
+            out[j] = t
+        return out
+
+    def tensor_maps(self, ins) -> bytes:
+        """The TMA descriptors of q, k and v [b, s, h, d], 128 bytes each.  The
+        stride of a dim of one element (any number in torch) is replaced by one
+        that the encoder takes."""
+        c = self.c
+        buf = (ctypes.c_char * 448)()
+        at = (ctypes.addressof(buf) + 63) & ~63
+        encode = self.module.lib.molten_encode_tma_4d
+        for n, t in enumerate(ins[:3]):
+            b, s, h, d = t.shape
+            sb, ss, sh, _ = t.stride()
+            box = (64, c["per"], c["positions"], 1) if n == 0 else (64, 1, 128, 1)
+            _capi.check(encode(at + 128 * n, self.code, t.data_ptr(), self.dims.pack(d, h, s, b),
+                               self.strides.pack(2 * sh if h > 1 else 16, 2 * ss if s > 1 else 16,
+                                                 2 * sb if b > 1 else 16),
+                               self.box.pack(*box)), "encoding a TMA descriptor")
+        return ctypes.string_at(at, 384)
+
+    def run(self, ins, out, stream):
+        q, k, v = ins[:3]
+        lengths = ins[3].data_ptr() if len(ins) > 3 else 0
+        c = self.c
+        self.need_aligned(-1, out, 16)
+        if c["kind"] == "tiles":
+            block = (self.tensor_maps(ins)
+                     + self.tiles_head.pack(v.data_ptr(), lengths, out.data_ptr(), self.status,
+                                            *v.stride()[:3]))
+            self.launch(block + self.rest, stream)
+            return
+        part = None
+        if self.part:
+            import torch
+            part = torch.empty(self.part, dtype=torch.float32, device=q.device)
+        block = self.head.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), lengths, out.data_ptr(),
+                               0 if part is None else part.data_ptr(),
+                               *q.stride()[:3], *k.stride()[:3], *v.stride()[:3]) + self.rest
+        self.launch(block, stream)
+        if part is not None:
+            self.launch(block, stream, self.join[0], self.entry + b"_join")
+
+
+class _Sample(_Bound):
+    head = Struct("<7Qq")
+    slots = ("temperature", "top_k", "top_p", "min_p")
+
+    def setup(self):
+        c = self.c
+        self.cfg = self.config(c["rows"] * c["ranks"], c["block"], c["ranks"], c["smem"])
+        self.rest = self.tail(_capi.SampleArgs, "rows")
+        # where each parameter stands among the tensors of a call
+        self.at, n = [], 2
+        for name in self.slots:
+            given = name in c["params"] and 2 + c["params"].index(name) not in c["scalars"]
+            self.at.append(n if given else -1)
+            n += given
+
+    def fill(self, a):
+        c = self.c
+        a.rows, a.vocab, a.run, a.ranks = c["rows"], c["vocab"], c["run"], c["ranks"]
+        a.temperature_all, a.top_p_all = 1.0, 1.0        # without a parameter: no limit
+        for pos, value in c["scalars"].items():
+            name = c["params"][pos - 2]
             setattr(a, name + "_all", int(value) if name == "top_k" else float(value))
-    spec.module(device).launch(entry, _cfg(c["rows"] * c["ranks"], c["block"], c["ranks"], c["smem"]), a,
-                               stream)
+
+    def conform(self, ins):
+        x = _merged(ins[0], 1)
+        self.need_aligned(0, x, x.element_size())
+        return [x] + ins[1:]
+
+    def run(self, ins, out, stream):
+        x = ins[0]
+        t, k, p, m = [ins[j].data_ptr() if j > 0 else 0 for j in self.at]
+        block = self.head.pack(x.data_ptr(), ins[1].data_ptr(), t, k, p, m, out.data_ptr(),
+                               x.stride(-2))
+        self.launch(block + self.rest, stream)
 
 
-_LAUNCH = {ModelOpType.MATVEC_Q4: _launch_q4, ModelOpType.ROTATE_POSITIONS: _launch_rope,
-           ModelOpType.WINDOW_ATTENTION: _launch_window, ModelOpType.SAMPLE: _launch_sample}
+_BOUND = {ModelOpType.MATVEC_Q4: _Q4, ModelOpType.ROTATE_POSITIONS: _Rope,
+          ModelOpType.WINDOW_ATTENTION: _Window, ModelOpType.SAMPLE: _Sample}
 
 # operands a kernel takes as strided views; the rest are made contiguous
 STRIDED = {ModelOpType.MATVEC_Q4: (0,), ModelOpType.ROTATE_POSITIONS: (0,),
            ModelOpType.WINDOW_ATTENTION: (0, 1, 2), ModelOpType.SAMPLE: (0,)}
+
+
+def _bound(spec, i: int, device: int) -> _Bound:
+    key = ("model", i, device)
+    b = spec._cfgs.get(key)
+    if b is None:
+        b = spec._cfgs[key] = _BOUND[spec.plan.kernels[i].config["op"]](spec, i, device)
+    return b
+
+
+def launch_model_op(spec, i: int, env: dict, device: int, stream: int) -> None:
+    """Launch sub-kernel ``i`` of ``spec`` on ``stream``."""
+    b = _bound(spec, i, device)
+    # (operand positions of scalars are left out: SAMPLE's ``at`` counts them)
+    ins = [env[o.op_id] for o in b.sk.operands]
+    b.run(b.conform(ins), env[b.sk.outputs[0].op_id], stream)
+
+
+class ModelCall:
+    """The short way into a plan that is one model operator: ``call(tensors)``
+    with contiguous, 16-byte aligned tensors on the current device, on its
+    current stream; ``NotImplemented`` for anything else."""
+
+    def __init__(self, spec, tensors):
+        import torch
+        plan = spec.plan
+        self.spec = spec
+        sk = plan.kernels[0]
+        self.dtypes = [t.dtype for t in tensors]
+        self.shapes = [t.shape for t in tensors]
+        place = {op_id: n for n, op_id in enumerate(plan.inputs)}
+        self.order = [place[o.op_id] for o in sk.operands]
+        self.in_order = self.order == list(range(len(tensors)))
+        self.out_shape, self.out_dtype = tuple(plan.output_shapes[0]), spec.out_dtypes[0]
+        self.empty = torch.empty
+        self.current_device = torch._C._cuda_getDevice
+        self.current_stream = torch._C._cuda_getCurrentRawStream
+
+    @staticmethod
+    def fits(spec) -> bool:
+        plan = spec.plan
+        return (len(plan.kernels) == 1 and plan.kernels[0].family == "model" and not plan.temps
+                and len(plan.outputs) == 1
+                and len({o.op_id for o in plan.kernels[0].operands}) == len(plan.inputs)
+                and all(d > 0 for d in plan.output_shapes[0]))
+
+    def __call__(self, tensors):
+        if len(tensors) != len(self.shapes):
+            return NotImplemented
+        device = tensors[0].get_device()
+        if device < 0 or device != self.current_device():
+            return NotImplemented
+        for t, dtype, shape in zip(tensors, self.dtypes, self.shapes):
+            if (t.dtype is not dtype or t.shape != shape or t.get_device() != device
+                    or not t.is_contiguous() or t.data_ptr() % 16):
+                return NotImplemented
+        out = self.empty(self.out_shape, dtype=self.out_dtype, device=tensors[0].device)
+        ins = tensors if self.in_order else [tensors[n] for n in self.order]
+        _bound(self.spec, 0, device).run(ins, out, self.current_stream(device))
+        return out

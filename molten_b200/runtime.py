@@ -34,7 +34,7 @@ from typing import Optional
 from . import _capi
 from .build import build_cubin, default_cache_dir
 from .codegen import CodeGenerator, GeneratedKernel, KernelConfig, kernel_entry
-from .decode_launch import STRIDED, launch_model_op
+from .decode_launch import STRIDED, ModelCall, launch_model_op
 from .lowering import DTYPE_SIZE, LoweringError, canon_tensor_dtype
 
 _TORCH_DTYPES = None
@@ -85,6 +85,7 @@ class _Spec:
         self._cfgs: dict = {}
         self._tmaps: OrderedDict = OrderedDict()
         self.align = [_alignment_rules(sk) for sk in self.plan.kernels]
+        self.single = ModelCall.fits(self)
 
     def module(self, device: int) -> _capi.Module:
         m = self.modules.get(device)
@@ -460,8 +461,13 @@ class CompiledKernel:
     runtime: Optional["MoltenRuntime"] = None
     _specs: dict = field(default_factory=dict)
     _hosts: dict = field(default_factory=dict)
+    _last: Optional[ModelCall] = None     # the last call's specialisation, where it is one model operator
 
     def __call__(self, *tensors, out=None, stream=None, row_offset: int = 0):
+        if self._last is not None and out is None and stream is None:
+            res = self._last(tensors)
+            if res is not NotImplemented:
+                return res
         if self.kernel is None or self.runtime is None:
             raise RuntimeError(f"Kernel '{self.name}' not compiled. Call compile() first.")
         plan = self.kernel.plan
@@ -489,6 +495,8 @@ class CompiledKernel:
         else:
             outs = None
         res = spec.run(prepared, outs, stream, row_offset)
+        if not DEBUG and spec.single:
+            self._last = ModelCall(spec, tensors)
         return res[0] if len(res) == 1 else tuple(res)
 
     # -- specialisation -------------------------------------------------
