@@ -173,8 +173,8 @@ typedef struct molten_window_tc_args {
 /* Parameter block of the sampling kernels (device side: molten::SampleArgs in
  * molten/sample.cuh).  A parameter's vector may be null: its scalar is used
  * then (temperature 1, top_k 0, top_p 1 and min_p 0 leave every token).
- * Grid rows * ranks in clusters of `ranks`, run = ceil(vocab / (256 ranks)),
- * made odd. */
+ * Grid rows * ranks in clusters of `ranks`; run: tokens per thread, an odd
+ * number of 32-bit words with 256 * ranks * run >= vocab. */
 typedef struct molten_sample_args {
   const void* logits;            /* [rows, vocab], rows row_stride elements apart */
   const float* u;                /* [rows] in [0, 1) */

@@ -38,8 +38,7 @@ WINDOW_FEW_ROWS = 32              # rows of a key head up to which the few-row k
 WINDOW_STAGES, WINDOW_TILE = 3, 16
 WINDOW_POLY = 0                   # exponentials of every 32 on the FMA pipe
 
-SAMPLE_THREADS = 256
-SAMPLE_FIXED = 18848              # sizeof(SampleShared) (molten/sample.cuh)
+SAMPLE_FIXED = 2 * 8 * 24 + 32 * 24 + 2048 + 4096 + 2 * 2048 + 64   # of SampleShared (molten/sample.cuh)
 
 ROPE_MAX_AXES = 4
 ROPE_MAX_DIM = 1024
@@ -392,29 +391,42 @@ def _plan_window_tiles(c: dict, o: dict) -> dict:
     return c
 
 
+def _sample_fixed(dtype, threads) -> int:
+    packed = threads * 20 // DTYPE_SIZE[dtype]        # tokens: value and 16-bit index
+    return SAMPLE_FIXED + packed * (DTYPE_SIZE[dtype] + 2)
+
+
 def _plan_sample(op, sk, tune) -> dict:
     logits = sk.operands[0]
     vocab, rows = logits.shape[-1], prod(logits.shape[:-1])
     _need(rows * 8 < 2 ** 31, "sample: sizes beyond 2^31")
     o = tune.get("sample") or {}
 
+    word = 4 // DTYPE_SIZE[logits.dtype]              # tokens of 32 bits
+    # few rows: more threads, so that a pass over a thread's tokens is short (37 x 50257:
+    # 512 threads 62 us, 256 70; 128 x 32768: 83 and 50)
+    threads = int(o.get("threads") or (512 if rows * 8 <= 2 * SMS else 256))
+
     def run_of(ranks):
-        # consecutive tokens of a thread, an odd number (no bank conflicts)
-        return -(-vocab // (SAMPLE_THREADS * ranks)) | 1
+        # consecutive tokens of a thread: an odd number of words (no bank conflicts)
+        return word * (-(-vocab // (threads * ranks * word)) | 1)
 
     def smem_of(ranks):
-        return SAMPLE_FIXED + 4 * SAMPLE_THREADS * run_of(ranks)
-    # the fewest CTAs a row that leave room for three on an SM; more while SMs
-    # would have none
+        return _sample_fixed(logits.dtype, threads) + threads * run_of(ranks) * DTYPE_SIZE[logits.dtype] + 16
+    # the fewest CTAs a row that leave room for 768 threads on an SM; more while
+    # SMs would have none and threads many tokens (16 x 32768: 4 CTAs 19.8 us, 8
+    # 27.4; 16 x 131072: 98 and 69)
     ranks = 1
-    while ranks < 8 and (smem_of(ranks) > SMEM_SM // 3 - 1024
-                         or (rows * ranks < SMS and run_of(ranks) > 8)):
+    while ranks < 8 and (smem_of(ranks) > SMEM_SM * threads // 768 - 1024
+                         or (rows * ranks < SMS and run_of(ranks) > 24)):
         ranks *= 2
     ranks = int(o.get("ranks") or ranks)
-    _need(smem_of(ranks) <= SMEM_LIMIT,
+    # (a token's index within its CTA's part has 16 bits)
+    _need(smem_of(ranks) <= SMEM_LIMIT and threads * run_of(ranks) <= 65536,
           f"sample: a vocabulary of {vocab} does not fit the shared memory of a cluster")
     return {"rows": rows, "vocab": vocab, "ranks": ranks, "run": run_of(ranks),
-            "smem": smem_of(ranks), "block": SAMPLE_THREADS, "params": list(op.attrs.get("params", ())),
+            "smem": smem_of(ranks), "block": threads,
+            "min_ctas": int(o.get("min_ctas") or max(1, 768 // threads)), "params": list(op.attrs.get("params", ())),
             "flops": 2 * rows * vocab}
 
 
@@ -540,13 +552,12 @@ def _emit_sample(sk, name):
 
 using namespace molten;
 
-static_assert(sizeof(SampleShared) == {SAMPLE_FIXED} && SAMPLE_THREADS == {SAMPLE_THREADS},
-              "the launch's dynamic shared memory");
+static_assert(sizeof(SampleShared<{t}, {sk.config['block']}>) == {_sample_fixed(sk.operands[0].dtype, sk.config['block'])}, "the launch's dynamic shared memory");
 
-extern "C" __global__ void __launch_bounds__({SAMPLE_THREADS}, 3) {name}(const __grid_constant__ SampleArgs args) {{
+extern "C" __global__ void __launch_bounds__({sk.config['block']}, {sk.config['min_ctas']}) {name}(const __grid_constant__ SampleArgs args) {{
   extern __shared__ __align__(16) uint8_t smem_raw[];
   pdl_enter();
-  sample_row<{t}>(args, smem_raw);
+  sample_row<{t}, {sk.config['block']}>(args, smem_raw);
 }}
 """
 
