@@ -163,14 +163,17 @@ struct WindowItem {
     tiles = sink + end - start;
   }
   __device__ __forceinline__ int tile(int u) const { return u < sink ? u : u - sink + start; }
+  // (selects, not an index: the members stay in registers where t is a variable)
+  static __device__ __forceinline__ int of(const int (&x)[2], int t) { return t == 0 ? x[0] : x[1]; }
+  __device__ __forceinline__ bool any(int t) const { return of(pb, t) >= of(pa, t); }
   __device__ __forceinline__ bool need(int t, int j) const {
-    return pb[t] >= pa[t] && (j < need_sink[t] || (j >= lo[t] && j < hi[t]));
+    return any(t) && (j < of(need_sink, t) || (j >= of(lo, t) && j < of(hi, t)));
   }
   // every row of Q tile t sees all of key tile j
   __device__ __forceinline__ bool whole(const WindowTcArgs& a, int t, int j) const {
     const int k = j * 128;
-    return k + 127 <= pa[t] && first + i0 + t * a.positions >= 0 &&
-           (a.window < 0 || k > pb[t] - a.window || k + 128 <= a.sinks);
+    return k + 127 <= of(pa, t) && first + i0 + t * a.positions >= 0 &&
+           (a.window < 0 || k > of(pb, t) - a.window || k + 128 <= a.sinks);
   }
   // V needs no cleaning: whole for each Q tile that needs it, and both do
   __device__ __forceinline__ bool clean(const WindowTcArgs& a, int j) const {
@@ -182,6 +185,10 @@ struct WindowItem {
 // sees are one run (and the sinks).
 __device__ __forceinline__ bool window_tc_any(const WindowTcArgs& a, int pa, int pb, int j) {
   return j <= pb && (a.window < 0 || j > pa - a.window || j < a.sinks);
+}
+// The lowest n bits.
+__device__ __forceinline__ uint32_t window_tc_bits(int n) {
+  return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
 }
 __device__ __forceinline__ bool window_tc_sees(const WindowTcArgs& a, int p, int j) {
   return j <= p && (a.window < 0 || j > p - a.window || j < a.sinks);
@@ -200,38 +207,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
                "setp.ne.b32 p, %4, 0;\n\t"
                "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                :: "r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-// A warp's 32 lanes x 128 columns -> 128 registers a thread (the wait inside:
-// no use of them can move before it).
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&u)[128]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
-               "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-               "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-               "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
-               "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-               "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
-               "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
-               "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127"
-               "}, [%128];\n\t"
-               "tcgen05.wait::ld.sync.aligned;"
-               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
-                 "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]),
-                 "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]),
-                 "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31]),
-                 "=r"(u[32]), "=r"(u[33]), "=r"(u[34]), "=r"(u[35]), "=r"(u[36]), "=r"(u[37]), "=r"(u[38]), "=r"(u[39]),
-                 "=r"(u[40]), "=r"(u[41]), "=r"(u[42]), "=r"(u[43]), "=r"(u[44]), "=r"(u[45]), "=r"(u[46]), "=r"(u[47]),
-                 "=r"(u[48]), "=r"(u[49]), "=r"(u[50]), "=r"(u[51]), "=r"(u[52]), "=r"(u[53]), "=r"(u[54]), "=r"(u[55]),
-                 "=r"(u[56]), "=r"(u[57]), "=r"(u[58]), "=r"(u[59]), "=r"(u[60]), "=r"(u[61]), "=r"(u[62]), "=r"(u[63]),
-                 "=r"(u[64]), "=r"(u[65]), "=r"(u[66]), "=r"(u[67]), "=r"(u[68]), "=r"(u[69]), "=r"(u[70]), "=r"(u[71]),
-                 "=r"(u[72]), "=r"(u[73]), "=r"(u[74]), "=r"(u[75]), "=r"(u[76]), "=r"(u[77]), "=r"(u[78]), "=r"(u[79]),
-                 "=r"(u[80]), "=r"(u[81]), "=r"(u[82]), "=r"(u[83]), "=r"(u[84]), "=r"(u[85]), "=r"(u[86]), "=r"(u[87]),
-                 "=r"(u[88]), "=r"(u[89]), "=r"(u[90]), "=r"(u[91]), "=r"(u[92]), "=r"(u[93]), "=r"(u[94]), "=r"(u[95]),
-                 "=r"(u[96]), "=r"(u[97]), "=r"(u[98]), "=r"(u[99]), "=r"(u[100]), "=r"(u[101]), "=r"(u[102]), "=r"(u[103]),
-                 "=r"(u[104]), "=r"(u[105]), "=r"(u[106]), "=r"(u[107]), "=r"(u[108]), "=r"(u[109]), "=r"(u[110]), "=r"(u[111]),
-                 "=r"(u[112]), "=r"(u[113]), "=r"(u[114]), "=r"(u[115]), "=r"(u[116]), "=r"(u[117]), "=r"(u[118]), "=r"(u[119]),
-                 "=r"(u[120]), "=r"(u[121]), "=r"(u[122]), "=r"(u[123]), "=r"(u[124]), "=r"(u[125]), "=r"(u[126]), "=r"(u[127])
-               : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* u) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
@@ -282,21 +257,24 @@ __device__ __forceinline__ void window_tc_init(const WindowTcShared& s, const Wi
   tc_fence_before();
 }
 
-// Infinities and NaN of V that were cleaned away, added to columns c .. c + 31
-// of the row at position p, from the keys it sees (any weight above 0 carries
-// them into the sum).
-template <typename T>
-__device__ __noinline__ void window_tc_add_dirty(const WindowTcArgs& args, const WindowItem& w, int p,
-                                                 int c, float (&o)[32]) {
+// Infinities and NaN of V that were cleaned away, added to the stored output
+// row of position p from the keys it sees (any weight above 0 carries them into
+// the sum).
+template <typename T, typename OT>
+__device__ __noinline__ void window_tc_add_dirty(const WindowTcArgs& args, int item, int p, OT* dst) {
+  const WindowItem w(args, item);
+#pragma unroll 1
   for (int u = 0; u < w.tiles; ++u) {
     const int j = w.tile(u);
     if (w.clean(args, j)) continue;
+#pragma unroll 1
     for (int key = j * 128; key < j * 128 + 128 && key < w.len; ++key) {
       if (!window_tc_sees(args, p, key)) continue;
-      const T* v = static_cast<const T*>(args.v) + w.b * args.v_b + key * args.v_s + w.h * args.v_h + c;
-      for (int q = 0; q < 32 && c + q < args.dim; ++q) {
-        const float x = to_f32(v[q]);
-        if (!isfinite(x)) o[q] += x;
+      const T* v = static_cast<const T*>(args.v) + w.b * args.v_b + key * args.v_s + w.h * args.v_h;
+#pragma unroll 1
+      for (int c = 0; c < args.dim; ++c) {
+        const float x = to_f32(v[c]);
+        if (!isfinite(x)) dst[c] = from_f32<OT>(to_f32(dst[c]) + x);
       }
     }
   }
@@ -316,8 +294,7 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
   // the cleaning warps through barrier clean(e / 2 % S)
   bool ok = true;
   auto wait = [&](uint32_t b, uint32_t parity) {
-    if (ok && !attn_wait(b, parity & 1u)) { window_tc_fail(s, args); ok = false; }
-    if (*s.abort_flag) ok = false;
+    if (!attn_wait(b, parity & 1u)) { window_tc_fail(s, args); ok = false; }
     return ok;
   };
 
@@ -393,7 +370,7 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
               const uint32_t d = tmem + L::TM_O + 128u * t, p = tmem + L::TM_S + 128u * t;
 #pragma unroll
               for (int kk = 0; kk < 8; ++kk)
-                umma_f16_ts(d, p + 8u * kk, umma_desc(v_base + 2048u * kk, (uint32_t)L::CHUNK, 1024u),
+                umma_f16_ts(d, p + 8u * kk + (kk < 4 ? 0u : 32u), umma_desc(v_base + 2048u * kk, (uint32_t)L::CHUNK, 1024u),
                             IDESC_O, begun[t] || kk != 0 ? 1u : 0u);
               umma_commit(bar.o_full(t));
               begun[t] = true;
@@ -503,7 +480,7 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
       const bool real = r < args.per * args.positions && i < args.nq;
       const int p = w.first + i;
       float mref = -INFINITY, sum = 0.0f;            // maximum the weights are taken from; their sum
-      const bool run = w.pb[t] >= w.pa[t];
+      const bool run = w.any(t);
       if (run) {
         bool begun = false;
         for (int u = 0; u < w.tiles; ++u) {
@@ -517,24 +494,38 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
           }
           ++sn;
           tc_fence_after();
-          uint32_t x[128];
-          tmem_ld128(s_at, x);
+          // 64 columns of S at a time: half a row leaves registers for the rest
+          // (with a whole one in registers spills doubled the time); the lower
+          // half is read twice, a few hundred cycles that the other Q tile's
+          // warp covers
           const bool whole = w.whole(args, t, j);
-          if (!whole) {
-            // columns from c0 on (or below cs) and up to c1 are seen
-            const int c1 = p - j * 128;
-            const int c0 = args.window < 0 ? -1 : p - args.window - j * 128;
-            const int cs = args.sinks - j * 128;
+          // columns behind c0 (or before cs) and up to c1 are seen
+          const int c1 = p - j * 128 + 1;
+          const int c0 = args.window < 0 ? 0 : p - args.window - j * 128 + 1;
+          const int cs = args.sinks - j * 128;
+          float x[64];
+          auto load = [&](int half) {
+            tmem_ld64(s_at + 64 * half, x);
+            if (whole) return;
 #pragma unroll
-            for (int c = 0; c < 128; ++c)
-              if (!(c <= c1 && (c > c0 || c < cs))) x[c] = 0xFF800000u;          // -inf
+            for (int q = 0; q < 2; ++q) {
+              const int k = 64 * half + 32 * q;
+              const uint32_t seen = window_tc_bits(c1 - k) & (~window_tc_bits(c0 - k) | window_tc_bits(cs - k));
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (!(seen >> c & 1u)) x[32 * q + c] = -INFINITY;
+            }
+          };
+          float top[4] = {mref, mref, mref, mref};
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            load(half);
+#pragma unroll
+            for (int c = 0; c < 64; c += 8)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) top[q] = fmaxf(fmaxf(top[q], x[c + q]), x[c + 4 + q]);
           }
-          float top[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) top[q] = __uint_as_float(x[q]);
-#pragma unroll
-          for (int c = 4; c < 128; ++c) top[c % 4] = fmaxf(top[c % 4], __uint_as_float(x[c]));
-          const float mn = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), mref);
+          const float mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
           if (!begun) {
             mref = mn;
           } else if (__any_sync(0xffffffffu, real && mn > mref + slack)) {
@@ -563,32 +554,26 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
           }
           begun = true;
           const float off = mref == -INFINITY ? 0.0f : -mref * C2;
-          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          if (whole) {
+          const float2 scale2 = make_float2(C2, C2), off2 = make_float2(off, off);
+          float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-            for (int c = 0; c < 128; ++c) {
-              const float e = attn_exp2<POLY>(c, fmaf(__uint_as_float(x[c]), C2, off));
-              part[c % 4] += e;
-              x[c] = __float_as_uint(e);
+          for (int half = 1; half >= 0; --half) {
+            if (half == 0) load(0);
+            uint32_t y[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              float2 e = ffma2(make_float2(x[2 * c], x[2 * c + 1]), scale2, off2);
+              e.x = attn_exp2<POLY>(2 * c, e.x);
+              e.y = attn_exp2<POLY>(2 * c + 1, e.y);
+              part[c % 2] = fadd2(part[c % 2], e);
+              Slot<T, 2> two;
+              const float f[2] = {e.x, e.y};
+              pack_slot<T, 2>(two, f);
+              y[c] = *reinterpret_cast<const uint32_t*>(&two);
             }
-          } else {
-#pragma unroll
-            for (int c = 0; c < 128; ++c) {
-              const float e = fast_exp2(fmaf(__uint_as_float(x[c]), C2, off));
-              part[c % 4] += e;
-              x[c] = __float_as_uint(e);
-            }
+            tmem_st32(s_at + 64 * half, y);          // (each half's P over its own S)
           }
-          sum += (part[0] + part[1]) + (part[2] + part[3]);
-#pragma unroll
-          for (int c = 0; c < 64; ++c) {
-            Slot<T, 2> two;
-            const float f[2] = {__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])};
-            pack_slot<T, 2>(two, f);
-            x[c] = *reinterpret_cast<const uint32_t*>(&two);
-          }
-          tmem_st32(s_at, x);
-          tmem_st32(s_at + 32, x + 32);
+          sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
@@ -615,7 +600,6 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
         if (c >= args.dim) continue;
 #pragma unroll
         for (int q = 0; q < 32; ++q) o[q] = sum == 0.0f ? 0.0f : o[q] * inv;
-        if (dirty && real) window_tc_add_dirty<T>(args, w, p, c, o);
         if (real) {
 #pragma unroll
           for (int q = 0; q < 32; q += 8) {
@@ -626,6 +610,7 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
           }
         }
       }
+      if (dirty && real) window_tc_add_dirty<T, OT>(args, it, p, dst);
       if (run) {
         tc_fence_before();
         __syncwarp();
