@@ -22,12 +22,21 @@
 //                rounded to the type of V (the tensor core takes operands of
 //                one type; relative 2^-9 or 2^-12 a weight) back to TMEM.
 //
-// Bound by the tensor core (4 D operations a visible pair) and, next to it, by
-// the EX2 unit: a 128 x 128 tile takes some 1024 cycles of either.  O is
-// rescaled only when a row's maximum has grown by more than 2^8 since the last
-// time: the weights stay below 2^8 and O and the sum share the factor, so
-// nothing is lost, and most rescales (each a round trip of O through
-// registers) never happen.
+// A 128 x 128 tile takes some 1024 cycles of the tensor core (4 D operations a
+// visible pair) and as many of the EX2 unit; what bounds it is the chain of one
+// Q tile: S, the exponentials of its halves, P V.  P is handed over by halves,
+// so the first half's P V runs under the second's exponentials, and a logit is
+// read once: weights are taken from an offset that moves, with O and the sum
+// rescaled, only when a logit exceeds it by more than 2^8, so there is no pass
+// for the maximum first.  The weights stay below 2^8 and O and the sum share the
+// factor, so nothing is lost.
+//
+// Measured: 8192 tokens, 32 heads over 8, head dim 128, window 2048: 271 us (889
+// TFLOP/s of visible pairs); 4 x 500 tokens over up to 2900, head dim 64, window
+// 1000: 28 us.  With a whole row of S in registers (spills) the first took 489,
+// with its maximum first 314.  S by halves, so that it can be computed ahead:
+// 285 (N = 64 takes the tensor core as long as N = 128); an issuing warp for
+// each Q tile: 325; 4 of 32 exponentials on the FMA pipe: 274.
 //
 // P = 0 times an infinity or NaN is NaN, so V rows that no query of the item
 // sees (behind the length, before the window) are zeroed in shared memory
@@ -71,8 +80,8 @@ struct WindowTcLayout {
   static constexpr int STAGE_BYTES = DCH * CHUNK;    // one K or V tile
   static constexpr int RING_OFFSET = 2 * Q_BYTES;
   static constexpr int BAR_OFFSET = RING_OFFSET + STAGES * STAGE_BYTES;
-  // full[S] empty[S] clean[S] q_full[2] q_empty[2] s_full[2] p_full[2] o_full[2] o_free[2] done
-  static constexpr int NUM_BARS = 3 * STAGES + 13;
+  // full[S] empty[S] clean[S] q_full[2] q_empty[2] s_full[2] p_full[4] o_half[2] o_full[2] o_free[2] done
+  static constexpr int NUM_BARS = 3 * STAGES + 17;
   static constexpr int SMEM_BYTES = BAR_OFFSET + NUM_BARS * 8 + 8 + 8 * 4 + 8 + 1024;
   static constexpr int THREADS = 384;
   static constexpr uint32_t TM_S = 0, TM_O = 256;    // + 128 for Q tile 1
@@ -86,7 +95,8 @@ template <class L> struct WindowTcBars {
   __device__ __forceinline__ uint32_t q_full(int t) const { return base + 8u * (3 * L::STAGES + t); }
   __device__ __forceinline__ uint32_t q_empty(int t) const { return base + 8u * (3 * L::STAGES + 2 + t); }
   __device__ __forceinline__ uint32_t s_full(int t) const { return base + 8u * (3 * L::STAGES + 4 + t); }
-  __device__ __forceinline__ uint32_t p_full(int t) const { return base + 8u * (3 * L::STAGES + 6 + t); }
+  __device__ __forceinline__ uint32_t p_full(int t, int half) const { return base + 8u * (3 * L::STAGES + 13 + 2 * t + half); }
+  __device__ __forceinline__ uint32_t o_half(int t) const { return base + 8u * (3 * L::STAGES + 6 + t); }
   __device__ __forceinline__ uint32_t o_full(int t) const { return base + 8u * (3 * L::STAGES + 8 + t); }
   __device__ __forceinline__ uint32_t o_free(int t) const { return base + 8u * (3 * L::STAGES + 10 + t); }
   __device__ __forceinline__ uint32_t done() const { return base + 8u * (3 * L::STAGES + 12); }
@@ -223,6 +233,13 @@ __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// One lane of a converged warp, the same at each call.
+__device__ __forceinline__ bool window_tc_elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0u;
+}
+
 template <class L>
 __device__ __forceinline__ void window_tc_init(const WindowTcShared& s, const WindowTcArgs& args) {
   const int tid = threadIdx.x, warp = tid / 32;
@@ -237,7 +254,9 @@ __device__ __forceinline__ void window_tc_init(const WindowTcShared& s, const Wi
       mbar_init(b.q_full(t), 1);
       mbar_init(b.q_empty(t), 1);
       mbar_init(b.s_full(t), 1);
-      mbar_init(b.p_full(t), 4);                     // the Q tile's softmax warps
+      mbar_init(b.p_full(t, 0), 4);                  // the Q tile's softmax warps
+      mbar_init(b.p_full(t, 1), 4);
+      mbar_init(b.o_half(t), 1);
       mbar_init(b.o_full(t), 1);
       mbar_init(b.o_free(t), 4);
     }
@@ -280,7 +299,7 @@ __device__ __noinline__ void window_tc_add_dirty(const WindowTcArgs& args, int i
   }
 }
 
-template <class L, typename T, typename OT, int POLY>
+template <class L, typename T, typename OT>
 __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const WindowTcArgs& args) {
   constexpr bool F16IN = std::is_same<T, f16>::value;
   constexpr uint32_t S = L::STAGES;
@@ -344,74 +363,109 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
     }
   } else if (warp == 1) {
     // --------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    // (the whole warp takes these steps, so that what describes an MMA is the
+    // same in every lane and held in uniform registers; one lane issues.  With
+    // the steps in one lane only, each MMA took as long to issue as to run)
+    {
+      const bool leader = window_tc_elect();
+      auto wait_all = [&](uint32_t b, uint32_t parity) {
+        ok = __all_sync(0xffffffffu, attn_wait(b, parity & 1u));
+        if (!ok && lane == 0) window_tc_fail(s, args);
+        return ok;
+      };
       constexpr uint32_t IDESC_S = umma_idesc<128, 128, F16IN, true>();
       constexpr uint32_t IDESC_O = umma_idesc<128, L::DP, F16IN, false>();
-      uint32_t n = 0;                                // key tiles done
       uint32_t qn[2] = {0, 0}, pn[2] = {0, 0}, on[2] = {0, 0};   // Q tiles, P tiles, items of O
+      // the next ring entry and the next V's cleaning barrier, with their parities
+      uint32_t st = 0, ph = 0, cst = 0, cph = 0;
+      auto advance = [](uint32_t& at, uint32_t& parity) {
+        if (++at == S) { at = 0; parity ^= 1u; }
+      };
+      // descriptors without their address (it is added in units of 16 bytes)
+      const uint64_t by_row = umma_desc(0u, 16u, 1024u), by_col = umma_desc(0u, (uint32_t)L::CHUNK, 1024u);
+      const uint32_t q_at = smem_u32(s.q) >> 4, ring_at = smem_u32(s.ring) >> 4;
       for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
         const WindowItem w(args, it);
-        bool begun[2] = {false, false};              // O_t holds this item's sums
+        bool begun[2] = {false, false}, asked[2] = {false, false};   // O_t holds sums; Q_t is there
+        bool needed[2] = {false, false};             // by Q tile t: the key tile before
         // step u: P V of tile u - 1 and S of tile u, for either Q tile in turn
         for (int u = 0; u <= w.tiles && w.tiles > 0 && ok; ++u) {
-          const int j = u < w.tiles ? w.tile(u) : -1, prev = u > 0 ? w.tile(u - 1) : -1;
-          const uint32_t ke = 2u * (n + u), ve = ke - 1u;        // ring entries of K_u, V_u-1
-          if (j >= 0 && !wait(bar.full(ke % S), ke / S)) break;
-          if (prev >= 0) {
-            if (!wait(bar.full(ve % S), ve / S) || !wait(bar.clean(ve / 2u % S), ve / 2u / S)) break;
+          const bool has_k = u < w.tiles, has_v = u > 0;
+          const int j = has_k ? w.tile(u) : 0;
+          uint32_t v_st = 0, k_st = 0;
+          if (has_v) {
+            if (!wait_all(bar.clean(cst), cph)) break;   // (the cleaning warps have waited for the tile)
+            v_st = st;
+            advance(st, ph);
+            advance(cst, cph);
           }
+          if (has_k) {
+            if (!wait_all(bar.full(st), ph)) break;
+            k_st = st;
+            advance(st, ph);
+          }
+          const uint64_t v_desc = by_col + (ring_at + v_st * (uint32_t)(L::STAGE_BYTES / 16));
+          const uint64_t k_desc = by_row + (ring_at + k_st * (uint32_t)(L::STAGE_BYTES / 16));
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (prev >= 0 && w.need(t, prev)) {
-              if (!begun[t] && !wait(bar.o_free(t), on[t]++ + 1u)) break;
-              if (!wait(bar.p_full(t), pn[t]++)) break;
-              tc_fence_after();
-              const uint32_t v_base = smem_u32(s.ring + (ve % S) * L::STAGE_BYTES);
+            if (has_v && needed[t]) {
+              if (!begun[t] && !wait_all(bar.o_free(t), on[t]++ + 1u)) break;
               const uint32_t d = tmem + L::TM_O + 128u * t, p = tmem + L::TM_S + 128u * t;
 #pragma unroll
-              for (int kk = 0; kk < 8; ++kk)
-                umma_f16_ts(d, p + 8u * kk + (kk < 4 ? 0u : 32u), umma_desc(v_base + 2048u * kk, (uint32_t)L::CHUNK, 1024u),
-                            IDESC_O, begun[t] || kk != 0 ? 1u : 0u);
-              umma_commit(bar.o_full(t));
+              for (int half = 0; half < 2; ++half) {
+                if (!wait_all(bar.p_full(t, half), pn[t])) break;
+                tc_fence_after();
+                if (leader) {
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                  umma_f16_ts(d, p + 64u * half + 8u * kk, v_desc + 128u * (4 * half + kk), IDESC_O,
+                              begun[t] || (half | kk) != 0 ? 1u : 0u);
+                if (half == 0) umma_commit(bar.o_half(t));
+                }
+              }
+              if (!ok) break;
+              ++pn[t];
               begun[t] = true;
             }
-            if (j >= 0 && w.need(t, j)) {
+            needed[t] = has_k && w.need(t, j);
+            if (needed[t]) {
               // (S_t is free: its last P has been used, and MMAs run in order)
-              if (!(qn[t] & 0x80000000u)) {
-                if (!wait(bar.q_full(t), qn[t])) break;
-                qn[t] |= 0x80000000u;                // waited for in this item
+              if (!asked[t]) {
+                if (!wait_all(bar.q_full(t), qn[t]++)) break;
+                asked[t] = true;
               }
               tc_fence_after();
               const uint32_t d = tmem + L::TM_S + 128u * t;
-              const uint32_t a_base = smem_u32(s.q + t * L::Q_BYTES);
-              const uint32_t b_base = smem_u32(s.ring + (ke % S) * L::STAGE_BYTES);
+              const uint64_t q_desc = by_row + (q_at + t * (uint32_t)(L::Q_BYTES / 16));
+              if (leader) {
 #pragma unroll
               for (int c = 0; c < L::DCH; ++c)
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
-                  umma_f16(d, umma_desc(a_base + c * L::CHUNK + 32u * kk, 16u, 1024u),
-                           umma_desc(b_base + c * L::CHUNK + 32u * kk, 16u, 1024u), IDESC_S,
-                           (c | kk) != 0 ? 1u : 0u);
+                  umma_f16(d, q_desc + (uint32_t)(c * (L::CHUNK / 16) + 2 * kk),
+                           k_desc + (uint32_t)(c * (L::CHUNK / 16) + 2 * kk), IDESC_S, (c | kk) != 0 ? 1u : 0u);
               umma_commit(bar.s_full(t));
+              }
             }
           }
           if (!ok) break;
-          if (prev >= 0) umma_commit(bar.empty(ve % S));
-          if (j >= 0) umma_commit(bar.empty(ke % S));
-          if (u == w.tiles - 1) {
+          if (leader) {
+            if (has_v) umma_commit(bar.empty(v_st));
+            if (has_k) umma_commit(bar.empty(k_st));
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-              if (qn[t] & 0x80000000u) {             // the item's last S: Q_t is free
-                umma_commit(bar.q_empty(t));
-                qn[t] = (qn[t] & 0x7fffffffu) + 1u;
-              }
+            for (int t = 0; t < 2; ++t) {
+              if (u == w.tiles - 1 && asked[t]) umma_commit(bar.q_empty(t));     // the item's last S
+              if (u == w.tiles && begun[t]) umma_commit(bar.o_full(t));          // its last P V
+            }
           }
+          __syncwarp();
         }
-        n += (uint32_t)w.tiles;
       }
       // all MMAs this thread issued must finish before TMEM is released
-      umma_commit(bar.done());
-      if (!attn_wait(bar.done(), 0u)) { if (args.status) atomicOr(args.status, kWindowTimeout); }
+      if (leader) {
+        umma_commit(bar.done());
+        if (!attn_wait(bar.done(), 0u)) { if (args.status) atomicOr(args.status, kWindowTimeout); }
+      }
     }
   } else if (warp < 4) {
     // ----------------------------------------------------------- cleaning
@@ -439,7 +493,7 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
           const bool all = key <= pa && (args.window < 0 || key > pb - args.window || key < args.sinks);
           if (any && all) continue;
           uint8_t* row = s.ring + (e % S) * L::STAGE_BYTES + r * 128;
-#pragma unroll 1
+#pragma unroll 4
           for (int q = 0; q < L::DCH * 8; ++q) {     // 16-byte chunks, the lanes' on different banks
             uint4* at = reinterpret_cast<uint4*>(row + (q >> 3) * L::CHUNK + (((q + lane) & 7) << 4));
             if (!any) { *at = make_uint4(0u, 0u, 0u, 0u); continue; }
@@ -473,13 +527,14 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
     const uint32_t o_at = tmem + lane_at + L::TM_O + 128u * t;
     const float C2 = args.scale_log2;
     const float slack = 8.0f / C2;                   // growth of the maximum left in the weights
-    uint32_t sn = 0, seq = 0;
+    uint32_t sn = 0, rn = 0, seq = 0;                // tiles of S; items with any
     for (int it = blockIdx.x; it < items && ok; it += gridDim.x, ++seq) {
       const WindowItem w(args, it);
       const int i = w.i0 + t * args.positions + r / args.per;    // this row's query
       const bool real = r < args.per * args.positions && i < args.nq;
       const int p = w.first + i;
-      float mref = -INFINITY, sum = 0.0f;            // maximum the weights are taken from; their sum
+      // weights are 2^(x C2 + off); a logit above `limit` moves `off`
+      float off = 0.0f, limit = -INFINITY, sum = 0.0f;
       const bool run = w.any(t);
       if (run) {
         bool begun = false;
@@ -494,77 +549,76 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
           }
           ++sn;
           tc_fence_after();
-          // 64 columns of S at a time: half a row leaves registers for the rest
-          // (with a whole one in registers spills doubled the time); the lower
-          // half is read twice, a few hundred cycles that the other Q tile's
-          // warp covers
+          // 64 columns of S at a time, each read once: half a row leaves registers
+          // for the rest (a whole one spilled, at twice the time), and its P V
+          // runs under the other half's exponentials
           const bool whole = w.whole(args, t, j);
           // columns behind c0 (or before cs) and up to c1 are seen
           const int c1 = p - j * 128 + 1;
           const int c0 = args.window < 0 ? 0 : p - args.window - j * 128 + 1;
           const int cs = args.sinks - j * 128;
-          float x[64];
-          auto load = [&](int half) {
-            tmem_ld64(s_at + 64 * half, x);
-            if (whole) return;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int k = 64 * half + 32 * q;
-              const uint32_t seen = window_tc_bits(c1 - k) & (~window_tc_bits(c0 - k) | window_tc_bits(cs - k));
-#pragma unroll
-              for (int c = 0; c < 32; ++c)
-                if (!(seen >> c & 1u)) x[32 * q + c] = -INFINITY;
-            }
-          };
-          float top[4] = {mref, mref, mref, mref};
-#pragma unroll
+#pragma unroll 1
           for (int half = 0; half < 2; ++half) {
-            load(half);
+            float x[64];
+            tmem_ld64(s_at + 64 * half, x);
+            if (!whole) {
 #pragma unroll
-            for (int c = 0; c < 64; c += 8)
+              for (int q = 0; q < 2; ++q) {
+                const int k = 64 * half + 32 * q;
+                const uint32_t seen = window_tc_bits(c1 - k) & (~window_tc_bits(c0 - k) | window_tc_bits(cs - k));
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                  if (!(seen >> c & 1u)) x[32 * q + c] = -INFINITY;
+              }
+            }
+            float top[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) top[q] = fmaxf(x[q], x[q + 4]);
+#pragma unroll
+            for (int c = 8; c < 64; c += 8)
 #pragma unroll
               for (int q = 0; q < 4; ++q) top[q] = fmaxf(fmaxf(top[q], x[c + q]), x[c + 4 + q]);
-          }
-          const float mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-          if (!begun) {
-            mref = mn;
-          } else if (__any_sync(0xffffffffu, real && mn > mref + slack)) {
-            // rescale O once P V of the last tile is done
-            const bool done = attn_wait(bar.o_full(t), sn & 1u);         // (its number is sn - 2)
-            if (!__all_sync(0xffffffffu, done ? 1 : 0)) {
-              if (lane == 0) window_tc_fail(s, args);
-              ok = false;
-              break;
-            }
-            tc_fence_after();
+            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             // (each row by its own maximum: no row's result depends on another's)
-            const bool grown = real && mn > mref + slack;
-            const float fix = !grown ? 1.0f : mref == -INFINITY ? 0.0f : fast_exp2((mref - mn) * C2);
-            sum *= fix;
-            if (grown) mref = mn;
+            const bool grown = real && mx > limit;
+            if (__any_sync(0xffffffffu, grown)) {
+              const float moved = grown ? -mx * C2 : off;
+              // (the first maximum of a row: O and the sum are 0)
+              const float fix = grown && limit > -INFINITY ? fast_exp2(moved - off) : 1.0f;
+              off = moved;
+              limit = grown ? mx + slack : limit;
+              sum *= fix;
+              // P V of all tiles before is done (their S came first); of this one's
+              // first half it may be running
+              if (half == 1) {
+                const bool done = attn_wait(bar.o_half(t), (sn + 1u) & 1u);      // (tile sn - 1)
+                if (!__all_sync(0xffffffffu, done ? 1 : 0)) {
+                  if (lane == 0) window_tc_fail(s, args);
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
+              }
+              if (begun || half == 1) {
 #pragma unroll 1
-            for (int c = 0; c < L::DP; c += 32) {
-              float o[32];
-              tmem_ld32(o_at + c, o);
-              uint32_t y[32];
+                for (int c = 0; c < L::DP; c += 32) {
+                  float o[32];
+                  tmem_ld32(o_at + c, o);
+                  uint32_t y[32];
 #pragma unroll
-              for (int q = 0; q < 32; ++q) y[q] = __float_as_uint(o[q] * fix);
-              tmem_st32(o_at + c, y);
+                  for (int q = 0; q < 32; ++q) y[q] = __float_as_uint(o[q] * fix);
+                  tmem_st32(o_at + c, y);
+                }
+              }
             }
-          }
-          begun = true;
-          const float off = mref == -INFINITY ? 0.0f : -mref * C2;
-          const float2 scale2 = make_float2(C2, C2), off2 = make_float2(off, off);
-          float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-          for (int half = 1; half >= 0; --half) {
-            if (half == 0) load(0);
+            const float2 scale2 = make_float2(C2, C2), off2 = make_float2(off, off);
+            float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
             uint32_t y[32];
 #pragma unroll
             for (int c = 0; c < 32; ++c) {
               float2 e = ffma2(make_float2(x[2 * c], x[2 * c + 1]), scale2, off2);
-              e.x = attn_exp2<POLY>(2 * c, e.x);
-              e.y = attn_exp2<POLY>(2 * c + 1, e.y);
+              e.x = fast_exp2(e.x);
+              e.y = fast_exp2(e.y);
               part[c % 2] = fadd2(part[c % 2], e);
               Slot<T, 2> two;
               const float f[2] = {e.x, e.y};
@@ -572,15 +626,17 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
               y[c] = *reinterpret_cast<const uint32_t*>(&two);
             }
             tmem_st32(s_at + 64 * half, y);          // (each half's P over its own S)
+            sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar.p_full(t, half));
           }
-          sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar.p_full(t));
+          if (!ok) break;
+          begun = true;
         }
         if (!ok) break;
-        const bool done = attn_wait(bar.o_full(t), (sn + 1u) & 1u);
+        const bool done = attn_wait(bar.o_full(t), rn++ & 1u);
         if (!__all_sync(0xffffffffu, done && !*s.abort_flag)) {
           if (lane == 0) window_tc_fail(s, args);
           ok = false;
@@ -593,20 +649,34 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
       OT* dst = static_cast<OT*>(args.out) +
                 (((long long)w.b * args.nq + i) * args.kv_heads * args.per + w.h * args.per + r % args.per) *
                     (long long)args.dim;
+      // whole sectors where rows start on one (each lane writes its own row)
+      const bool wide = args.dim % 16 == 0 && (reinterpret_cast<uintptr_t>(args.out) & 31u) == 0u;
 #pragma unroll 1
       for (int c = 0; c < L::DP; c += 32) {
         float o[32];
         if (run) tmem_ld32(o_at + c, o);             // (the whole warp)
         if (c >= args.dim) continue;
+        uint32_t y[16];
 #pragma unroll
-        for (int q = 0; q < 32; ++q) o[q] = sum == 0.0f ? 0.0f : o[q] * inv;
-        if (real) {
+        for (int q = 0; q < 16; ++q) {
+          Slot<OT, 2> two;
+          const float f[2] = {sum == 0.0f ? 0.0f : o[2 * q] * inv, sum == 0.0f ? 0.0f : o[2 * q + 1] * inv};
+          pack_slot<OT, 2>(two, f);
+          y[q] = *reinterpret_cast<const uint32_t*>(&two);
+        }
+        if (!real) continue;
 #pragma unroll
-          for (int q = 0; q < 32; q += 8) {
-            if (c + q >= args.dim) break;
-            Slot<OT, 8> so;
-            pack_slot<OT, 8>(so, *reinterpret_cast<const float(*)[8]>(&o[q]));
-            store_slot<kStoreDefault, OT, 8>(dst + c + q, so);
+        for (int q = 0; q < 2; ++q) {
+          if (c + 16 * q >= args.dim) break;
+          uint32_t* at = reinterpret_cast<uint32_t*>(dst + c + 16 * q);
+          const uint32_t* v = y + 8 * q;
+          if (wide) {
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                         :: "l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                            "r"(v[7]) : "memory");
+          } else {
+            *reinterpret_cast<uint4*>(at) = make_uint4(v[0], v[1], v[2], v[3]);
+            if (c + 16 * q + 8 < args.dim) *reinterpret_cast<uint4*>(at + 4) = make_uint4(v[4], v[5], v[6], v[7]);
           }
         }
       }

@@ -36,7 +36,6 @@ SMEM_SM = 228 * 1024
 WINDOW_MAX_DIM = 128
 WINDOW_FEW_ROWS = 32              # rows of a key head up to which the few-row kernel runs
 WINDOW_STAGES, WINDOW_TILE = 3, 16
-WINDOW_POLY = 0                   # exponentials of every 32 on the FMA pipe
 
 SAMPLE_FIXED = 2 * 8 * 24 + 32 * 24 + 2048 + 4096 + 2 * 2048 + 64   # of SampleShared (molten/sample.cuh)
 
@@ -382,12 +381,11 @@ def _plan_window_tiles(c: dict, o: dict) -> dict:
     _need(items < 2 ** 31, "window_attention: sizes beyond the kernel's range")
     dch = dp // 64
     stages = int(o.get("stages") or (5 if dp == 128 else 10))
-    bars = 3 * stages + 13
+    bars = 3 * stages + 17
     smem = 2 * dch * 16384 + stages * dch * 16384 + bars * 8 + 48 + 1024
     _need(smem <= SMEM_LIMIT, f"window_attention: {stages} stages need {smem} bytes")
-    poly = int(o.get("poly", WINDOW_POLY))
     c.update(kind="tiles", positions=positions, blocks=blocks, items=items, stages=stages,
-             smem=smem, block=384, poly=poly, ranks=1, parts=1)
+             smem=smem, block=384, ranks=1, parts=1)
     return c
 
 
@@ -516,7 +514,7 @@ extern "C" __global__ void __launch_bounds__({c['block']}, 1) {name}(const __gri
   window_tc_init<Layout_{name}>(sh, args);     // mbarriers + TMEM allocation
   pdl_enter();                                 // no global access before this
   __syncthreads();
-  window_tc_roles<Layout_{name}, {t}, {ot}, {c['poly']}>(sh, args);
+  window_tc_roles<Layout_{name}, {t}, {ot}>(sh, args);
   tc_fence_before();
   __syncthreads();
   window_tc_teardown<Layout_{name}>(sh);       // TMEM release
