@@ -36,7 +36,8 @@
 // 1000: 28 us.  With a whole row of S in registers (spills) the first took 489,
 // with its maximum first 314.  S by halves, so that it can be computed ahead:
 // 285 (N = 64 takes the tensor core as long as N = 128); an issuing warp for
-// each Q tile: 325; 4 of 32 exponentials on the FMA pipe: 274.
+// each Q tile: 325; 4 of 32 exponentials on the FMA pipe: 274; two softmax
+// threads a row (16 warps of 96 registers, spills): 387.
 //
 // P = 0 times an infinity or NaN is NaN, so V rows that no query of the item
 // sees (behind the length, before the window) are zeroed in shared memory
