@@ -213,50 +213,67 @@ def _plan_q4(op, sk, tune) -> dict:
     o = tune.get("q4") or {}
     groups, w = s.shape[1], group // 32
     planes = 3 if x.dtype == "float32" else 1
-    # up to 8 rows: small CTAs, several to an SM, one tile's latency behind
-    # another's; more rows: an SM's warps share one staged x
-    warps = int(o.get("warps") or (8 if nt == 1 else 16))
-    few = n <= 16 * 2 * SMS                           # one tile for each of two CTAs an SM
-    # the warps of a CTA split k, as far as there are groups for them
-    warps_n = int(o.get("warps_n") or (1 if few else 2))
-    while "warps_n" not in o and warps_n < warps and warps // warps_n > groups:
-        warps_n *= 2
-    tiles = -(-n // (16 * warps_n))
-    warps_k = warps // warps_n
-    # few row tiles: a cluster per tile splits k until every SM has a CTA, as
-    # long as each warp keeps a group
-    ksplit = 1
-    while ksplit < Q4_MAX_KSPLIT and tiles * ksplit < SMS and groups >= 2 * ksplit * warps_k:
-        ksplit *= 2
-    ksplit = int(o.get("ksplit") or ksplit)
-    occupancy = int(o.get("occupancy") or (1 if warps > 8 else 2 if few else 3))
-    limit = (SMEM_SM // occupancy - 1024) // 1024 * 1024
-    per_cta = -(-groups // ksplit)                    # groups of one CTA
-    group_bytes = m * (planes * 64 * w + 8)
-    fixed = 16 + 2 * warps * nt * 128 * 4
-    sums = warps_n * 16 * m * 4                       # of one tile
-    if warps == 8 and fixed + per_cta * group_bytes > limit and "occupancy" not in o:
-        occupancy, limit = 2, SMEM_SM // 2 - 1024
-    # x is staged whole where it fits, else in the fewest equal chunks
-    chunk, chunks = per_cta, 1
-    if fixed + per_cta * group_bytes + (Q4_SUMS_BYTES if ksplit > 1 else 0) > limit:
-        room = limit - Q4_SUMS_BYTES - fixed
-        _need(room >= group_bytes, f"matvec_q4: {m} rows of K = {k} do not fit")
-        chunks = -(-per_cta // (room // group_bytes))
-        chunk = -(-per_cta // chunks)
-    keep = chunks > 1 or ksplit > 1                   # tiles' sums stay in shared memory
-    teams = max(1, min(tiles, SMS * occupancy // ksplit))
-    if keep:
-        teams = max(teams, -(-tiles // max(1, Q4_SUMS_BYTES // sums)))
-    tiles_per_cta = -(-tiles // teams)
-    smem = fixed + chunk * group_bytes + (tiles_per_cta * sums if keep else 0)
-    _need(smem <= SMEM_LIMIT, f"matvec_q4: {m} rows of K = {k} do not fit")
-    depth = int(o.get("depth") or 2)
-    return {"m": m, "n": n, "k": k, "group": group, "nt": nt, "warps": warps, "warps_n": warps_n,
-            "tiles": tiles, "ksplit": ksplit, "depth": depth, "zeros": len(sk.operands) == 4,
-            "chunk": chunk, "min_ctas": occupancy, "teams": teams,
-            "tiles_per_cta": tiles_per_cta, "smem": smem, "block": 32 * warps,
-            "flops": 2 * m * n * k}
+
+    def layout(warps, warps_n, ksplit, occupancy):
+        """One way to run it, or None: warps of a CTA, of these along the rows
+        of q, CTAs of a cluster along k, CTAs of an SM."""
+        # the warps of a CTA split k, as far as there are groups for them
+        while "warps_n" not in o and warps_n < warps and warps // warps_n > groups:
+            warps_n *= 2
+        tiles = -(-n // (16 * warps_n))
+        limit = (SMEM_SM // occupancy - 1024) // 1024 * 1024
+        per_cta = -(-groups // ksplit)                # groups of one CTA
+        if ksplit > groups:                           # (one would have none)
+            return None
+        group_bytes = m * (planes * 64 * w + 8)
+        fixed = 16 + 2 * warps * nt * 128 * 4
+        sums = warps_n * 16 * m * 4                   # of one tile
+        # x is staged whole where it fits, else in the fewest equal chunks
+        chunk, chunks = per_cta, 1
+        if fixed + per_cta * group_bytes + (Q4_SUMS_BYTES if ksplit > 1 else 0) > limit:
+            room = limit - Q4_SUMS_BYTES - fixed
+            if room < group_bytes:
+                return None
+            chunks = -(-per_cta // (room // group_bytes))
+            chunk = -(-per_cta // chunks)
+        keep = chunks > 1 or ksplit > 1               # tiles' sums stay in shared memory
+        teams = max(1, min(tiles, SMS * occupancy // ksplit))
+        if keep:
+            teams = max(teams, -(-tiles // max(1, Q4_SUMS_BYTES // sums)))
+        tiles_per_cta = -(-tiles // teams)
+        smem = fixed + chunk * group_bytes + (tiles_per_cta * sums if keep else 0)
+        if smem > SMEM_LIMIT:
+            return None
+        # microseconds, from 850 measured layouts of 23 shapes (one in six off by a
+        # third): the first term is instructions issued, the next two a warp's
+        # latency a group, then staging x by the SM and by a CTA, a tile's end, and
+        # what splitting k over CTAs costs
+        waves = -(-teams * ksplit // (SMS * occupancy))
+        ctas = min(occupancy, -(-teams * ksplit // SMS))
+        rounds = tiles_per_cta * waves
+        warps_k = warps // warps_n
+        steps = rounds * sum(-(-min(chunk, per_cta - i * chunk) // warps_k) for i in range(chunks))
+        columns, staged = nt * planes, waves * per_cta * m * group * planes
+        split = ksplit.bit_length() - 1
+        cost = (0.0103 * ctas * warps * steps * columns + (0.071 * w + 0.18) * steps
+                + staged * (0.045 * ctas / 1024 + 1.66 / (2048 * warps)) + 1.09 * chunks * waves
+                + rounds * (0.24 * chunks + 0.0083 * ctas * warps * columns + 0.01 * keep * m)
+                + (1.14 + 0.42 * (rounds - 1)) * split + (0.17 * rounds if split else 0.0))
+        return cost, {"m": m, "n": n, "k": k, "group": group, "nt": nt, "warps": warps, "warps_n": warps_n,
+                      "tiles": tiles, "ksplit": ksplit, "depth": int(o.get("depth") or 2),
+                      "zeros": len(sk.operands) == 4, "chunk": chunk, "min_ctas": occupancy, "teams": teams,
+                      "tiles_per_cta": tiles_per_cta, "smem": smem, "block": 32 * warps,
+                      "flops": 2 * m * n * k}
+
+    # 24 warps an SM only with one column block of one plane (registers)
+    shapes = [(8, 3), (8, 2), (16, 1)] if nt == 1 and planes == 1 else [(8, 2), (16, 1)]
+    ways = [layout(int(o.get("warps") or warps), int(o.get("warps_n") or warps_n), int(o.get("ksplit") or ksplit),
+                   int(o.get("occupancy") or occupancy))
+            for warps, occupancy in shapes for warps_n in (1, 2, 4)
+            for ksplit in (1, 2, 4, 8) if ksplit <= Q4_MAX_KSPLIT]
+    ways = [way for way in ways if way]
+    _need(ways, f"matvec_q4: {m} rows of K = {k} do not fit")
+    return min(ways, key=lambda way: way[0])[1]
 
 
 def _plan_rope(op, sk, tune) -> dict:
