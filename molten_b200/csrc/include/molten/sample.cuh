@@ -34,9 +34,10 @@
 // each filter, 158 us; the same unfiltered 103 us (0.99 TB/s).
 //
 // Only the tail that top_p surely drops, of which it needs nothing but the
-// total, is summed in fp32: its error, near 1e-9 of the whole, moves the border
-// past a token (of some 1e-5 of the whole) for one row in 10^4, and that one
-// token's presence changes the draw once in 10^2 or less.
+// total, has fp32 terms (summed by a thread, then in fp64).  Each is off by up to
+// some 2^-20, without a common part, so the total of thousands by near 1e-8 of
+// itself; that moves the border past a token (of some 1e-5 of the whole) for one
+// row in 10^3 or fewer, and the token at the border is one of the least likely.
 //
 // All CTAs of a cluster compute the same values from the same numbers, so they
 // take the same steps.
@@ -720,7 +721,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
     if (rank == 0 && tid == 0) a.out[row] = -1;
     return;
   }
-  if (!(temperature > 0.0f)) {
+  if (!(temperature >= 1e-30f)) {                    // (1 / temperature stays a float)
     // (the first of the ranks' first indexes, as two halves of 16 bits)
     int at = 0x7fffffff;
     sm_each(mine, a.run, [&](int i, float x) {
@@ -769,11 +770,14 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
     // the tokens from there up; the weight of the rest, in fp32
     int hits = 0;
     float rest = 0.0f;
-    const float c1 = (float)k.c * (1.0f / 256.0f);
+    // (two floats: an error of the factor would be the same in every term)
+    const float c1 = (float)(k.c / 256.0), c1_low = (float)(k.c / 256.0 - (double)c1);
     if (by_weight && top_p < 1.0f)
       sm_each(mine, a.run, [&](int, float x) {
         hits += x >= from ? 1 : 0;
-        rest += x >= from ? 0.0f : fast_exp2((x - k.m) * c1);
+        const float d = x - k.m;
+        const float e = fast_exp2(fmaf(d, c1, d * c1_low));              // (NaN of -inf)
+        rest += x < from && x >= -3.402823466e38f ? e : 0.0f;
       });
     else
       sm_each(mine, a.run, [&](int, float x) { hits += x >= from ? 1 : 0; });

@@ -203,7 +203,7 @@ def plan_model_op(graph, op_id: int, outs, shapes: dict, dts: dict, tune: dict) 
 def _plan_q4(op, sk, tune) -> dict:
     x, q, s = sk.operands[:3]
     k, n = x.shape[-1], q.shape[0]
-    m = prod(x.shape[:-1])
+    m = max(1, prod(x.shape[:-1]))                    # (no rows: planned as one, not launched)
     _need(m <= Q4_MAX_ROWS, f"matvec_q4 takes at most {Q4_MAX_ROWS} rows of x, got {m}")
     _need(k < 2 ** 31 and n < 2 ** 31 - 512, "matvec_q4: sizes beyond 2^31")
     if len(sk.operands) == 4:

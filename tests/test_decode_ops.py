@@ -1,0 +1,336 @@
+"""The operators of a decode step without a GPU: shapes and refusals, launch
+plans over their ranges, parameter blocks, and that their kernels compile."""
+import ctypes
+import random
+
+import pytest
+
+from molten_b200 import _capi, cli, decode, graphs
+from molten_b200.build import build_cubin
+from molten_b200.codegen import CodeGenerator, compile_graph
+from molten_b200.fusion import FusionEngine
+from molten_b200.ir import DataflowGraph, ModelOpType, OpType, TensorShape as TS
+from molten_b200.lowering import LoweringError
+
+
+def config_of(g, dtype, **tune):
+    grp = FusionEngine().fuse(g)[0]
+    k = CodeGenerator(dtype=dtype, tune=tune or None).generate(g, grp)
+    assert [sk.family for sk in k.plan.kernels] == ["model"]
+    return k.plan.kernels[0].config
+
+
+def refused(g, text, dtype="bfloat16"):
+    with pytest.raises(LoweringError, match=text):
+        compile_graph(g, dtype=dtype)
+
+
+# ------------------------------------------------------------------ refusals
+def q4_graph(x, q, s, z=None, qdt="uint8", zdt="bfloat16"):
+    g = DataflowGraph("q4")
+    ids = [g.add_input("x", TS(x), dtype="bfloat16"), g.add_input("q", TS(q), dtype=qdt),
+           g.add_input("s", TS(s), dtype="bfloat16")]
+    zid = g.add_input("z", TS(z), dtype=zdt) if z else None
+    g.add_output(g.matvec_q4(*ids, zeros=zid, name="y"))
+    return g
+
+
+@pytest.mark.parametrize("x,q,s,z,text", [
+    ([1, 256], [64, 100], [64, 2], None, "nibbles"),
+    ([1, 256], [64, 128], [63, 2], None, "scales"),
+    ([1, 256], [64, 128], [64, 1], None, "scales"),            # groups of 256
+    ([1, 96], [64, 48], [64, 1], None, "scales"),              # groups of 96
+    ([1, 256], [64, 128], [64, 2], [64, 4], "zeros"),
+    ([33, 256], [64, 128], [64, 2], None, "at most 32 rows"),
+    ([3, 11, 256], [64, 128], [64, 2], None, "at most 32 rows"),
+    ([1, 256], [64, 128, 1], [64, 2], None, "needs x"),
+])
+def test_matvec_q4_refusals(x, q, s, z, text):
+    refused(q4_graph(x, q, s, z), text)
+
+
+def test_matvec_q4_refuses_types():
+    refused(q4_graph([1, 256], [64, 128], [64, 2], [64, 2], zdt="float32"), "one dtype")
+    g = DataflowGraph("q4")
+    x, q = g.add_input("x", TS([1, 256]), dtype="int32"), g.add_input("q", TS([64, 128]), dtype="uint8")
+    s = g.add_input("s", TS([64, 2]), dtype="int32")
+    g.add_output(g.matvec_q4(x, q, s))
+    refused(g, "float type")
+
+
+def rope_graph(x, tables, pos, sections=None, packed=False, style="half", x_dtype="bfloat16"):
+    g = DataflowGraph("rope")
+    xi = g.add_input("x", TS(x), dtype=x_dtype)
+    c = g.add_input("cos", TS(tables), dtype="float32")
+    s = None if packed else g.add_input("sin", TS(tables), dtype="float32")
+    p = g.add_input("positions", TS(pos), dtype="int32")
+    g.add_output(g.rope(xi, c, sin=s, style=style, positions=p, sections=sections))
+    return g
+
+
+@pytest.mark.parametrize("x,tables,pos,sections,text", [
+    ([2, 8, 4, 63], [16, 31], [1, 2, 8], None, "even head_dim"),
+    ([2, 8, 4, 64], [16, 64], [1, 2, 8], None, "rope table"),
+    ([2, 8, 4, 64], [16, 32], [2, 2, 8], None, "positions of shape"),
+    ([2, 8, 4, 64], [16, 32], [3, 2, 7], [16, 8, 8], "positions of shape"),
+    ([2, 8, 4, 64], [16, 32], [2, 8], [16, 16], "positions of shape"),
+    ([2, 8, 4, 64], [16, 32], [3, 2, 8], [16, 8, 4], "sections"),
+    ([2, 8, 4, 64], [16, 32], [5, 2, 8], [16, 4, 4, 4, 4], "sections"),
+    ([2, 8, 4, 64], [16, 32], [2, 2, 8], [36, -4], "sections"),
+    ([4, 64], [16, 32], [1, 4], None, "rank >= 3"),
+    ([2, 8, 4, 2048], [16, 1024], [1, 2, 8], None, "head_dim"),
+])
+def test_rope_positions_refusals(x, tables, pos, sections, text):
+    refused(rope_graph(x, tables, pos, sections), text)
+
+
+def test_rope_sections_need_positions_and_a_known_style():
+    g = DataflowGraph("rope")
+    x, f = g.add_input("x", TS([2, 8, 4, 64])), g.add_input("f", TS([8, 64]))
+    with pytest.raises(ValueError, match="sections need positions"):
+        g.rope(x, f, sections=[16, 16])
+    refused(rope_graph([2, 8, 4, 64], [16, 32], [1, 2, 8], style="thirds"), "style")
+
+
+def window_graph(q, k, v=None, lengths=None, dtype="bfloat16", v_dtype=None, **kw):
+    g = DataflowGraph("window")
+    ids = [g.add_input("q", TS(q), dtype=dtype), g.add_input("k", TS(k), dtype=dtype),
+           g.add_input("v", TS(v or k), dtype=v_dtype or dtype)]
+    n = g.add_input("lengths", TS(lengths), dtype="int32") if lengths else None
+    g.add_output(g.window_attention(*ids, lengths=n, **kw))
+    return g
+
+
+@pytest.mark.parametrize("q,k,v,lengths,kw,text", [
+    ([2, 1, 8, 64], [2, 10, 3, 64], None, None, {}, "8 heads over 3"),
+    ([2, 1, 8, 64], [3, 10, 4, 64], None, None, {}, "needs q"),
+    ([2, 1, 8, 64], [2, 10, 4, 32], None, None, {}, "needs q"),
+    ([2, 1, 8, 64], [2, 10, 4, 64], [2, 11, 4, 64], None, {}, "needs q"),
+    ([2, 1, 8, 60], [2, 10, 4, 60], None, None, {}, "multiple of 8"),
+    ([2, 1, 8, 136], [2, 10, 4, 136], None, None, {}, "at most 128"),
+    ([2, 1, 8, 64], [2, 0, 4, 64], None, None, {}, "at least one key"),
+    ([2, 1, 8, 64], [2, 10, 4, 64], None, [3], {}, "lengths"),
+    ([2, 1, 8, 64], [2, 10, 4, 64], None, None, {"window": 0}, "window 0"),
+    ([2, 1, 8, 64], [2, 10, 4, 64], None, None, {"sinks": -1}, "sinks"),
+    ([2, 1, 8, 64], [2, 10, 4, 64], None, None, {"scale": 0.0}, "positive"),
+    ([2, 1, 8, 64], [2, 10, 4, 64], None, None, {"scale": float("inf")}, "positive"),
+    ([2, 1, 8, 64], [2, 10, 4, 64], None, None, {"scale": float("nan")}, "positive"),
+    ([1, 40, 256, 64], [1, 40, 1, 64], None, None, {}, "at most 128"),       # heads over one key head
+])
+def test_window_attention_refusals(q, k, v, lengths, kw, text):
+    refused(window_graph(q, k, v, lengths, **kw), text)
+
+
+def test_window_attention_takes_16_bit_types_only():
+    refused(window_graph([1, 1, 2, 64], [1, 9, 2, 64], dtype="float32"), "bf16 or fp16", "float32")
+
+
+def test_sample_refusals():
+    def graph(logits, u, **params):
+        g = DataflowGraph("sample")
+        x, r = g.add_input("x", TS(logits), dtype="float32"), g.add_input("u", TS(u), dtype="float32")
+        ids = {n: g.add_input(n, TS(s), dtype="float32" if n != "top_k" else "int32")
+               for n, s in params.items()}
+        g.add_output(g.sample(x, r, **ids))
+        return g
+    refused(graph([4, 100], [3]), "u of shape", "float32")
+    refused(graph([100], []), "vocabulary", "float32")
+    refused(graph([4, 100], [4], top_p=[5]), "top_p of shape", "float32")
+    refused(graph([4, 100], [4], top_k=[4, 1]), "top_k of shape", "float32")
+    refused(graphs.sample(1, 2 ** 20), "does not fit", "float32")
+    compile_graph(graph([2, 2, 100], [2, 2], top_k=[2, 2]), dtype="float32")
+
+
+def test_model_operators_do_not_take_scalar_operands():
+    g = DataflowGraph("q4")
+    x, q = g.add_input("x", TS([1, 256])), g.add_input("q", TS([64, 128]), dtype="uint8")
+    c = g.add_constant("s", 1.0)
+    g.add_output(g.add_op(ModelOpType.MATVEC_Q4, [x, q, c]))
+    with pytest.raises(LoweringError):
+        compile_graph(g, dtype="bfloat16")
+
+
+# --------------------------------------------------------------------- plans
+def test_q4_plans_over_the_range():
+    rng = random.Random(1)
+    for _ in range(150):
+        group = rng.choice((32, 64, 128))
+        k = group * rng.randint(1, 16384 // group)
+        n, m = rng.choice((1, 15, 16, 17, rng.randint(1, 200000))), rng.randint(1, 32)
+        dt = rng.choice(("bfloat16", "float16", "float32"))
+        c = config_of(graphs.matvec_q4(m, n, k, group, dtype=dt, zeros=rng.random() < 0.5), dt)
+        groups = k // group
+        assert c["tiles"] * 16 * c["warps_n"] >= n > (c["tiles"] - 1) * 16 * c["warps_n"]
+        assert c["warps"] % c["warps_n"] == 0 and c["ksplit"] <= groups
+        assert 1 <= c["teams"] <= c["tiles"] or c["teams"] == 1
+        assert c["tiles_per_cta"] * c["teams"] >= c["tiles"]
+        assert c["chunk"] * c["ksplit"] >= groups or c["chunk"] >= 1
+        assert c["smem"] <= decode.SMEM_LIMIT and (c["smem"] + 1024) * c["min_ctas"] <= decode.SMEM_SM + 4096
+
+
+def test_q4_largest_rows_still_fit():
+    for dt in ("bfloat16", "float32"):
+        c = config_of(graphs.matvec_q4(32, 4096, 128 * 1000, 128, dtype=dt), dt)
+        assert c["chunk"] < 1000 and c["smem"] <= decode.SMEM_LIMIT
+
+
+def test_rope_plans_over_the_range():
+    rng = random.Random(2)
+    for _ in range(150):
+        dim, heads = 2 * rng.randint(1, 512), rng.randint(1, 200)
+        dt, style = rng.choice(("bfloat16", "float16", "float32")), rng.choice(("half", "interleaved"))
+        c = config_of(graphs.rope_positions(rng.randint(1, 9), rng.randint(1, 5000), heads, dim, table=100,
+                                            dtype=dt, style=style), dt)
+        assert 1 <= c["block"] <= 1024
+        assert c["block"] == c["head_lanes"] * c["tokens_per_cta"] * (
+            dim // 2 // (c["vec"] if style == "half" else c["vec"] // 2))
+
+
+def test_window_plans_over_the_range():
+    rng = random.Random(3)
+    for _ in range(200):
+        per, kv = rng.choice((1, 2, 4, 5, 8, 32)), rng.randint(1, 16)
+        new, cache = rng.choice((1, 2, 7, 33, 500, 8192)), rng.randint(1, 200000)
+        dim = 8 * rng.randint(1, 16)
+        c = config_of(graphs.window_attention(rng.randint(1, 64), new, cache, per * kv, kv, dim,
+                                              window=rng.choice((None, 1, 100, 4096)),
+                                              sinks=rng.choice((0, 1, 4, 200))), "bfloat16")
+        assert (c["kind"] == "tiles") == (new * per > decode.WINDOW_FEW_ROWS)
+        if c["kind"] == "tiles":
+            assert 0 < c["positions"] * per <= 128 and c["blocks"] * 2 * c["positions"] >= new
+            assert c["smem"] <= decode.SMEM_LIMIT
+        else:
+            assert 8 * c["nb"] >= c["rows"] and c["ranks"] in (1, 2, 4, 8)
+            assert c["smem_launch"] <= decode.SMEM_LIMIT
+            assert c["parts"] == 1 or c["ranks"] == 8
+
+
+def test_window_wider_than_the_cache_is_none():
+    for w in (4097, 10 ** 9):
+        assert config_of(graphs.window_attention(1, 1, 4096, 8, 8, 64, window=w), "bfloat16")["window"] == -1
+    assert config_of(graphs.window_attention(1, 1, 4096, 8, 8, 64, sinks=5000), "bfloat16")["sinks"] == 4096
+
+
+def test_sample_plans_over_the_range():
+    rng = random.Random(4)
+    for _ in range(200):
+        vocab, rows = int(2 ** rng.uniform(0, 18.3)), rng.randint(1, 2000)
+        dt = rng.choice(("float32", "bfloat16", "float16"))
+        c = config_of(graphs.sample(rows, vocab, dtype=dt), dt)
+        word = 1 if dt == "float32" else 2
+        assert c["block"] * c["run"] * c["ranks"] >= vocab
+        assert c["run"] % word == 0 and c["run"] // word % 2 == 1
+        assert c["block"] * c["run"] <= 65536 and c["smem"] <= decode.SMEM_LIMIT
+
+
+def test_empty_batches_have_plans():
+    for g, dt in ((graphs.matvec_q4(0, 64, 256, 64), "bfloat16"), (graphs.rope_positions(0, 4, 2, 64), "bfloat16"),
+                  (graphs.rope_positions(2, 0, 2, 64), "bfloat16"), (graphs.window_attention(0, 1, 9, 4, 2, 64), "bfloat16"),
+                  (graphs.window_attention(0, 90, 90, 4, 2, 64), "bfloat16"), (graphs.sample(0, 100), "float32")):
+        assert config_of(g, dt)["block"] > 0
+
+
+def test_sources_depend_on_types_not_sizes():
+    def source(g, dt):
+        return compile_graph(g, dtype=dt)[0].source
+    # few rows: the warps of a CTA and its ring are in the source as well
+    some = {source(graphs.window_attention(b, 1, cache, 32, 8, 128, window=w), "bfloat16")
+            for b in (1, 3, 16, 64, 200) for cache in (100, 4096, 50000) for w in (None, 100, 3000)}
+    assert len(some) <= 3
+    assert (source(graphs.window_attention(1, 500, 4096, 32, 8, 128), "bfloat16")
+            == source(graphs.window_attention(7, 64, 999, 16, 4, 72, window=None), "bfloat16"))
+    a = compile_graph(graphs.sample(256, 100003), dtype="float32")[0]
+    b = compile_graph(graphs.sample(300, 90000), dtype="float32")[0]
+    assert a.source == b.source and a.plan.key != b.plan.key
+
+
+# ----------------------------------------------------------- parameter blocks
+def test_struct_layouts():
+    assert ctypes.sizeof(_capi.Q4Args) == 88 and _capi.Q4Args.n.offset == 48
+    assert ctypes.sizeof(_capi.RopePosArgs) == 120 and _capi.RopePosArgs.heads.offset == 80
+    assert ctypes.sizeof(_capi.WindowArgs) == 168 and _capi.WindowArgs.batch.offset == 120
+    assert ctypes.sizeof(_capi.WindowTcArgs) == 512 and _capi.WindowTcArgs.batch.offset == 440
+    assert ctypes.sizeof(_capi.SampleArgs) == 96 and _capi.SampleArgs.rows.offset == 64
+
+
+def test_tensor_map_arguments_are_checked():
+    lib = _capi.load_library()
+    buf = ctypes.create_string_buffer(256)
+    at = (ctypes.addressof(buf) + 63) & ~63
+    good = dict(tmap=at, dtype=_capi.DT_BF16, base=4096, dims=(128, 8, 100, 2), strides=(256, 2048, 204800),
+                box=(64, 1, 128, 1))
+
+    def call(**kw):
+        a = dict(good, **kw)
+        return lib.molten_encode_tma_4d(
+            a["tmap"], a["dtype"], a["base"],
+            a["dims"] and bytes((ctypes.c_uint64 * 4)(*a["dims"])),
+            a["strides"] and bytes((ctypes.c_uint64 * 3)(*a["strides"])),
+            a["box"] and bytes((ctypes.c_uint32 * 4)(*a["box"])))
+    for bad in (dict(tmap=None), dict(base=None), dict(dims=None), dict(strides=None), dict(box=None),
+                dict(tmap=at + 8), dict(base=4104), dict(dtype=7), dict(dims=(128, 0, 100, 2)),
+                dict(dims=(128, 8, 2 ** 33, 2)), dict(strides=(256, 2040, 204800)),
+                dict(strides=(0, 2048, 204800)), dict(strides=(256, 2048, 2 ** 40)),
+                dict(box=(72, 1, 128, 1)), dict(box=(60, 1, 128, 1)), dict(box=(64, 1, 257, 1)),
+                dict(box=(64, 0, 128, 1))):
+        assert call(**bad) == 1, bad
+
+
+# ------------------------------------------------------- kernels, JSON, reports
+@pytest.mark.parametrize("graph,dtype", [
+    (graphs.matvec_q4(1, 512, 512, 64), "bfloat16"),
+    (graphs.matvec_q4(20, 512, 512, 32, dtype="float32", zeros=True), "float32"),
+    (graphs.rope_positions(2, 8, 4, 128, sections=[16, 24, 24]), "bfloat16"),
+    (graphs.window_attention(1, 1, 4096, 32, 8, 128), "bfloat16"),
+    (graphs.window_attention(1, 100, 4096, 32, 8, 64, dtype="float16"), "float16"),
+    (graphs.sample(2, 1000, top_k=True, top_p=0.9), "float32"),
+])
+def test_kernels_compile(graph, dtype, tmp_path):
+    k = compile_graph(graph, dtype=dtype)[0]
+    assert build_cubin(k.source, k.name, cache_dir=tmp_path).stat().st_size > 1000
+
+
+def decode_graph():
+    g = DataflowGraph("step")
+    x = g.add_input("x", TS([2, 512]), dtype="bfloat16")
+    w = g.add_input("w", TS([512]), dtype="bfloat16")
+    q = g.add_input("q", TS([1000, 256]), dtype="uint8")
+    s = g.add_input("s", TS([1000, 8]), dtype="bfloat16")
+    u = g.add_input("u", TS([2]), dtype="float32")
+    logits = g.matvec_q4(g.rms_norm(x, w, "norm"), q, s, name="logits")
+    g.add_output(g.sample(logits, u, top_k=g.add_constant("k", 40), name="token"))
+    return g
+
+
+def test_json_round_trip_and_commands(tmp_path, capsys):
+    import json
+    for g in (graphs.sample(2, 100, top_k=50, top_p=True), decode_graph(),
+              graphs.window_attention(1, 1, 64, 4, 2, 64), graphs.rope_positions(1, 4, 2, 64, sections=[8, 8, 16])):
+        data = cli.graph_to_json(g)
+        back = cli.graph_from_json(json.loads(json.dumps(data)))
+        assert cli.graph_to_json(back) == data
+        assert [o.op_type for o in back.ops.values()] == [o.op_type for o in g.ops.values()]
+    p = tmp_path / "g.json"
+    p.write_text(json.dumps(cli.graph_to_json(decode_graph())))
+    assert cli.main(["compile", str(p), "-o", str(tmp_path / "out"), "--dtype", "bfloat16"]) == 0
+    assert "kernel(s)" in capsys.readouterr().out
+    text = "".join(f.read_text() for f in (tmp_path / "out").glob("molten_fused_*.cu"))
+    assert "q4_matvec.cuh" in text and "sample.cuh" in text
+
+
+def test_a_chain_keeps_its_order_and_types():
+    ks = compile_graph(decode_graph(), dtype="bfloat16")
+    fams = [sk.family for k in ks for sk in k.plan.kernels]
+    assert fams.count("model") == 2 and fams[-1] == "model"
+    out = ks[-1].plan.kernels[-1].outputs[0]
+    assert out.dtype == "int32" and out.shape == (2,)
+
+
+def test_a_token_cannot_enter_float_arithmetic():
+    g = decode_graph()
+    tok = g._outputs[-1]
+    src = g.ops[tok].inputs[0] if g.ops[tok].op_type == OpType.OUTPUT else tok
+    g.add_output(g.add_op(OpType.EXP, [src]))
+    with pytest.raises(LoweringError):
+        for k in compile_graph(g, dtype="bfloat16"):
+            pass
