@@ -74,7 +74,7 @@ struct SampleSums { double x; float y, z; };         // sums of a thread
 
 template <typename T, int THREADS>
 struct SampleShared {
-  static constexpr int PACKED = THREADS * 20 / (int)sizeof(T);
+  static constexpr int PACKED = THREADS * 32 / (int)sizeof(T);
   SampleShare ex[2][SAMPLE_MAX_RANKS];   // exchanged values of the ranks
   SampleShare red[32];
   double table[256];               // 2^(j / 256)
@@ -821,6 +821,10 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
       k.run = max(0, min(per, (here + WORD - 1) / WORD * WORD - tid * per));
       lo = from;
     }
+  }
+  if (!packed) {                                     // the whole row, its tail included
+    many = count;
+    tail = 0.0;
   }
   const int at = sample_draw<T, THREADS>(k, per, lo, many, tail, u, top_k, top_p, min_p);
   if (at < 0) return;

@@ -407,7 +407,7 @@ def _plan_window_tiles(c: dict, o: dict) -> dict:
 
 
 def _sample_fixed(dtype, threads) -> int:
-    packed = threads * 20 // DTYPE_SIZE[dtype]        # tokens: value and 16-bit index
+    packed = threads * 32 // DTYPE_SIZE[dtype]        # tokens: value and 16-bit index
     return SAMPLE_FIXED + packed * (DTYPE_SIZE[dtype] + 2)
 
 

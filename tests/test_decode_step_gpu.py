@@ -322,6 +322,17 @@ def test_sample_extreme_temperatures(rt, dtype, top_p, top_k):
     check_sample(tokens[-2:], x[-2:], u[-2:], temperature=torch.tensor([1e30, 1e300], dtype=torch.float64), **given)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,vocab,top_p", [(64, 131072, 0.93), (64, 131072, 0.999), (40, 20011, 0.99)])
+def test_sample_many_kept_tokens(rt, dtype, rows, vocab, top_p):
+    """Flat rows, of which the filters keep more or fewer tokens than fit the
+    packed list."""
+    x, u = sample_inputs(rows, vocab, dtype, seed=rows)
+    t = torch.linspace(0.5, 3.0, rows, device=DEV)
+    tokens = compiled(rt, graphs.sample(rows, vocab, dtype=dtype, top_p=top_p), dtype)(x, u, t)
+    check_sample(tokens, x, u, temperature=t, top_p=torch.full((rows,), top_p))
+
+
 # ---------------------------------------------------- tensors that coincide
 def test_the_same_tensor_twice(rt):
     x, q, s, _ = q4_inputs(2, 100, 256, 64, "bfloat16", False)
