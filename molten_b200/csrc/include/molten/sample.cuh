@@ -29,9 +29,10 @@
 // each with all.  Rows whose kept tokens do not fit the packed list go the same
 // way with the whole row in its place.
 //
-// Measured: 1 x 32768 fp32 with top_k and top_p 23.5 us; 64 x 131072 bf16 with
-// top_p and min_p, 16000 tokens kept, 137 us; 256 x 100003 fp32, some rows with
-// each filter, 158 us; the same unfiltered 103 us (0.99 TB/s).
+// Measured: 1 x 32768 fp32 with top_k and top_p 23.6 us; 64 x 131072 bf16 with
+// top_p and min_p, 16000 tokens kept, 109 us (137 with the tokens that are surely
+// kept left in the border's search); 256 x 100003 fp32, some rows with each
+// filter, 159 us; the same unfiltered 103 us (0.99 TB/s).
 //
 // Only the tail that top_p surely drops, of which it needs nothing but the
 // total, has fp32 terms (summed by a thread, then in fp64).  Each is off by up to
@@ -270,6 +271,7 @@ struct Sampler {
   int run, ranks, rank, tid;
   float m, cut;                    // largest logit; below this one weights are 0
   double c;                        // weights: 2^((x - m) c / 256)
+  float sure;                      // top_p keeps all above this one (no top_k)
 
   // 2^(t / 256), -256000 <= t <= 0
   __device__ __forceinline__ double power(double t) const {
@@ -470,9 +472,10 @@ struct Sampler {
   // The border among the tokens of [lo, hi], `count` of them or fewer.
   // by_weight = false: the token of rank `goal`, from 1, from the largest down.
   // by_weight = true: the first token at which the running weight reaches
-  // `goal`.  Returns its value; *ties: how many tokens of that value are kept.
-  __device__ __noinline__ float border(bool by_weight, float lo, float hi, int count, double goal, double* ties) {
-    double n = 0.0;                                  // count or weight above hi
+  // `goal`; n: count or weight above hi.  Returns its value; *ties: how many tokens
+  // of that value are kept.
+  __device__ __noinline__ float border(bool by_weight, float lo, float hi, int count, double goal, double n,
+                                       double* ties) {
 #pragma unroll 1
     for (int step = 0; step < 64 && lo < hi; ++step) {
       const Bins bins(lo, hi);
@@ -531,25 +534,27 @@ __device__ __noinline__ int sample_draw(Sampler<T, THREADS>& k, int per, float l
   float tau = -INFINITY;
   double ties = 0.0;
   if (top_k > 0) {
-    tau = k.border(false, lo, k.m, count, (double)top_k, &ties);
+    tau = k.border(false, lo, k.m, count, (double)top_k, 0.0, &ties);
     count = top_k;
     tail = 0.0;
   }
   if (top_p < 1.0f) {
-    double w = 0.0;
+    double w = 0.0, high = 0.0;                      // weight; of the tokens above `sure`
     float lowest = INFINITY;
     sm_each<2>(mine, run, [&](int, float x) {
       const double v = k.weight(x);
       w += x > tau ? v : 0.0;
+      high += x > k.sure ? v : 0.0;
       lowest = fminf(lowest, x > tau ? x : INFINITY);
     });
-    const SampleShare got = sm_combine<THREADS>(sh, ranks, rank, {-lowest, 0.0f, w, 0.0});
+    const SampleShare got = sm_combine<THREADS>(sh, ranks, rank, {-lowest, 0.0f, w, high});
     const double wt = tau == -INFINITY ? 0.0 : k.weight(tau);
     const double goal = fmax((double)top_p, 0.0) * (got.z + tail + ties * wt);
     if (tau > -INFINITY && goal > got.z) {           // inside the ties of top_k's border
       ties = fmin(ties, fmax(1.0, ceil((goal - got.z) / wt)));
     } else if (goal > 0.0) {
-      tau = k.border(true, -got.x, k.m, count, goal, &ties);
+      const bool narrow = -got.x < k.sure && k.sure < k.m;
+      tau = k.border(true, -got.x, narrow ? k.sure : k.m, count, goal, narrow ? got.w : 0.0, &ties);
       ties = fmax(ties, 1.0);
     } else {
       tau = k.m;                                     // the largest token at least
@@ -713,7 +718,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
   if (tid < 256) sh.table[tid] = exp2((double)tid * (1.0 / 256.0));
   __syncthreads();
 
-  Sampler<T, THREADS> k{sh, xs + tid * a.run, a.run, a.ranks, rank, tid, 0.0f, 0.0f, 0.0};
+  Sampler<T, THREADS> k{sh, xs + tid * a.run, a.run, a.ranks, rank, tid, 0.0f, 0.0f, 0.0, INFINITY};
   const T* mine = k.mine;
   const SampleShare range = sm_combine<THREADS>(sh, a.ranks, rank, {top, -bottom, (double)finite, 0.0});
   k.m = range.x;
@@ -756,6 +761,10 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
       k.select_bins(by_weight, bins, lo, 0.0, by_weight ? -1.0 : (double)top_k, (double)top_p, &b0, &b1);
       // a little below the last bin's lower edge: its tokens are among the packed
       const float depth = ((float)b1 + 0.6f) * 2.0f / bins.inv;
+      if (by_weight && b0 > 0) {
+        const float height = ((float)b0 - 0.6f) * 2.0f / bins.inv;
+        k.sure = (k.m - height) + 4e-7f * (fabsf(k.m) + height);
+      }
       if (b1 < SAMPLE_BINS - 1) from = fmaxf(lo, (k.m - depth) - 4e-7f * (fabsf(k.m) + depth));
     }
   }
