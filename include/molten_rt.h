@@ -174,7 +174,7 @@ typedef struct molten_window_tc_args {
  * molten/sample.cuh).  A parameter's vector may be null: its scalar is used
  * then (temperature 1, top_k 0, top_p 1 and min_p 0 leave every token).
  * Grid rows * ranks in clusters of `ranks`; run: tokens per thread, an odd
- * number of 32-bit words with 256 * ranks * run >= vocab. */
+ * number of 32-bit words with block * ranks * run >= vocab. */
 typedef struct molten_sample_args {
   const void* logits;            /* [rows, vocab], rows row_stride elements apart */
   const float* u;                /* [rows] in [0, 1) */

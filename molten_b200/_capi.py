@@ -44,6 +44,7 @@ SIGNATURES = {
 
 
 LAUNCH_PDL = 1          # MOLTEN_LAUNCH_PDL
+STATUS_POSITION = 4096  # molten::kRopePositionRange: not a wait, a position past its table
 
 
 class LaunchCfg(ctypes.Structure):

@@ -166,6 +166,8 @@ def cmd_info() -> int:
     print("                 TMA-staged ring, persistent stream form)")
     print("  Elementwise:   N-op chains with per-column / per-row broadcasting")
     print("  MatMul:        tcgen05/TMEM GEMM with a fused elementwise epilogue")
+    print("  Decode step:   4-bit matrix-vector products, RoPE at given positions,")
+    print("                 attention over a window and the first keys, sampling")
     print("  Output:        .cu + nvcc-built sm_100a cubins, loaded through the")
     print("                 libmolten_rt.so C ABI (include/molten_rt.h)")
     print("  Precision:     fp32 compute; fp32, bf16 or fp16 I/O")

@@ -33,7 +33,7 @@ struct RopePosArgs {
   int tokens_per_cta, reserved;
 };
 
-enum RopePosStatus { kRopePositionRange = 1024 };
+enum RopePosStatus { kRopePositionRange = 4096 };
 
 template <typename TT, int NP, bool PACKED, bool TVEC>
 __device__ __forceinline__ void rope_table(const RopePosArgs& a, long long token, int p0,

@@ -291,7 +291,9 @@ class _Spec:
             torch.cuda.synchronize(di)
             bits = _capi.read_status(di, True)
             if bits:
-                raise _capi.MoltenError(f"{self.gk.name}: a bounded wait ran out on device {di} "
+                what = ("a position lies past its table" if bits == _capi.STATUS_POSITION
+                        else "a bounded wait ran out")
+                raise _capi.MoltenError(f"{self.gk.name}: {what} on device {di} "
                                         f"(status word {bits:#x})")
         return outs
 

@@ -259,7 +259,7 @@ def test_rope_position_past_the_table_is_reported(rt):
     pos = torch.tensor([[0, 5, 4]], dtype=torch.int32, device=DEV)
     out = compiled(rt, graphs.rope_positions(1, 3, 2, 8, 5, dtype="float32"), "float32")(x, cos, sin, pos)
     assert torch.equal(out[:, 1], x[:, 1])
-    assert MoltenRuntime.read_status(0) == 1024 and MoltenRuntime.read_status(0) == 0
+    assert MoltenRuntime.read_status(0) == 4096 and MoltenRuntime.read_status(0) == 0
 
 
 # --------------------------------------------------------- window attention
