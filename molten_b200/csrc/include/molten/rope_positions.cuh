@@ -14,6 +14,10 @@
 // their loads issued first: the table costs one read per HPT heads instead of
 // one per head (it is fp32 and as wide as x, so it would triple the L1
 // traffic).
+//
+// Measured, bf16 with fp32 tables: 4 x 4096 tokens of 32 heads of 128, one axis
+// 45.7 us (5.9 TB/s), three axes at random positions 50.4 (each section's table
+// rows come from L2); 48 tokens of 40 heads 2.1 us.
 #pragma once
 
 #include "molten/common.cuh"
