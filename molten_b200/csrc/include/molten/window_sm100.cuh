@@ -31,13 +31,15 @@
 // for the maximum first.  The weights stay below 2^8 and O and the sum share the
 // factor, so nothing is lost.
 //
-// Measured: 8192 tokens, 32 heads over 8, head dim 128, window 2048: 271 us (889
+// Measured: 8192 tokens, 32 heads over 8, head dim 128, window 2048: 256 us (941
 // TFLOP/s of visible pairs); 4 x 500 tokens over up to 2900, head dim 64, window
-// 1000: 28 us.  With a whole row of S in registers (spills) the first took 489,
+// 1000: 27.3 us.  With a whole row of S in registers (spills) the first took 489,
 // with its maximum first 314.  S by halves, so that it can be computed ahead:
-// 285 (N = 64 takes the tensor core as long as N = 128); an issuing warp for
-// each Q tile: 325; 4 of 32 exponentials on the FMA pipe: 274; two softmax
-// threads a row (16 warps of 96 registers, spills): 387.
+// 270 (N = 64 takes the tensor core as long as N = 128); an issuing warp for
+// each Q tile: 310; 4 of 32 exponentials on the FMA pipe: 274 where none was 271;
+// two softmax threads a row (16 warps of 96 registers, spills): 387; the next
+// half's S loaded ahead: 267.  The waits for S and P poll (all asleep: 270; all
+// polling without a pause: 293), the others, of warps with time, sleep.
 //
 // P = 0 times an infinity or NaN is NaN, so V rows that no query of the item
 // sees (behind the length, before the window) are zeroed in shared memory
@@ -300,6 +302,16 @@ __device__ __noinline__ void window_tc_add_dirty(const WindowTcArgs& args, int i
   }
 }
 
+// sum + 0 x, for two 16-bit numbers: 0, or NaN from the first infinity or NaN on.
+template <typename T>
+__device__ __forceinline__ uint32_t window_tc_zeros(uint32_t x, uint32_t sum) {
+  if constexpr (std::is_same<T, f16>::value)
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(sum) : "r"(x), "r"(0u), "r"(sum));
+  else
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(sum) : "r"(x), "r"(0u), "r"(sum));
+  return sum;
+}
+
 template <class L, typename T, typename OT>
 __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const WindowTcArgs& args) {
   constexpr bool F16IN = std::is_same<T, f16>::value;
@@ -370,7 +382,7 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
     {
       const bool leader = window_tc_elect();
       auto wait_all = [&](uint32_t b, uint32_t parity) {
-        ok = __all_sync(0xffffffffu, attn_wait(b, parity & 1u));
+        ok = __all_sync(0xffffffffu, mbar_wait(b, parity & 1u));
         if (!ok && lane == 0) window_tc_fail(s, args);
         return ok;
       };
@@ -494,20 +506,31 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
           const bool all = key <= pa && (args.window < 0 || key > pb - args.window || key < args.sinks);
           if (any && all) continue;
           uint8_t* row = s.ring + (e % S) * L::STAGE_BYTES + r * 128;
-#pragma unroll 4
-          for (int q = 0; q < L::DCH * 8; ++q) {     // 16-byte chunks, the lanes' on different banks
-            uint4* at = reinterpret_cast<uint4*>(row + (q >> 3) * L::CHUNK + (((q + lane) & 7) << 4));
-            if (!any) { *at = make_uint4(0u, 0u, 0u, 0u); continue; }
-            uint4 x = *at;
+          // 16-byte chunks, the lanes' on different banks.  0 x sums up to NaN in a
+          // row with an infinity or NaN (rare: those are looked through again)
+          auto chunk = [&](int q) {
+            return reinterpret_cast<uint4*>(row + (q >> 3) * L::CHUNK + (((q + lane) & 7) << 4));
+          };
+          uint32_t sum = 0u;
+#pragma unroll 8
+          for (int q = 0; q < L::DCH * 8; ++q) {
+            if (!any) { *chunk(q) = make_uint4(0u, 0u, 0u, 0u); continue; }
+            const uint4 x = *chunk(q);
+            sum = window_tc_zeros<T>(x.x, window_tc_zeros<T>(x.y, window_tc_zeros<T>(x.z, window_tc_zeros<T>(x.w, sum))));
+          }
+          if ((sum & 0x7FFF7FFFu) == 0u) continue;
+          found = true;
+#pragma unroll 1
+          for (int q = 0; q < L::DCH * 8; ++q) {
+            uint4 x = *chunk(q);
             uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
-            bool bad = false;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               constexpr uint32_t EXP = F16IN ? 0x7C00u : 0x7F80u;
-              if ((xs[i] & EXP) == EXP) { xs[i] &= 0xFFFF0000u; bad = true; }
-              if ((xs[i] >> 16 & EXP) == EXP) { xs[i] &= 0x0000FFFFu; bad = true; }
+              if ((xs[i] & EXP) == EXP) xs[i] &= 0xFFFF0000u;
+              if ((xs[i] >> 16 & EXP) == EXP) xs[i] &= 0x0000FFFFu;
             }
-            if (bad) { *at = x; found = true; }
+            *chunk(q) = x;
           }
         }
         if (found) s.dirty[seq & 7u] = (int)seq + 1;
@@ -542,7 +565,12 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
         for (int u = 0; u < w.tiles; ++u) {
           const int j = w.tile(u);
           if (!w.need(t, j)) continue;
-          const bool got = attn_wait(bar.s_full(t), sn & 1u);
+          const bool whole = w.whole(args, t, j);
+          // columns behind c0 (or before cs) and up to c1 are seen
+          const int c1 = p - j * 128 + 1;
+          const int c0 = args.window < 0 ? 0 : p - args.window - j * 128 + 1;
+          const int cs = args.sinks - j * 128;
+          const bool got = mbar_wait(bar.s_full(t), sn & 1u);
           if (!__all_sync(0xffffffffu, got && !*s.abort_flag)) {
             if (lane == 0) window_tc_fail(s, args);
             ok = false;
@@ -553,11 +581,6 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
           // 64 columns of S at a time, each read once: half a row leaves registers
           // for the rest (a whole one spilled, at twice the time), and its P V
           // runs under the other half's exponentials
-          const bool whole = w.whole(args, t, j);
-          // columns behind c0 (or before cs) and up to c1 are seen
-          const int c1 = p - j * 128 + 1;
-          const int c0 = args.window < 0 ? 0 : p - args.window - j * 128 + 1;
-          const int cs = args.sinks - j * 128;
 #pragma unroll 1
           for (int half = 0; half < 2; ++half) {
             float x[64];
