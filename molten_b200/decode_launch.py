@@ -313,6 +313,21 @@ def launch_model_op(spec, i: int, env: dict, device: int, stream: int) -> None:
     b.run(b.conform(ins), env[b.sk.outputs[0].op_id], stream)
 
 
+def refuse_overlap(sk, tensors, out) -> None:
+    """An output may not lie in memory that other blocks of the same kernel
+    still read.  (RoPE turns pairs where they are: its x may be its output.)"""
+    start, end = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    for n, t in enumerate(tensors):
+        if t.numel() == 0 or not out.numel():
+            continue
+        span = 1 + sum((d - 1) * s for d, s in zip(t.shape, t.stride()))
+        if t.data_ptr() < end and start < t.data_ptr() + span * t.element_size():
+            if (sk.config["op"] == ModelOpType.ROTATE_POSITIONS and n == 0 and t.data_ptr() == start
+                    and t.is_contiguous() and t.dtype == out.dtype):
+                continue
+            raise RuntimeError(f"{sk.config['op'].name}: the output overlaps an input")
+
+
 class ModelCall:
     """The short way into a plan that is one model operator: ``call(tensors)``
     with contiguous, 16-byte aligned tensors on the current device, on its

@@ -264,8 +264,8 @@ class DataflowGraph:
         w is 1).  Equal logits count by index, the lowest first.  The token is
         the first, by index, at which the running weight of the kept tokens
         exceeds u times their sum.  ``temperature`` below 1e-30 takes the
-        largest logit.  NaN logits and -inf are never drawn; a row of nothing
-        else gives -1.  Weights and sums have 64 bits, but for the weight that
+        largest logit.  NaN logits and -inf are never drawn (a row of nothing
+        else gives -1); +inf counts as the largest finite number of its type.  Weights and sums have 64 bits, but for the weight that
         ``top_p`` surely drops, whose total has 32-bit terms."""
         params = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
         given = [k for k, v in params.items() if v is not None]

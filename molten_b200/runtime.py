@@ -34,7 +34,7 @@ from typing import Optional
 from . import _capi
 from .build import build_cubin, default_cache_dir
 from .codegen import CodeGenerator, GeneratedKernel, KernelConfig, kernel_entry
-from .decode_launch import STRIDED, ModelCall, launch_model_op
+from .decode_launch import STRIDED, ModelCall, launch_model_op, refuse_overlap
 from .lowering import DTYPE_SIZE, LoweringError, canon_tensor_dtype
 
 _TORCH_DTYPES = None
@@ -494,6 +494,8 @@ class CompiledKernel:
         if out is not None:
             outs = list(out) if isinstance(out, (list, tuple)) else [out]
             self._check_outs(spec, outs, dev)
+            if spec.single:
+                refuse_overlap(spec.plan.kernels[0], prepared, outs[0])
         else:
             outs = None
         res = spec.run(prepared, outs, stream, row_offset)
@@ -540,13 +542,13 @@ class CompiledKernel:
     @staticmethod
     def _conform(spec: _Spec, tensors):
         plan = spec.plan
-        gemm_b, strided = set(), None
+        gemm_b, strided, whole = set(), set(), set()
         for sk in plan.kernels:
             # what a model operator alone reads may stay strided
             takes = {o.op_id for o in sk.operands
                      if sk.family == "model" and o.index in STRIDED[sk.config["op"]]}
-            leaves = {o.op_id for o in sk.operands} - takes
-            strided = (takes if strided is None else strided | takes) - leaves
+            strided |= takes
+            whole |= {o.op_id for o in sk.operands} - takes
             if sk.family == "gemm" and not sk.config.get("split3"):
                 # (an fp32 B is read whole by its split kernel: contiguous)
                 gemm_b.add(sk.operands[sk.b_operand].op_id)
@@ -555,7 +557,7 @@ class CompiledKernel:
             if op_id in gemm_b and t.dim() == 2 and t.stride(1) == 1 \
                     and (t.stride(0) * t.element_size()) % 16 == 0:
                 out.append(t)              # a column slice of B is fine for TMA
-            elif op_id in strided:
+            elif op_id in strided - whole:
                 out.append(t)
             else:
                 out.append(t.contiguous())

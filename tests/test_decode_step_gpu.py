@@ -295,6 +295,84 @@ def test_misaligned_and_strided_inputs(rt, call):
     assert torch.equal(ck(*ins), want)
 
 
+@pytest.mark.parametrize("first", ["exp", "product"])
+def test_an_input_of_two_kernels_may_be_strided(rt, first):
+    """Only the product takes rows with gaps; the other kernel of the graph
+    needs x without them, whichever comes first."""
+    g = DataflowGraph("both")
+    x = g.add_input("x", TS([3, 256]), dtype="bfloat16")
+    q = g.add_input("q", TS([64, 128]), dtype="uint8")
+    s = g.add_input("s", TS([64, 4]), dtype="bfloat16")
+    ops = {"exp": lambda: g.exp(x, "e"), "product": lambda: g.matvec_q4(x, q, s, name="y")}
+    made = {name: ops[name]() for name in (("exp", "product") if first == "exp" else ("product", "exp"))}
+    g.add_output(made["exp"])
+    g.add_output(made["product"])
+    xs, qs, ss, _ = q4_inputs(3, 64, 256, 64, "bfloat16", False)
+    wide = torch.zeros(3, 512, dtype=torch.bfloat16, device=DEV)
+    wide[:, :256] = xs
+    e, y = Step.chain((g, [rt.compile(k) for k in compile_graph(g, dtype="bfloat16")]), wide[:, :256], qs, ss)
+    check_q4(y, xs, qs, ss, None, "bfloat16")
+    ref = torch.exp(xs.double())
+    assert bool(((e.double() - ref).abs() <= (half_step("bfloat16") + 2.0 ** -20) * ref).all())
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_the_default_stream_by_number(rt, call):
+    ck, ins = call(rt, 0)
+    want = ck(*ins).clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ck(*ins, stream=torch.cuda.default_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_wrong_types_and_devices_are_refused(rt):
+    ck, (q, k, v, n) = tiles_call(rt)
+    with pytest.raises((RuntimeError, ValueError)):
+        ck(q, k, v, n.long())
+    with pytest.raises((RuntimeError, ValueError)):
+        ck(q, k, v.float(), n)
+    with pytest.raises(RuntimeError):
+        ck(q, k, v, n.cpu())
+    ck, (x, u, t, top_k) = sample_call(rt)
+    with pytest.raises((RuntimeError, ValueError)):
+        ck(x, u.double(), t, top_k)
+    with pytest.raises((RuntimeError, ValueError)):
+        ck(x, u[:-1], t, top_k)
+
+
+def test_outputs_do_not_overlap_inputs(rt):
+    x, q, s, _ = q4_inputs(2, 256, 256, 64, "bfloat16", False)
+    ck = compiled(rt, graphs.matvec_q4(2, 256, 256, 64), "bfloat16")
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ck(x, q, s, out=x)
+    ck, (qq, k, v, n) = tiles_call(rt)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ck(qq, k, v, n, out=qq)
+    buf = torch.zeros(2 * qq.numel() - 8, dtype=qq.dtype, device=DEV)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ck(buf[:qq.numel()].view(qq.shape), k, v, n, out=buf[-qq.numel():].view(qq.shape))
+    # RoPE in place
+    ck, ins = rope_call(rt)
+    want = ck(*ins).clone()
+    assert ck(*ins, out=ins[0]).data_ptr() == ins[0].data_ptr() and torch.equal(ins[0], want)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        wide = torch.zeros(want.numel() + 8, dtype=want.dtype, device=DEV)
+        ck(wide[:-8].view(want.shape), *ins[1:], out=wide[8:].view(want.shape))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_an_infinity_in_x_stays_in_its_row(rt, dtype):
+    x, q, s, z = q4_inputs(4, 80, 512, 64, dtype, True)
+    x[1, 100], x[2, 7] = torch.inf, torch.nan
+    y = compiled(rt, graphs.matvec_q4(4, 80, 512, 64, zeros=True, dtype=dtype), dtype)(x, q, s, z)
+    keep = torch.tensor([0, 3], device=DEV)
+    check_q4(y[keep], x[keep], q, s, z, dtype)
+    assert not torch.isfinite(y[1:3]).any()
+
+
 def test_shapes_in_turn(rt):
     ck = compiled(rt, graphs.sample(4, 1000), "float32")
     cases = [(sample_inputs(r, v, "float32", r), torch.full((r,), 1.3, device=DEV))
