@@ -44,6 +44,11 @@ def _merged(t, keep: int):
     return t.contiguous().view((lead,) + tail)
 
 
+def _copied(t):
+    """t in memory of its own, contiguous and aligned."""
+    return t.clone() if t.is_contiguous() else t.contiguous()
+
+
 def _aligned(t, nbytes: int, strides) -> bool:
     return t.data_ptr() % nbytes == 0 and all(s * t.element_size() % nbytes == 0 for s in strides)
 
@@ -112,9 +117,8 @@ class _Q4(_Bound):
 
     def conform(self, ins):
         x = _merged(ins[0], 1)
-        if not _aligned(x, 16, x.stride()[:-1]) and x.shape[0] > 1:
-            x = x.contiguous()
-        self.need_aligned(0, x, 16)
+        if not _aligned(x, 16, x.stride()[:-1] if x.shape[0] > 1 else ()):
+            x = _copied(x)
         self.need_aligned(1, ins[1], 16)
         for j in range(2, len(ins)):
             self.need_aligned(j, ins[j], ins[j].element_size())
@@ -152,8 +156,7 @@ class _Rope(_Bound):
         if c["xvec"]:
             slot = min(16, c["vec"] * x.element_size())
             if not _aligned(x, slot, x.stride()[:-1]):
-                x = x.contiguous()
-            self.need_aligned(0, x, slot)
+                x = _copied(x)
         if c["tvec"]:
             for j in range(1, len(ins) - 1):
                 self.need_aligned(j, ins[j], c["table_slot"])
@@ -207,7 +210,8 @@ class _Window(_Bound):
             if ((t.stride(3) != 1 and t.shape[3] > 1) or not _aligned(t, 16, t.stride()[:3])
                     or (self.c["kind"] == "tiles"
                         and any(n > 1 and x == 0 for n, x in zip(t.shape, t.stride())))):
-                t = t.contiguous()
+                # (a cache that is only misplaced is not copied at every call)
+                t = _copied(t) if j == 0 else t.contiguous()
             self.need_aligned(j, t, 16)
             out[j] = t
         return out

@@ -5,7 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from molten_b200 import graphs
+from molten_b200 import _capi, graphs
 from molten_b200.codegen import compile_graph
 from molten_b200.ir import DataflowGraph, OpType, TensorShape as TS
 from molten_b200.runtime import MoltenRuntime
@@ -341,6 +341,27 @@ def test_wrong_types_and_devices_are_refused(rt):
         ck(x, u.double(), t, top_k)
     with pytest.raises((RuntimeError, ValueError)):
         ck(x, u[:-1], t, top_k)
+
+
+@pytest.mark.parametrize("call,which", [(q4_call, [0]), (rope_call, [0]), (few_call, [0, 3]), (tiles_call, [0, 3]),
+                                        (sample_call, [0, 1, 2, 3])])
+def test_misplaced_inputs(rt, call, which):
+    ck, ins = call(rt, 0)
+    want = ck(*ins).clone()
+    for j in which:
+        buf = torch.empty(ins[j].numel() + 1, dtype=ins[j].dtype, device=DEV)
+        moved = buf[1:].view(ins[j].shape)
+        moved.copy_(ins[j])
+        assert torch.equal(ck(*ins[:j], moved, *ins[j + 1:]), want), j
+
+
+def test_misplaced_caches_are_refused(rt):
+    for call in (few_call, tiles_call):
+        ck, (q, k, v, n) = call(rt, 0)
+        moved = torch.empty(k.numel() + 1, dtype=k.dtype, device=DEV)[1:].view(k.shape)
+        for ins in ((q, moved, v, n), (q, k, moved, n)):
+            with pytest.raises(_capi.MoltenError, match="aligned"):
+                ck(*ins)
 
 
 def test_outputs_do_not_overlap_inputs(rt):
