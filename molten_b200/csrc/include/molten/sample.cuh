@@ -29,10 +29,11 @@
 // each with all.  Rows whose kept tokens do not fit the packed list go the same
 // way with the whole row in its place.
 //
-// Measured: 1 x 32768 fp32 with top_k and top_p 23.6 us; 64 x 131072 bf16 with
-// top_p and min_p, 16000 tokens kept, 109 us (137 with the tokens that are surely
-// kept left in the border's search); 256 x 100003 fp32, some rows with each
-// filter, 159 us; the same unfiltered 103 us (0.99 TB/s).
+// Measured: 1 x 32768 fp32 with top_k and top_p 23.3 us; 64 x 131072 bf16 with
+// top_p and min_p, 16000 tokens kept, 100 us (132 with the tokens that are surely
+// kept left in the border's search, 109 with their weights behind a branch); 256 x
+// 100003 fp32, some rows with each filter, 158 us; the same unfiltered 103 us
+// (0.99 TB/s).
 //
 // Only the tail that top_p surely drops, of which it needs nothing but the
 // total, has fp32 terms (summed by a thread, then in fp64).  Each is off by up to
@@ -424,13 +425,14 @@ struct Sampler {
     // `group` lanes to a token, each with some of those it is compared with; the
     // ranks share the tokens (and meet in an exchange, behind which the lists
     // may be filled anew)
-    int group = 32;
-    while (group > 1 && have * group > ranks * THREADS) group /= 2;
+    int lanes = 5;
+    while (lanes > 0 && have << lanes > ranks * THREADS) --lanes;
+    const int group = 1 << lanes;
     float best = -INFINITY;
     double above = 0.0;
 #pragma unroll 1
-    for (int i0 = 0; i0 < have; i0 += ranks * THREADS / group) {
-      const int i = i0 + (rank * THREADS + tid) / group;
+    for (int i0 = 0; i0 < have; i0 += (ranks * THREADS) >> lanes) {
+      const int i = i0 + ((rank * THREADS + tid) >> lanes);
       const float x = i < have ? s.all[i] : -INFINITY;
       unsigned long long gt = 0ull, eq = 0ull;
 #pragma unroll 4
@@ -490,20 +492,20 @@ struct Sampler {
       const bool listed = left <= SAMPLE_LIST;
       double above = 0.0;
       float top = -INFINITY, low = INFINITY;
-#pragma unroll 1
-      for (int i = 0; i < run; ++i) {
-        const float x = to_f32(mine[i]);
-        if (!(x >= lo && x <= hi)) continue;
-        const int b = bins.of(x);
-        if (b < b0) above += by_weight ? weight(x) : 1.0;
-        if (b < b0 || b > b1) continue;
+      // (weights without a branch: those of several tokens overlap)
+      sm_each<4>(mine, run, [&](int, float x) {
+        const bool in = x >= lo && x <= hi;
+        const int b = in ? bins.of(x) : BINS;
+        const double v = by_weight ? weight(x) : 1.0;
+        above += b < b0 ? v : 0.0;
+        if (b < b0 || b > b1 || !in) return;
         top = fmaxf(top, x);
         low = fminf(low, x);
         if (listed) {
           const int at = atomicAdd(&s.list_n, 1);
           if (at < SAMPLE_LIST) s.list[at] = x;
         }
-      }
+      });
       const SampleShare got = sm_combine<THREADS>(s, ranks, rank, {top, -low, above, 0.0});
       n += got.z;
       hi = got.x;
@@ -541,7 +543,7 @@ __device__ __noinline__ int sample_draw(Sampler<T, THREADS>& k, int per, float l
   if (top_p < 1.0f) {
     double w = 0.0, high = 0.0;                      // weight; of the tokens above `sure`
     float lowest = INFINITY;
-    sm_each<2>(mine, run, [&](int, float x) {
+    sm_each<4>(mine, run, [&](int, float x) {
       const double v = k.weight(x);
       w += x > tau ? v : 0.0;
       high += x > k.sure ? v : 0.0;
