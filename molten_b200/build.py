@@ -1,4 +1,5 @@
-"""nvcc driver: builds libmolten_rt.so and the generated kernels' cubins.
+"""nvcc driver: builds libmolten_rt.so and the generated kernels' cubins (and, with
+the host compiler, the short host path of model operators).
 
 Every device build targets sm_100a only:
 ``nvcc -gencode arch=compute_100a,code=sm_100a -lineinfo -O3``.
@@ -113,5 +114,41 @@ def build_runtime(verbose: bool = False, force: bool = False) -> Path:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise BuildError(f"building libmolten_rt.so failed:\n{res.stderr[-4000:]}")
+    os.replace(tmp, out)
+    return out
+
+
+def call_library() -> Path:
+    """Where the short host path is built, for this torch and Python."""
+    import sys
+    import torch
+    tag = "".join(c if c.isalnum() else "_" for c in torch.__version__)
+    return LIB_DIR / f"molten_call.py{sys.version_info[0]}{sys.version_info[1]}.torch{tag}.so"
+
+
+def build_call(verbose: bool = False, force: bool = False) -> Path:
+    """Build the short host path of model operators (``csrc/call.cpp``) against the
+    installed torch."""
+    import sysconfig
+    import torch
+    LIB_DIR.mkdir(exist_ok=True)
+    out = call_library()
+    src = CSRC_DIR / "call.cpp"
+    deps = [src, ABI_INCLUDE / "molten_rt.h"]
+    if out.exists() and not force and all(out.stat().st_mtime >= d.stat().st_mtime for d in deps):
+        return out
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    tmp = LIB_DIR / f".molten_call.{os.getpid()}.so"
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{ABI_INCLUDE}", f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}",
+           f"-I{cuda / 'include'}", f"-I{sysconfig.get_paths()['include']}", "-o", str(tmp), str(src),
+           f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd))
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise BuildError(f"building {out.name} failed:\n{res.stderr[-4000:]}")
     os.replace(tmp, out)
     return out

@@ -34,7 +34,7 @@ from typing import Optional
 from . import _capi
 from .build import build_cubin, default_cache_dir
 from .codegen import CodeGenerator, GeneratedKernel, KernelConfig, kernel_entry
-from .decode_launch import STRIDED, ModelCall, launch_model_op, refuse_overlap
+from .decode_launch import STRIDED, ModelCall, launch_model_op, refuse_overlap, short_call
 from .lowering import DTYPE_SIZE, LoweringError, canon_tensor_dtype
 
 _TORCH_DTYPES = None
@@ -463,7 +463,7 @@ class CompiledKernel:
     runtime: Optional["MoltenRuntime"] = None
     _specs: dict = field(default_factory=dict)
     _hosts: dict = field(default_factory=dict)
-    _last: Optional[ModelCall] = None     # the last call's specialisation, where it is one model operator
+    _last: object = None     # the short way into the last call's plan, where that is one model operator
 
     def __call__(self, *tensors, out=None, stream=None, row_offset: int = 0):
         if self._last is not None and out is None and stream is None:
@@ -500,7 +500,7 @@ class CompiledKernel:
             outs = None
         res = spec.run(prepared, outs, stream, row_offset)
         if not DEBUG and spec.single:
-            self._last = ModelCall(spec, tensors)
+            self._last = short_call(spec, tensors)
         return res[0] if len(res) == 1 else tuple(res)
 
     # -- specialisation -------------------------------------------------

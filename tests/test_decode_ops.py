@@ -334,3 +334,30 @@ def test_a_token_cannot_enter_float_arithmetic():
     with pytest.raises(LoweringError):
         for k in compile_graph(g, dtype="bfloat16"):
             pass
+
+
+# ------------------------------------------------------- the short host path
+def test_short_call_checks_its_plan_and_its_tensors():
+    torch = pytest.importorskip("torch")
+    from molten_b200.build import build_call
+    from molten_b200.decode_launch import native_call
+    build_call()
+    call, cfg = native_call(), bytes(_capi.LaunchCfg())
+    assert call is not None
+    x = ((torch.float32, (2, 3)),)
+    good = [1, 1, 1, b"k", cfg, bytes(64), ((0, 0), (8, -1)), (), x, (2, 3), torch.float32, 0]
+    c = call(*good)
+    for where, bad in ((4, b"short"), (5, bytes(2000)), (6, ((60, 0),)), (6, ((0, 1),)), (6, ((-8, 0),)), (2, 0),
+                       (7, ((0, 0, 1, bytes(32), bytes(24), bytes(16)),)), (7, ((0, 0, 1, b"", b"", b""),)),
+                       (8, ((1, (2, 3)),)), (9, [2, 3]), (10, 5)):
+        args = list(good)
+        args[where] = bad
+        with pytest.raises((ValueError, TypeError)):
+            call(*args)
+    # anything that is not a CUDA tensor of that type and shape: the general path
+    for tensors in ((), (torch.zeros(2, 3),), (torch.zeros(3, 2),), (1,), (None,), (torch.nn.Parameter(torch.zeros(2, 3)),)):
+        assert c(tensors) is NotImplemented
+    with pytest.raises(TypeError):
+        c(torch.zeros(2, 3))
+    with pytest.raises(TypeError):
+        c((), ())

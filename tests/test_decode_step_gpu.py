@@ -394,6 +394,36 @@ def test_an_infinity_in_x_stays_in_its_row(rt, dtype):
     assert not torch.isfinite(y[1:3]).any()
 
 
+@pytest.mark.parametrize("call", CALLS)
+def test_short_ways_agree(rt, call):
+    """The native short way, the same steps in Python and the general path."""
+    from molten_b200.decode_launch import ModelCall, native_call
+    assert native_call() is not None                 # (built with the rest of the library)
+    ck, ins = call(rt, 0)
+    want = ck(*ins).clone()
+    spec = ck._spec_for(ins)
+    assert isinstance(ck._last, ModelCall if call is few_call else native_call())   # (parts take a second kernel)
+    assert torch.equal(ModelCall(spec, ins)(tuple(ins)), want)
+    assert torch.equal(ck._last(tuple(ins)), want)
+    assert torch.equal(ck(*ins, out=torch.empty_like(want)), want)
+    wide = torch.zeros(ins[0].shape + (2,), dtype=ins[0].dtype, device=DEV)[..., 0]
+    for other in (tuple(ins[:-1]), (wide, *ins[1:]), (ins[0].float(), *ins[1:]) if ins[0].dtype != torch.float32
+                  else (ins[0].half(), *ins[1:]), (ins[0][:1], *ins[1:]), (ins[0].cpu(), *ins[1:])):
+        if other[0].shape != ins[0].shape or other[0].dtype != ins[0].dtype or other[0] is wide or len(other) < len(ins) \
+                or not other[0].is_cuda:
+            assert ck._last(other) is NotImplemented
+
+
+def test_short_way_of_one_token_attention(rt):
+    q, k, v = attention_inputs(2, 1, 300, 8, 2, 128, "bfloat16")
+    n = torch.tensor([300, 77], dtype=torch.int32, device=DEV)
+    for lengths in (True, False):
+        ck = window_kernel(rt, 2, 1, 300, 8, 2, 128, 100, 2, "bfloat16", lengths=lengths)
+        ins = (q, k, v, n) if lengths else (q, k, v)
+        for _ in range(3):
+            check_attention(ck(*ins), q, k, v, n if lengths else torch.full_like(n, 300), 100, 2, "bfloat16", 2.0 ** -16)
+
+
 def test_shapes_in_turn(rt):
     ck = compiled(rt, graphs.sample(4, 1000), "float32")
     cases = [(sample_inputs(r, v, "float32", r), torch.full((r,), 1.3, device=DEV))
