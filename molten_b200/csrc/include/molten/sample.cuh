@@ -29,10 +29,10 @@
 // each with all.  Rows whose kept tokens do not fit the packed list go the same
 // way with the whole row in its place.
 //
-// Measured: 1 x 32768 fp32 with top_k and top_p 23.3 us; 64 x 131072 bf16 with
+// Measured: 1 x 32768 fp32 with top_k and top_p 21.7 us; 64 x 131072 bf16 with
 // top_p and min_p, 16000 tokens kept, 100 us (132 with the tokens that are surely
 // kept left in the border's search, 109 with their weights behind a branch); 256 x
-// 100003 fp32, some rows with each filter, 158 us; the same unfiltered 103 us
+// 100003 fp32, some rows with each filter, 156 us; the same unfiltered 103 us
 // (0.99 TB/s).
 //
 // Only the tail that top_p surely drops, of which it needs nothing but the
@@ -458,16 +458,21 @@ struct Sampler {
     }
     if (tid % 32 == 0) s.red[tid / 32] = {best, 0.0f, above, 0.0};
     __syncthreads();
-    best = -INFINITY;
+    best = s.red[tid % (THREADS / 32)].x;
+    above = s.red[tid % (THREADS / 32)].z;
 #pragma unroll 1
-    for (int w = 0; w < THREADS / 32; ++w)
-      if (s.red[w].x > best) { best = s.red[w].x; above = s.red[w].z; }
+    for (int d = THREADS / 64; d >= 1; d /= 2) {
+      const float y = __shfl_xor_sync(0xffffffffu, best, d);
+      const double z = __shfl_xor_sync(0xffffffffu, above, d);
+      if (y > best) { best = y; above = z; }
+    }
     const SampleShare* ex = sm_publish(s, ranks, rank, {best, 0.0f, above, 0.0});
     best = -INFINITY;
 #pragma unroll 1
     for (int r = 0; r < ranks; ++r)
       if (ex[r].x > best) { best = ex[r].x; above = ex[r].z; }
-    *ties = ceil((need - above) / (by_weight ? weight(best) * unit : 1.0));
+    const double each = by_weight ? weight(best) * unit : 1.0;
+    *ties = need - above <= each ? 1.0 : ceil((need - above) / each);    // (a division only where values repeat)
     return best;
   }
 
@@ -653,6 +658,14 @@ __device__ __noinline__ int sample_draw(Sampler<T, THREADS>& k, int per, float l
   return lane == 0 ? owner * per + (found >= 0 ? found : last) : -1;
 }
 
+// The table of powers, before the kernel waits for the one ahead of it.
+template <typename T, int THREADS>
+__device__ __forceinline__ void sample_table(uint8_t* raw) {
+  SampleShared<T, THREADS>& sh = *reinterpret_cast<SampleShared<T, THREADS>*>(raw);
+  if (threadIdx.x < 256) sh.table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 256.0));
+}
+
+// The token of a row (behind sample_table).
 template <typename T, int THREADS>
 __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
   SampleShared<T, THREADS>& sh = *reinterpret_cast<SampleShared<T, THREADS>*>(raw);
@@ -717,7 +730,6 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
   const int behind = head + slots * VEC;
   if (behind + tid < n) xs[behind + tid] = clean(src[behind + tid]);   // (fewer than VEC)
   for (int i = n + tid; i < part; i += THREADS) xs[i] = from_f32<T>(-INFINITY);
-  if (tid < 256) sh.table[tid] = exp2((double)tid * (1.0 / 256.0));
   __syncthreads();
 
   Sampler<T, THREADS> k{sh, xs + tid * a.run, a.run, a.ranks, rank, tid, 0.0f, 0.0f, 0.0, INFINITY};

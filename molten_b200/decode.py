@@ -571,6 +571,7 @@ static_assert(sizeof(SampleShared<{t}, {sk.config['block']}>) == {_sample_fixed(
 
 extern "C" __global__ void __launch_bounds__({sk.config['block']}, {sk.config['min_ctas']}) {name}(const __grid_constant__ SampleArgs args) {{
   extern __shared__ __align__(16) uint8_t smem_raw[];
+  sample_table<{t}, {sk.config['block']}>(smem_raw);
   pdl_enter();
   sample_row<{t}, {sk.config['block']}>(args, smem_raw);
 }}
