@@ -418,29 +418,37 @@ def _plan_sample(op, sk, tune) -> dict:
     o = tune.get("sample") or {}
 
     word = 4 // DTYPE_SIZE[logits.dtype]              # tokens of 32 bits
-    # few rows: more threads, so that a pass over a thread's tokens is short (37 x 50257:
-    # 512 threads 62 us, 256 70; 128 x 32768: 83 and 50)
-    threads = int(o.get("threads") or (512 if rows * 8 <= 2 * SMS else 256))
 
-    def run_of(ranks):
+    def run_of(threads, ranks):
         # consecutive tokens of a thread: an odd number of words (no bank conflicts)
         return word * (-(-vocab // (threads * ranks * word)) | 1)
 
-    def smem_of(ranks):
-        return _sample_fixed(logits.dtype, threads) + threads * run_of(ranks) * DTYPE_SIZE[logits.dtype] + 16
-    # the fewest CTAs a row that leave room for 768 threads on an SM; more while
-    # SMs would have none and threads many tokens (16 x 32768: 4 CTAs 19.8 us, 8
-    # 27.4; 16 x 131072: 98 and 69)
-    ranks = 1
-    while ranks < 8 and (smem_of(ranks) > SMEM_SM * threads // 768 - 1024
-                         or (rows * ranks < SMS and run_of(ranks) > 24)):
-        ranks *= 2
-    ranks = int(o.get("ranks") or ranks)
+    def smem_of(threads, ranks):
+        return (_sample_fixed(logits.dtype, threads)
+                + threads * run_of(threads, ranks) * DTYPE_SIZE[logits.dtype] + 16)
+
+    def ranks_of(threads, at_once):
+        # the fewest CTAs a row that leave room for 768 threads on an SM; more
+        # where threads have many tokens and all rows still run at once (30 x
+        # 50257: 4 CTAs of 512 threads a row 42.0 us, 8 52.4; 16 x 131072: 68.5 and
+        # 50.9; 100 x 20000: 4 of 256 threads 46.9, 2 54.5)
+        ranks = 1
+        while ranks < 8 and (smem_of(threads, ranks) > SMEM_SM * threads // 768 - 1024
+                             or (rows * ranks * 2 <= at_once and run_of(threads, ranks) > 24)):
+            ranks *= 2
+        return ranks
+    # 512 threads where all rows run at once without long runs (128 x 8000: 23.5
+    # us, 256 threads 32.9; 100 x 20000: 55 and 46.9); a few clusters more than SMs
+    # still count as at once
+    wide = ranks_of(512, SMS * 11 // 10)
+    few = rows * wide <= SMS * 11 // 10 and (wide == 8 or run_of(512, wide) <= 36)
+    threads = int(o.get("threads") or (512 if few else 256))
+    ranks = int(o.get("ranks") or (wide if few and threads == 512 else ranks_of(threads, SMS * 28 // 10)))
     # (a token's index within its CTA's part has 16 bits)
-    _need(smem_of(ranks) <= SMEM_LIMIT and threads * run_of(ranks) <= 65536,
+    _need(smem_of(threads, ranks) <= SMEM_LIMIT and threads * run_of(threads, ranks) <= 65536,
           f"sample: a vocabulary of {vocab} does not fit the shared memory of a cluster")
-    return {"rows": rows, "vocab": vocab, "ranks": ranks, "run": run_of(ranks),
-            "smem": smem_of(ranks), "block": threads,
+    return {"rows": rows, "vocab": vocab, "ranks": ranks, "run": run_of(threads, ranks),
+            "smem": smem_of(threads, ranks), "block": threads,
             "min_ctas": int(o.get("min_ctas") or max(1, 768 // threads)), "params": list(op.attrs.get("params", ())),
             "flops": 2 * rows * vocab}
 
