@@ -154,7 +154,9 @@ typedef struct molten_window_args {
  * from molten_encode_tma_4d: q [dim, heads, nq, batch] in boxes of {64, per,
  * positions, 1}, k and v [dim, kv_heads, cache, batch] in boxes of {64, 1, 128,
  * 1}.  positions = 128 / per; blocks = ceil(nq / (2 positions)); the grid is
- * at most one CTA per SM. */
+ * at most one CTA per SM.  With parts > 1 the kernel "<name>_join" follows with
+ * the same block, a warp to each of batch * kv_heads * blocks * 256 rows, and
+ * `part` holds that number * parts * (dim + 4) floats, 16-byte aligned; parts <= 32. */
 typedef struct molten_window_tc_args {
   MOLTEN_ALIGN64 unsigned char tmap_q[128];
   MOLTEN_ALIGN64 unsigned char tmap_k[128];
@@ -167,7 +169,9 @@ typedef struct molten_window_tc_args {
   int batch, nq, cache, kv_heads, per, dim;
   int window, sinks;             /* window < 0: every earlier key */
   float scale_log2;              /* scale * log2(e), positive */
-  int positions, blocks, reserved;
+  int positions, blocks;
+  int parts;                     /* CTAs that share the keys of an item */
+  float* part;                   /* parts > 1: work space (below) */
 } molten_window_tc_args;
 
 /* Parameter block of the sampling kernels (device side: molten::SampleArgs in

@@ -122,8 +122,8 @@ class WindowTcArgs(ctypes.Structure):
                 + [(n, ctypes.c_int) for n in ("batch", "nq", "cache", "kv_heads", "per", "dim",
                                                "window", "sinks")]
                 + [("scale_log2", ctypes.c_float)]
-                + [(n, ctypes.c_int) for n in ("positions", "blocks", "reserved")]
-                + [("tail_", ctypes.c_ubyte * 24)])
+                + [(n, ctypes.c_int) for n in ("positions", "blocks", "parts")]
+                + [("part", ctypes.c_void_p), ("tail_", ctypes.c_ubyte * 16)])
 
 
 class SampleArgs(ctypes.Structure):

@@ -41,6 +41,10 @@
 // half's S loaded ahead: 267.  The waits for S and P poll (all asleep: 270; all
 // polling without a pause: 293), the others, of warps with time, sleep.
 //
+// Where items are fewer than SMs, several CTAs share the key tiles of one; a
+// second kernel joins their sums (1 x 64 tokens over 8000, window 4096: 69 -> 36
+// us; 1 x 128 over 30000: 425 -> 74).
+//
 // P = 0 times an infinity or NaN is NaN, so V rows that no query of the item
 // sees (behind the length, before the window) are zeroed in shared memory
 // before their MMA, and so are infinities and NaN in rows that only some
@@ -69,7 +73,8 @@ struct alignas(64) WindowTcArgs {
   float scale_log2;                // scale * log2(e), positive
   int positions;                   // positions of one Q tile
   int blocks;                      // pairs of Q tiles of a request
-  int reserved;
+  int parts;                       // CTAs that share the key tiles of an item
+  float* part;                     // parts > 1: [item][Q tile][128 rows][dim sums, offset, sum of weights, 2 unused]
 };
 
 enum WindowTcStatus { kWindowTimeout = 2048 };
@@ -134,14 +139,17 @@ __device__ __forceinline__ void window_tc_fail(const WindowTcShared& s, const Wi
 
 // The key tiles of a work item: [0, sink) and [start, end) in ascending order;
 // of these Q tile t needs those below need_sink[t] and in [lo[t], hi[t]).
+// PARTS: items are shared by args.parts CTAs, each with a run of the tiles.
+template <bool PARTS>
 struct WindowItem {
   int b, h, first, len;            // first: position of query 0
   int i0;                          // first query of the item
-  int sink, start, end, tiles;
+  int sink, start, end, tiles, skip;   // skip: tiles of the parts before
   int lo[2], hi[2], need_sink[2];
   int pa[2], pb[2];                // positions of the Q tiles' first and last rows; pb < pa: none
   __device__ __forceinline__ WindowItem(const WindowTcArgs& a, int item) {
-    const int block = item % a.blocks, rest = item / a.blocks;
+    const int part = PARTS ? item % a.parts : 0, whole_item = PARTS ? item / a.parts : item;
+    const int block = whole_item % a.blocks, rest = whole_item / a.blocks;
     h = rest % a.kv_heads;
     b = rest / a.kv_heads;
     int n = a.lengths ? a.lengths[b] : a.cache;
@@ -174,11 +182,27 @@ struct WindowItem {
     else if (pb[0] >= pa[0] && pb[1] >= pa[1]) sink = min(max(need_sink[0], need_sink[1]), start);
     else sink = min(sink, start);
     tiles = sink + end - start;
+    skip = 0;
+    if constexpr (PARTS) {
+      skip = (int)((long long)tiles * part / a.parts);
+      tiles = (int)((long long)tiles * (part + 1) / a.parts) - skip;
+    }
   }
-  __device__ __forceinline__ int tile(int u) const { return u < sink ? u : u - sink + start; }
+  __device__ __forceinline__ int tile(int u) const {
+    const int v = PARTS ? u + skip : u;
+    return v < sink ? v : v - sink + start;
+  }
   // (selects, not an index: the members stay in registers where t is a variable)
   static __device__ __forceinline__ int of(const int (&x)[2], int t) { return t == 0 ? x[0] : x[1]; }
   __device__ __forceinline__ bool any(int t) const { return of(pb, t) >= of(pa, t); }
+  // (tiles ascend: some tile of this part is among the sinks' or the window's)
+  __device__ __forceinline__ bool has(int t) const {
+    if (!PARTS || !any(t)) return any(t);
+    if (tiles == 0) return false;
+    const int j0 = tile(0), j1 = tile(tiles - 1);
+    return j0 < of(need_sink, t) ||
+           max(max(j0, start), of(lo, t)) <= min(j1, of(hi, t) - 1);
+  }
   __device__ __forceinline__ bool need(int t, int j) const {
     return any(t) && (j < of(need_sink, t) || (j >= of(lo, t) && j < of(hi, t)));
   }
@@ -232,6 +256,15 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* u) {
                  "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]),
                  "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31]) : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&u)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
+        "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -282,9 +315,9 @@ __device__ __forceinline__ void window_tc_init(const WindowTcShared& s, const Wi
 // Infinities and NaN of V that were cleaned away, added to the stored output
 // row of position p from the keys it sees (any weight above 0 carries them into
 // the sum).
-template <typename T, typename OT>
+template <bool PARTS, typename T, typename OT>
 __device__ __noinline__ void window_tc_add_dirty(const WindowTcArgs& args, int item, int p, OT* dst) {
-  const WindowItem w(args, item);
+  const WindowItem<PARTS> w(args, item);
 #pragma unroll 1
   for (int u = 0; u < w.tiles; ++u) {
     const int j = w.tile(u);
@@ -312,7 +345,7 @@ __device__ __forceinline__ uint32_t window_tc_zeros(uint32_t x, uint32_t sum) {
   return sum;
 }
 
-template <class L, typename T, typename OT>
+template <class L, typename T, typename OT, bool PARTS>
 __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const WindowTcArgs& args) {
   constexpr bool F16IN = std::is_same<T, f16>::value;
   constexpr uint32_t S = L::STAGES;
@@ -320,7 +353,7 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t tmem = *s.tmem_slot;
   const WindowTcBars<L> bar{s.bars};
-  const int items = args.batch * args.kv_heads * args.blocks;
+  const int items = args.batch * args.kv_heads * args.blocks * (PARTS ? args.parts : 1);
   // ring entries in order K, V, K, V ...: entry e lies in stage e % S, and the
   // barriers of its e / S-th use have that parity; V tile e / 2 is passed on by
   // the cleaning warps through barrier clean(e / 2 % S)
@@ -335,7 +368,7 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
     if (lane == 0) {
       const uint32_t q_bytes = (uint32_t)(L::DCH * 128 * args.per * args.positions);
       uint32_t entry = 0, qn[2] = {0, 0};
-      auto load = [&](const CUtensorMap* map, const WindowItem& w, int j) {
+      auto load = [&](const CUtensorMap* map, const WindowItem<PARTS>& w, int j) {
         const uint32_t st = entry % S;
         if (!wait(bar.empty(st), entry / S + 1u)) return;
         mbar_expect_tx(bar.full(st), (uint32_t)L::STAGE_BYTES);
@@ -346,9 +379,9 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
         ++entry;
       };
       for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
-        const WindowItem w(args, it);
+        const WindowItem<PARTS> w(args, it);
         for (int t = 0; t < 2; ++t) {
-          if (w.pb[t] < w.pa[t]) continue;
+          if (!w.has(t)) continue;
           if (!wait(bar.q_empty(t), qn[t] + 1u)) break;
           ++qn[t];
           mbar_expect_tx(bar.q_full(t), q_bytes);
@@ -398,7 +431,7 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
       const uint64_t by_row = umma_desc(0u, 16u, 1024u), by_col = umma_desc(0u, (uint32_t)L::CHUNK, 1024u);
       const uint32_t q_at = smem_u32(s.q) >> 4, ring_at = smem_u32(s.ring) >> 4;
       for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
-        const WindowItem w(args, it);
+        const WindowItem<PARTS> w(args, it);
         bool begun[2] = {false, false}, asked[2] = {false, false};   // O_t holds sums; Q_t is there
         bool needed[2] = {false, false};             // by Q tile t: the key tile before
         // step u: P V of tile u - 1 and S of tile u, for either Q tile in turn
@@ -486,7 +519,7 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
     // barriers cannot run ahead of these warps)
     uint32_t n = 0, seq = 0;
     for (int it = blockIdx.x; it < items && ok; it += gridDim.x, ++seq) {
-      const WindowItem w(args, it);
+      const WindowItem<PARTS> w(args, it);
       const bool v0 = w.pb[0] >= w.pa[0], v1 = w.pb[1] >= w.pa[1];
       const int pa = v0 ? w.pa[0] : w.pa[1], pb = v1 ? w.pb[1] : w.pb[0];
       for (int u = 0; u < w.tiles && ok; ++u) {
@@ -553,13 +586,13 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
     const float slack = 8.0f / C2;                   // growth of the maximum left in the weights
     uint32_t sn = 0, rn = 0, seq = 0;                // tiles of S; items with any
     for (int it = blockIdx.x; it < items && ok; it += gridDim.x, ++seq) {
-      const WindowItem w(args, it);
+      const WindowItem<PARTS> w(args, it);
       const int i = w.i0 + t * args.positions + r / args.per;    // this row's query
       const bool real = r < args.per * args.positions && i < args.nq;
       const int p = w.first + i;
       // weights are 2^(x C2 + off); a logit above `limit` moves `off`
       float off = 0.0f, limit = -INFINITY, sum = 0.0f;
-      const bool run = w.any(t);
+      const bool run = w.has(t);
       if (run) {
         bool begun = false;
         for (int u = 0; u < w.tiles; ++u) {
@@ -670,6 +703,31 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
       }
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       const bool dirty = s.dirty[seq & 7u] == (int)seq + 1;
+      if constexpr (PARTS) {
+        // this part's sums as they are, with their offset (+inf: no key seen)
+        float* mine = args.part + ((long long)(it * 2 + t) * 128 + r) * (args.dim + 4);
+#pragma unroll 1
+        for (int c = 0; c < L::DP; c += 16) {
+          uint32_t o[16];
+          if (run) tmem_ld16(o_at + c, o);
+          if (!real || !run || c >= args.dim) continue;
+#pragma unroll
+          for (int q = 0; q < 16; q += 4)
+            if (c + q < args.dim)
+              *reinterpret_cast<uint4*>(mine + c + q) = make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]);
+        }
+        if (real) {
+          *reinterpret_cast<float2*>(mine + args.dim) =
+              limit == -INFINITY && sum == 0.0f ? make_float2(INFINITY, 0.0f) : make_float2(off, sum);
+          if (dirty && run) window_tc_add_dirty<PARTS, T, float>(args, it, p, mine);
+        }
+        if (run) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar.o_free(t));
+        }
+        continue;
+      }
       OT* dst = static_cast<OT*>(args.out) +
                 (((long long)w.b * args.nq + i) * args.kv_heads * args.per + w.h * args.per + r % args.per) *
                     (long long)args.dim;
@@ -704,13 +762,60 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
           }
         }
       }
-      if (dirty && real) window_tc_add_dirty<T, OT>(args, it, p, dst);
+      if (dirty && real) window_tc_add_dirty<PARTS, T, OT>(args, it, p, dst);
       if (run) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar.o_free(t));
       }
     }
+  }
+}
+
+// The parts of each row joined: a warp to a row of a Q tile.  With o_p the sums
+// under offset off_p, o = sum_p o_p 2^(off - off_p) for off = min off_p.
+template <typename OT>
+__device__ __forceinline__ void window_tc_join(const WindowTcArgs& args) {
+  const int lane = threadIdx.x % 32, pitch = args.dim + 4;
+  const long long id = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  const int r = (int)(id % 128), t = (int)(id / 128 % 2);
+  const long long item = id / 256;                   // without the part
+  if (item >= (long long)args.batch * args.kv_heads * args.blocks) return;
+  const int block = (int)(item % args.blocks);
+  const long long rest = item / args.blocks;
+  const int h = (int)(rest % args.kv_heads), b = (int)(rest / args.kv_heads);
+  const int i = (block * 2 + t) * args.positions + r / args.per;
+  if (r >= args.per * args.positions || i >= args.nq) return;
+  const float* mine = args.part + ((item * args.parts * 2 + t) * 128 + r) * (long long)pitch;
+  const long long step = 256ll * pitch;              // to the next part
+  // a lane to a part: its offset and weight (32 parts at most)
+  float2 z = make_float2(INFINITY, 0.0f);
+  if (lane < args.parts) z = *reinterpret_cast<const float2*>(mine + lane * step + args.dim);
+  float off = z.x, sum;
+#pragma unroll
+  for (int d = 16; d >= 1; d /= 2) off = fminf(off, __shfl_xor_sync(0xffffffffu, off, d));
+  const float f = z.x == INFINITY ? 0.0f : fast_exp2(off - z.x);     // +inf: it saw no key
+  sum = z.x == INFINITY ? 0.0f : z.y * f;
+#pragma unroll
+  for (int d = 16; d >= 1; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int p = 0; p < args.parts; ++p) {
+    const float fp = __shfl_sync(0xffffffffu, f, p);
+    const bool none = __shfl_sync(0xffffffffu, z.x, p) == INFINITY;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = lane + 32 * q;
+      const float x = !none && c < args.dim ? mine[p * step + c] : 0.0f;
+      o[q] += isfinite(x) ? x * fp : x;              // (an infinity stays one under any weight)
+    }
+  }
+  OT* dst = static_cast<OT*>(args.out) +
+            (((long long)b * args.nq + i) * args.kv_heads * args.per + h * args.per + r % args.per) * args.dim;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int c = lane + 32 * q;
+    if (c < args.dim) dst[c] = from_f32<OT>(sum == 0.0f ? 0.0f : o[q] / sum);
   }
 }
 

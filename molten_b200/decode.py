@@ -401,8 +401,16 @@ def _plan_window_tiles(c: dict, o: dict) -> dict:
     bars = 3 * stages + 17
     smem = 2 * dch * 16384 + stages * dch * 16384 + bars * 8 + 48 + 1024
     _need(smem <= SMEM_LIMIT, f"window_attention: {stages} stages need {smem} bytes")
+    # fewer items than SMs: CTAs share an item's key tiles, at least two each (a
+    # tile takes some 1.9 us, the join some 5)
+    span = c["cache"] if c["window"] < 0 else min(c["cache"], c["window"] + c["sinks"] + 2 * positions)
+    tiles = span // 128 + 2
+    parts = max(1, min(SMS // max(items, 1), tiles // 2, 32))
+    parts = int(o.get("parts") or (parts if parts > 1 and tiles > 5 else 1))
+    _need(parts <= 32, f"window_attention: {parts} parts; at most 32")
+    _need(items * parts < 2 ** 31 // 256, "window_attention: sizes beyond the kernel's range")
     c.update(kind="tiles", positions=positions, blocks=blocks, items=items, stages=stages,
-             smem=smem, block=384, ranks=1, parts=1)
+             smem=smem, block=384, ranks=1, parts=parts)
     return c
 
 
@@ -468,7 +476,8 @@ def launch_record(sk: SubKernel) -> dict:
         rec.update(grid=c["rows"] * c["ranks"], cluster=c["ranks"])
     elif c["op"] == ModelOpType.WINDOW_ATTENTION:
         if c["kind"] == "tiles":
-            rec.update(kind="tiles", positions=c["positions"], blocks=c["blocks"], items=c["items"])
+            rec.update(kind="tiles", positions=c["positions"], blocks=c["blocks"], items=c["items"],
+                       parts=c["parts"])
         else:
             rec.update(kind="few", cluster=c["ranks"], parts=c["parts"], smem=c["smem_launch"],
                        grid=c["items"] * c["parts"] * c["ranks"])
@@ -539,10 +548,15 @@ extern "C" __global__ void __launch_bounds__({c['block']}, 1) {name}(const __gri
   window_tc_init<Layout_{name}>(sh, args);     // mbarriers + TMEM allocation
   pdl_enter();                                 // no global access before this
   __syncthreads();
-  window_tc_roles<Layout_{name}, {t}, {ot}>(sh, args);
+  window_tc_roles<Layout_{name}, {t}, {ot}, {_bool(c['parts'] > 1)}>(sh, args);
   tc_fence_before();
   __syncthreads();
   window_tc_teardown<Layout_{name}>(sh);       // TMEM release
+}}
+
+extern "C" __global__ void __launch_bounds__(256) {name}_join(const __grid_constant__ WindowTcArgs args) {{
+  pdl_enter();
+  window_tc_join<{ot}>(args);
 }}
 """
     lay = f"{c['dp']}, {c['nb']}, {c['warps']}, {c['stages']}"

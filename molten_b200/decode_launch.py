@@ -198,8 +198,11 @@ class _Window(_Bound):
     def setup(self):
         c = self.c
         if c["kind"] == "tiles":
-            self.cfg = self.config(min(c["items"], SMS), c["block"], 1, c["smem"])
+            self.cfg = self.config(min(c["items"] * c["parts"], SMS), c["block"], 1, c["smem"])
             self.rest = self.tail(_capi.WindowTcArgs, "batch")
+            self.part = c["items"] * 256 * c["parts"] * (c["dim"] + 4) if c["parts"] > 1 else 0
+            self.part_at = _capi.WindowTcArgs.part.offset - _capi.WindowTcArgs.batch.offset
+            self.join = self.config(c["items"] * 32, 256)
             self.status = _capi.status_word(self.device)
             self.code = _capi.DT_BF16 if self.sk.operands[0].dtype == "bfloat16" else _capi.DT_F16
         else:
@@ -215,7 +218,7 @@ class _Window(_Bound):
         a.per, a.dim, a.window, a.sinks = c["per"], c["dim"], c["window"], c["sinks"]
         a.scale_log2 = c["scale"] * LOG2E
         if c["kind"] == "tiles":
-            a.positions, a.blocks = c["positions"], c["blocks"]
+            a.positions, a.blocks, a.parts = c["positions"], c["blocks"], c["parts"]
         else:
             a.ranks, a.parts = c["ranks"], c["parts"]
 
@@ -257,6 +260,8 @@ class _Window(_Bound):
         d, kv, heads = c["dim"], c["kv_heads"], c["kv_heads"] * c["per"]
         q, k = (c["new"] * heads * d, heads * d, d), (c["cache"] * kv * d, kv * d, d)
         lengths = [(0, 3)] if len(self.sk.operands) > 3 else []
+        if self.part:
+            return None
         if c["kind"] == "tiles":
             maps = [(128 * n, n, self.code, self.dims.pack(d, h, s, c["batch"]),
                      self.strides.pack(2 * st[2], 2 * st[1], 2 * st[0]), self.box.pack(*box))
@@ -265,8 +270,6 @@ class _Window(_Bound):
                         + 2 * [(kv, c["cache"], k, (64, 1, 128, 1))])]
             return (bytes(384) + self.tiles_head.pack(0, 0, 0, self.status, *k) + self.rest,
                     [(384, 2)] + [(392 + at, j) for at, j in lengths] + [(400, -1)], maps)
-        if self.part:
-            return None
         return (self.head.pack(0, 0, 0, 0, 0, 0, *q, *k, *k) + self.rest,
                 [(0, 0), (8, 1), (16, 2)] + [(24 + at, j) for at, j in lengths] + [(32, -1)], [])
 
@@ -275,16 +278,22 @@ class _Window(_Bound):
         lengths = ins[3].data_ptr() if len(ins) > 3 else 0
         c = self.c
         self.need_aligned(-1, out, 16)
-        if c["kind"] == "tiles":
-            block = (self.tensor_maps(ins)
-                     + self.tiles_head.pack(v.data_ptr(), lengths, out.data_ptr(), self.status,
-                                            *v.stride()[:3]))
-            self.launch(block + self.rest, stream)
-            return
         part = None
         if self.part:
             import torch
             part = torch.empty(self.part, dtype=torch.float32, device=q.device)
+        if c["kind"] == "tiles":
+            block = (self.tensor_maps(ins)
+                     + self.tiles_head.pack(v.data_ptr(), lengths, out.data_ptr(), self.status,
+                                            *v.stride()[:3]))
+            rest = self.rest
+            if part is not None:
+                rest = (rest[:self.part_at] + part.data_ptr().to_bytes(8, "little")
+                        + rest[self.part_at + 8:])
+            self.launch(block + rest, stream)
+            if part is not None:
+                self.launch(block + rest, stream, self.join[0], self.entry + b"_join")
+            return
         block = self.head.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), lengths, out.data_ptr(),
                                0 if part is None else part.data_ptr(),
                                *q.stride()[:3], *k.stride()[:3], *v.stride()[:3]) + self.rest

@@ -431,6 +431,35 @@ def test_window_attention_many_rows(rt, case, dtype):
     assert torch.equal(out, ck(q, k, v, lengths))
 
 
+@pytest.mark.parametrize("parts", [1, 2, 3, 7, 32])
+@pytest.mark.parametrize("case", [
+    (1, 40, 1000, 8, 2, 128, 300, 5, [1000]), (2, 90, 700, 6, 2, 64, None, 0, [700, 40]),
+    (1, 300, 2000, 4, 4, 80, 130, 200, [1900]), (3, 65, 300, 7, 1, 128, 17, 1, [300, 0, 66])])
+def test_window_attention_many_rows_in_parts(parts, case):
+    """CTAs that share the key tiles of an item; some see no key of some Q tile."""
+    b, new, cache, heads, kv, d, window, sinks, lens = case
+    q, k, v = attention_inputs(b, new, cache, heads, kv, d, "bfloat16", seed=cache)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    # (compiled for other sizes: the call's plan takes the given parts)
+    ck = window_kernel(MoltenRuntime(tune={"window": {"parts": parts}}), 1, 130, 140, heads, kv, d, window, sinks,
+                       "bfloat16")
+    out = ck(q, k, v, lengths)
+    assert ck.specialization(q, k, v, lengths).plan.kernels[0].config["parts"] == parts
+    check_attention(out, q, k, v, lengths, window, sinks, "bfloat16", 2.0 ** -8)
+    assert torch.equal(ck(q, k, v, lengths), out)
+    # an infinity of V that some queries see, and one behind the lengths
+    v = v.clone()
+    v[0, lens[0] - 2, 0, 3] = torch.inf
+    v[:, max(lens):] = torch.nan
+    bad = ck(q, k, v, lengths)
+    seen = seen_mask(lengths, new, cache, window, sinks)[0, :, lens[0] - 2]
+    per = heads // kv
+    assert (bad[0, seen][:, :per, 3] == torch.inf).all()
+    keep = torch.ones_like(out, dtype=torch.bool)
+    keep[0, :, :per, 3] = ~seen[:, None]
+    assert torch.equal(bad[keep], out[keep])
+
+
 @pytest.mark.parametrize("spread", [8.0, 60.0])
 def test_window_attention_growing_maxima(rt, spread):
     """Scores whose maxima grow along the keys: O is rescaled, and large

@@ -187,7 +187,9 @@ def few_call(rt, seed=0):
 def tiles_call(rt, seed=0):
     q, k, v = attention_inputs(2, 100, 300, 8, 2, 64, "float16", seed)
     n = torch.tensor([300, 120 + seed], dtype=torch.int32, device=DEV)
-    return window_kernel(rt, 2, 100, 300, 8, 2, 64, 70, 3, "float16"), [q, k, v, n]
+    ck = window_kernel(rt, 2, 100, 300, 8, 2, 64, 70, 3, "float16")
+    assert ck.kernel.plan.kernels[0].config["parts"] == 1
+    return ck, [q, k, v, n]
 
 
 def sample_call(rt, seed=0):
@@ -197,7 +199,15 @@ def sample_call(rt, seed=0):
     return ck, [x, u, t, torch.tensor([0, 1, 50, 3000 + seed, 10], dtype=torch.int32, device=DEV)]
 
 
-CALLS = [q4_call, rope_call, few_call, tiles_call, sample_call]
+def parts_call(rt, seed=0):
+    q, k, v = attention_inputs(1, 70, 2000, 4, 1, 128, "bfloat16", seed)
+    n = torch.tensor([1900 + seed], dtype=torch.int32, device=DEV)
+    ck = window_kernel(rt, 1, 70, 2000, 4, 1, 128, 1500, 3, "bfloat16")
+    assert ck.kernel.plan.kernels[0].config["parts"] > 1
+    return ck, [q, k, v, n]
+
+
+CALLS = [q4_call, rope_call, few_call, tiles_call, parts_call, sample_call]
 
 
 @pytest.mark.parametrize("call", CALLS)
@@ -402,7 +412,7 @@ def test_short_ways_agree(rt, call):
     ck, ins = call(rt, 0)
     want = ck(*ins).clone()
     spec = ck._spec_for(ins)
-    assert isinstance(ck._last, ModelCall if call is few_call else native_call())   # (parts take a second kernel)
+    assert isinstance(ck._last, ModelCall if call in (few_call, parts_call) else native_call())   # (parts: a second kernel)
     assert torch.equal(ModelCall(spec, ins)(tuple(ins)), want)
     assert torch.equal(ck._last(tuple(ins)), want)
     assert torch.equal(ck(*ins, out=torch.empty_like(want)), want)
