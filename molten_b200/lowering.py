@@ -241,7 +241,9 @@ class GroupPlan:
     output_shapes: list
     kernels: list         # [SubKernel]
     temps: dict           # op id -> (shape, dtype) of intermediates
-    key: str = ""         # what tells plans of the same source apart (sizes passed at launch)
+    # what tells plans of the same source apart: which input feeds which operand,
+    # and sizes passed at launch
+    key: str = ""
 
 
 # ------------------------------------------------------------ group split

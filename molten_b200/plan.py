@@ -144,8 +144,8 @@ def plan_group(graph: DataflowGraph, group_op_ids, input_shapes: dict,
         outputs=list(outs), output_dtypes=[dts[o] for o in outs],
         output_shapes=[shapes[o] for o in outs],
         kernels=kernels, temps=temps,
-        key=repr([(sk.op_ids, sk.config) for sk in kernels if sk.family == "model"])
-        if any(sk.family == "model" for sk in kernels) else "")
+        key=repr((inputs, outs, [(o, graph.ops[o].inputs) for o in ordered],
+                  [(sk.op_ids, sk.config) for sk in kernels if sk.family == "model"])))
 
 
 SPLIT3_BLOCK = 256

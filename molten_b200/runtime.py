@@ -724,7 +724,8 @@ class MoltenRuntime:
         _capi.load_library()           # fail loudly when the runtime is missing
 
     def compile(self, kernel: GeneratedKernel) -> CompiledKernel:
-        # (the sources of model operators leave sizes to the launch: plan.key)
+        # (a source does not say which inputs its operands are, and those of model
+        # operators leave sizes to the launch: plan.key)
         text = kernel.source + (kernel.plan.key if kernel.plan is not None else "")
         key = hashlib.sha256(text.encode()).hexdigest()[:16]
         ck = self._compiled.get(key)

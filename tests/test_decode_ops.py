@@ -361,3 +361,52 @@ def test_short_call_checks_its_plan_and_its_tensors():
         c(torch.zeros(2, 3))
     with pytest.raises(TypeError):
         c((), ())
+
+
+# ------------------------------------------- which compiled kernel a graph gets
+@pytest.fixture
+def unbuilt(monkeypatch, tmp_path):
+    """A runtime that builds no cubins."""
+    from molten_b200 import runtime
+    monkeypatch.setattr(runtime, "build_cubin", lambda source, name, *a, **kw: tmp_path / f"{name}.cubin")
+    return runtime.MoltenRuntime(cache_dir=str(tmp_path))
+
+
+def wired(order, build, shapes, dtypes):
+    """A graph whose inputs are declared in ``order``."""
+    g = DataflowGraph("wired")
+    ids = {n: g.add_input(n, TS(shapes[n]), dtype=dtypes.get(n, "bfloat16")) for n in order}
+    g.add_output(build(g, ids))
+    return g
+
+
+WIRED = {
+    "window_attention": (("q", "k", "v"), ("q", "v", "k"), lambda g, i: g.window_attention(i["q"], i["k"], i["v"]),
+                         {n: [1, 4, 2, 64] for n in "qkv"}, {}),
+    "matvec_q4": (("x", "w", "s", "z"), ("x", "w", "z", "s"),
+                  lambda g, i: g.matvec_q4(i["x"], i["w"], i["s"], zeros=i["z"]),
+                  {"x": [2, 256], "w": [32, 128], "s": [32, 2], "z": [32, 2]}, {"w": "uint8"}),
+    "rope_positions": (("x", "c", "s", "p"), ("x", "s", "c", "p"),
+                       lambda g, i: g.rope(i["x"], i["c"], sin=i["s"], positions=i["p"]),
+                       {"x": [2, 5, 2, 64], "c": [9, 32], "s": [9, 32], "p": [1, 2, 5]},
+                       {"c": "float32", "s": "float32", "p": "int32"}),
+    "sample": (("x", "u", "t", "p"), ("x", "u", "p", "t"),
+               lambda g, i: g.sample(i["x"], i["u"], temperature=i["t"], top_p=i["p"]),
+               {"x": [3, 100], "u": [3], "t": [3], "p": [3]}, {n: "float32" for n in "utp"}),
+    "matmul": (("a", "b"), ("b", "a"), lambda g, i: g.matmul(i["a"], i["b"]), {n: [256, 256] for n in "ab"}, {}),
+    "rope": (("x", "c", "s"), ("x", "s", "c"), lambda g, i: g.rope(i["x"], i["c"], sin=i["s"]),
+             {"x": [1, 5, 2, 64], "c": [5, 32], "s": [5, 32]}, {}),
+}
+
+
+@pytest.mark.parametrize("name", WIRED)
+def test_inputs_in_another_order_are_another_kernel(name, unbuilt):
+    """The same source with its operands fed from other inputs."""
+    first, second, build, shapes, dtypes = WIRED[name]
+    ks = [compile_graph(wired(order, build, shapes, dtypes), dtype="bfloat16")[0] for order in (first, second, first)]
+    cks = [unbuilt.compile(k) for k in ks]
+    assert ks[0].source == ks[1].source
+    assert cks[0] is not cks[1] and cks[0] is cks[2]
+    for ck, k in zip(cks, ks):
+        for a, b in zip(ck.kernel.plan.kernels, k.plan.kernels):
+            assert [(o.index, o.op_id) for o in a.operands] == [(o.index, o.op_id) for o in b.operands]
