@@ -242,7 +242,7 @@ class GroupPlan:
     kernels: list         # [SubKernel]
     temps: dict           # op id -> (shape, dtype) of intermediates
     # what tells plans of the same source apart: which input feeds which operand,
-    # and sizes passed at launch
+    # attributes and sizes passed at launch
     key: str = ""
 
 

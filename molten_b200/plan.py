@@ -144,7 +144,10 @@ def plan_group(graph: DataflowGraph, group_op_ids, input_shapes: dict,
         outputs=list(outs), output_dtypes=[dts[o] for o in outs],
         output_shapes=[shapes[o] for o in outs],
         kernels=kernels, temps=temps,
-        key=repr((inputs, outs, [(o, graph.ops[o].inputs) for o in ordered],
+        # (attributes as they were given: other shapes are planned from them)
+        key=repr((inputs, outs,
+                  [(o, graph.ops[o].op_type.name, graph.ops[o].inputs, graph.ops[o].attrs)
+                   for o in ordered + [i for i in ext if i not in inputs]],
                   [(sk.op_ids, sk.config) for sk in kernels if sk.family == "model"])))
 
 

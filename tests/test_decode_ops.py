@@ -410,3 +410,26 @@ def test_inputs_in_another_order_are_another_kernel(name, unbuilt):
     for ck, k in zip(cks, ks):
         for a, b in zip(ck.kernel.plan.kernels, k.plan.kernels):
             assert [(o.index, o.op_id) for o in a.operands] == [(o.index, o.op_id) for o in b.operands]
+
+
+@pytest.mark.parametrize("one,other", [
+    (dict(window=None), dict(window=1000)), (dict(sinks=256), dict(sinks=5000)),
+    (dict(scale=None), dict(scale=64 ** -0.5)), (dict(window=513), dict(window=None))])
+def test_attributes_that_a_shape_hides_are_another_kernel(one, other, unbuilt):
+    """A window wider than the declared cache is no limit there, but one in a
+    longer cache: kernels are planned again for other shapes."""
+    import torch
+    from molten_b200 import runtime
+    args = (2, 1, 256, 8, 2, 64)
+    ks = [compile_graph(graphs.window_attention(*args, **kw), dtype="bfloat16")[0] for kw in (one, other, one)]
+    assert ks[0].source == ks[1].source and ks[0].plan.kernels[0].config == ks[1].plan.kernels[0].config
+    cks = [unbuilt.compile(k) for k in ks]
+    assert cks[0] is not cks[1] and cks[0] is cks[2]
+    # and each plans a longer cache, and wider heads, with its own attributes
+    for ck, kw in zip(cks, (one, other)):
+        tensors = [torch.empty(s, device="meta", dtype=t) for s, t in (
+            ((2, 1, 8, 128), torch.bfloat16), ((2, 9000, 2, 128), torch.bfloat16), ((2, 9000, 2, 128), torch.bfloat16),
+            ((2,), torch.int32))]
+        got = ck.specialization(*tensors).plan.kernels[0].config
+        want = config_of(graphs.window_attention(2, 1, 9000, 8, 2, 128, **kw), "bfloat16")
+        assert got == want
