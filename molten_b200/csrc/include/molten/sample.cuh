@@ -671,6 +671,9 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
   SampleShared<T, THREADS>& sh = *reinterpret_cast<SampleShared<T, THREADS>*>(raw);
   constexpr int VEC = 16 / sizeof(T);
   const int rank = blockIdx.x % a.ranks, row = blockIdx.x / a.ranks, tid = threadIdx.x;
+  // every CTA of the cluster has started: waited for before the first store to
+  // another's shared memory (a rank with few tokens or none gets there at once)
+  if (a.ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int part = THREADS * a.run, base = rank * part;
   const int n = max(0, min(part, a.vocab - base));
   const T* src = static_cast<const T*>(a.logits) + row * a.row_stride + base;
@@ -734,6 +737,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
 
   Sampler<T, THREADS> k{sh, xs + tid * a.run, a.run, a.ranks, rank, tid, 0.0f, 0.0f, 0.0, INFINITY};
   const T* mine = k.mine;
+  if (a.ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   const SampleShare range = sm_combine<THREADS>(sh, a.ranks, rank, {top, -bottom, (double)finite, 0.0});
   k.m = range.x;
   if (k.m == -INFINITY) {                            // nothing can be drawn

@@ -433,3 +433,19 @@ def test_attributes_that_a_shape_hides_are_another_kernel(one, other, unbuilt):
         got = ck.specialization(*tensors).plan.kernels[0].config
         want = config_of(graphs.window_attention(2, 1, 9000, 8, 2, 128, **kw), "bfloat16")
         assert got == want
+
+
+# ------------------------------------------------------------------- clusters
+@pytest.mark.parametrize("header,entry,first", [
+    ("sample.cuh", "void sample_row(", "sm_combine<"), ("window_decode.cuh", "void window_decode(", "mapa.shared::cluster"),
+    ("q4_matvec.cuh", "void q4_matvec(", "mapa.shared::cluster")])
+def test_clusters_have_started_before_their_memory_is_used(header, entry, first):
+    """Shared memory of another CTA of a cluster exists once that CTA runs: a
+    kernel meets at a cluster barrier before its first access there."""
+    from molten_b200.build import CSRC_DIR
+    text = (CSRC_DIR / "include" / "molten" / header).read_text()
+    body = text[text.index(entry):]
+    before = body[:body.index(first)]
+    assert "barrier.cluster.wait" in before or "q4_cluster_sync()" in before
+    if "barrier.cluster.wait" in before:
+        assert before.index("barrier.cluster.arrive") < before.index("barrier.cluster.wait")

@@ -670,3 +670,19 @@ def test_sample_constants_views_and_rank(rt):
     g.add_output(g.sample(xi, ui, temperature=g.add_constant("t", 0.0)))
     assert torch.equal(compiled(rt, g, "bfloat16")(x, u).long().view(12),
                        torch.from_numpy(sample_reference(x.reshape(12, 501), u.view(12), 0.0)[0]).to(DEV))
+
+
+@pytest.mark.parametrize("vocab", [1, 3, 700, 3000])
+def test_sample_ranks_without_tokens(vocab):
+    """Clusters of 8 CTAs, most of which hold no token and reach the first
+    exchange at once; many more rows than run at a time."""
+    rows = 3000
+    ck = compiled(MoltenRuntime(tune={"sample": {"ranks": 8}}), graphs.sample(2, 64, top_k=True, top_p=0.9), "float32")
+    x, u = sample_inputs(rows, vocab, "float32", seed=vocab)
+    t = torch.ones(rows, device=DEV)
+    k = torch.full((rows,), 40, dtype=torch.int32, device=DEV)
+    tokens = ck(x, u, t, k)
+    assert ck.specialization(x, u, t, k).plan.kernels[0].config["ranks"] == 8
+    check_sample(tokens[:200], x[:200], u[:200], top_k=k, top_p=0.9)
+    for _ in range(20):
+        assert torch.equal(ck(x, u, t, k), tokens)
