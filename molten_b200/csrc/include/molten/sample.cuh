@@ -274,7 +274,7 @@ struct Sampler {
   double c;                        // weights: 2^((x - m) c / 256)
   float sure;                      // top_p keeps all above this one (no top_k)
 
-  // 2^(t / 256), -256000 <= t <= 0
+  // 2^(t / 256), -256000 <= t <= 0 (the cut's is at least -254900)
   __device__ __forceinline__ double power(double t) const {
     const double big = t + 6755399441055744.0;       // 1.5 2^52: round(t) in the low bits
     const int k = __double2loint(big);
@@ -758,7 +758,9 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
     return;
   }
   k.c = 256.0 * 1.4426950408889634074 / (double)temperature;
-  k.cut = fmaxf((float)((double)k.m - 690.0 * (double)temperature), -3.402823466e38f);   // e^-690 = 2^-995
+  // e^-690 = 2^-995.  Rounded up: rounded down it can lie a whole step of m below
+  // for 690 T of half a step, and the exponent of a weight at it leaves its field
+  k.cut = fmaxf(__double2float_ru((double)k.m - 690.0 * (double)temperature), -3.402823466e38f);
 
   // `from`: what the filters keep is not below it
   float from = -INFINITY, lo = -range.y;
@@ -854,7 +856,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
     tail = 0.0;
   }
   const int at = sample_draw<T, THREADS>(k, per, lo, many, tail, u, top_k, top_p, min_p);
-  if (at < 0) return;
+  if (at < 0) return;                                // (one thread has it: the largest token weighs 1 and is kept)
   int token = base + at;
   if (packed) {
     int r = rank;

@@ -686,3 +686,31 @@ def test_sample_ranks_without_tokens(vocab):
     check_sample(tokens[:200], x[:200], u[:200], top_k=k, top_p=0.9)
     for _ in range(20):
         assert torch.equal(ck(x, u, t, k), tokens)
+
+
+@pytest.mark.parametrize("top", [10.0, -10.0, 1000.0])
+@pytest.mark.parametrize("use", ["", "k", "p", "m"])
+def test_sample_temperatures_below_the_spacing_of_logits(rt, top, use):
+    """The largest fp32 logit twice behind one 1 to 20 steps below it, with
+    temperatures from a thousandth of a step to some 30 of them: the lower one
+    weighs something, nothing, or less than any number."""
+    vocab, steps = 20000, 20
+    spacing = float(np.spacing(np.float32(top)))
+    ts = spacing * 2.0 ** torch.linspace(-11, 5, 48, device=DEV)
+    rows = steps * ts.numel()
+    x = top - 100 - 5 * torch.rand(rows, vocab, generator=gen_of(21), device=DEV)
+    at = torch.randint(1, vocab - 1, (rows,), generator=gen_of(22), device=DEV)
+    ups = torch.arange(1, steps + 1, device=DEV).repeat_interleave(ts.numel())
+    row = torch.arange(rows, device=DEV)
+    x[row, at - 1] = (top - ups.double() * spacing).float()            # (exact)
+    x[row, at], x[row, at + 1] = top, top
+    u = torch.rand(rows, generator=gen_of(23), device=DEV)
+    params = {"temperature": ts.repeat(steps)}
+    if use == "k":
+        params["top_k"] = torch.full((rows,), 4, dtype=torch.int32, device=DEV)
+    elif use:
+        params["top_p" if use == "p" else "min_p"] = torch.full((rows,), 0.97 if use == "p" else 1e-3, device=DEV)
+    ck = compiled(rt, graphs.sample(rows, vocab, top_k=use == "k", top_p=use == "p", min_p=use == "m"), "float32")
+    out = torch.full((rows,), -7, dtype=torch.int32, device=DEV)
+    ck(x, u, *params.values(), out=out)
+    check_sample(out, x, u, **params)
