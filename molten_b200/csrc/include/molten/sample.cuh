@@ -350,7 +350,9 @@ struct Sampler {
     // one.  Bounds in fp32: 0.01 bins cover the rounding of the bin's number,
     // 3e-5 that of exponents (up to 58, a few 2^-24 of that), of ex2.approx
     // (2^-22) and of the sums
-    const float width = 2.0f / bins.inv, c1 = (float)c * (1.0f / 256.0f), gap = bins.hi - m;
+    // (half differences, as in SampleBins: two finite values may lie further apart
+    // than the largest one)
+    const float width = 1.0f / bins.inv, c1 = (float)c * (1.0f / 128.0f), gap = 0.5f * bins.hi - 0.5f * m;
     float most[PER], least[PER];
     SampleSums own = {0.0, 0.0f, 0.0f};              // tokens, the most and the least weight
 #pragma unroll
@@ -360,7 +362,7 @@ struct Sampler {
       if (by_weight) {
         const float high = fminf(0.0f, gap - ((float)b - 0.51f) * width);
         // (the last bin also holds everything down to lo)
-        const float low = b == BINS - 1 ? lo - m : gap - ((float)b + 0.51f) * width;
+        const float low = b == BINS - 1 ? 0.5f * lo - 0.5f * m : gap - ((float)b + 0.51f) * width;
         own.y += (float)cs[q] * fast_exp2(high * c1);
         own.z += (float)cs[q] * fast_exp2(low * c1);
       }
@@ -783,7 +785,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
       const float depth = ((float)b1 + 0.6f) * 2.0f / bins.inv;
       if (by_weight && b0 > 0) {
         const float height = ((float)b0 - 0.6f) * 2.0f / bins.inv;
-        k.sure = (k.m - height) + 4e-7f * (fabsf(k.m) + height);
+        k.sure = (k.m - height) + 4e-7f * (fabsf(k.m) + height);         // (NaN past the range: no help)
       }
       if (b1 < SAMPLE_BINS - 1) from = fmaxf(lo, (k.m - depth) - 4e-7f * (fabsf(k.m) + depth));
     }
@@ -799,14 +801,15 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
     // the tokens from there up; the weight of the rest, in fp32
     int hits = 0;
     float rest = 0.0f;
-    // (two floats: an error of the factor would be the same in every term)
-    const float c1 = (float)(k.c / 256.0), c1_low = (float)(k.c / 256.0 - (double)c1);
+    // (two floats: an error of the factor would be the same in every term; half
+    // differences down to the cut, so that both products are finite)
+    const float c1 = (float)(k.c / 128.0), c1_low = (float)(k.c / 128.0 - (double)c1);
     if (by_weight && top_p < 1.0f)
       sm_each(mine, a.run, [&](int, float x) {
         hits += x >= from ? 1 : 0;
-        const float d = x - k.m;
-        const float e = fast_exp2(fmaf(d, c1, d * c1_low));              // (NaN of -inf)
-        rest += x < from && x >= -3.402823466e38f ? e : 0.0f;
+        const float d = 0.5f * fmaxf(x, k.cut) - 0.5f * k.m;
+        const float e = fast_exp2(fmaf(d, c1, d * c1_low));
+        rest += x < from && x >= k.cut ? e : 0.0f;
       });
     else
       sm_each(mine, a.run, [&](int, float x) { hits += x >= from ? 1 : 0; });

@@ -714,3 +714,25 @@ def test_sample_temperatures_below_the_spacing_of_logits(rt, top, use):
     out = torch.full((rows,), -7, dtype=torch.int32, device=DEV)
     ck(x, u, *params.values(), out=out)
     check_sample(out, x, u, **params)
+
+
+@pytest.mark.parametrize("kind", ["infinite", "cold", "hot"])
+def test_sample_masks_of_the_lowest_value(rt, kind):
+    """Masks of the type's lowest value beside +inf (the largest value), under
+    very low and under infinite temperatures: differences of two logits pass
+    the type's range."""
+    rows, vocab = 16, 3001
+    x, u = sample_inputs(rows, vocab, "float32", seed=31)
+    x[:, 5::3] = torch.finfo(torch.float32).min
+    t = 0.4 + torch.rand(rows, generator=gen_of(32), device=DEV)
+    if kind == "cold":
+        x[:, 7::500] = 9.0                             # (six of them)
+        t = 10.0 ** torch.linspace(-9, -28, rows, device=DEV)
+    else:
+        x[:, 7::500] = torch.inf
+    if kind == "hot":
+        t = torch.full_like(t, torch.inf)
+        t[::2] = 10.0 ** torch.linspace(36, 38.4, rows // 2, device=DEV)
+    for top_p in (0.55, 0.85):
+        tokens = compiled(rt, graphs.sample(rows, vocab, top_p=top_p), "float32")(x, u, t)
+        check_sample(tokens, x, u, temperature=t.double().clamp(max=1e300), top_p=top_p)
