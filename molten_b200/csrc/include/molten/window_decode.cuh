@@ -30,7 +30,9 @@
 // whatever a cache holds behind its last token or outside the window never
 // meets an MMA.  A key that only some queries see takes part with P = 0; if
 // its value holds an infinity or NaN (0 times that is NaN) the tile's P V is
-// done row by row instead.
+// done row by row instead.  A warp whose sums end with an infinity or NaN takes
+// its tiles once more, all of them row by row: the two parts of P times an
+// infinity can be infinities of both signs.
 //
 // Measured: 64 requests over caches of up to 8192, 32 heads over 8, head dim
 // 128, window 4096: 154 us, 7.0 TB/s of the keys and values that are seen; 1
@@ -260,10 +262,12 @@ __device__ __forceinline__ void window_decode(const WindowArgs& a, uint8_t* raw)
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  float o[NB][NK][4], mx[NB][2], sum[NB][2];         // O^T: dims 16 i + g, + 8; rows 2 t, 2 t + 1
+  // a second turn, with every tile done row by row, where the first left a NaN
+#pragma unroll 1
+  for (int turn = 0; turn < 2; ++turn) {
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) copy_tile(t0 + warp + s * WARPS, s);
-
-  float o[NB][NK][4], mx[NB][2], sum[NB][2];         // O^T: dims 16 i + g, + 8; rows 2 t, 2 t + 1
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
 #pragma unroll
@@ -352,8 +356,8 @@ __device__ __forceinline__ void window_decode(const WindowArgs& a, uint8_t* raw)
         }
     }
 
-    bool odd = false;                                // an infinity or NaN that P = 0 would meet
-    if (a.nq > 1 && !whole) {
+    bool odd = turn > 0;                             // an infinity or NaN that P = 0 would meet
+    if (a.nq > 1 && !whole && !odd) {
 #pragma unroll 1
       for (int i = lane; i < L::KV_BYTES / 4; i += 32) {
         const float2 f = wd_unpack<T>(*reinterpret_cast<const uint32_t*>(vt + 4 * i));
@@ -403,6 +407,19 @@ __device__ __forceinline__ void window_decode(const WindowArgs& a, uint8_t* raw)
     }
     __syncwarp();                                    // the stage is free for the next copy
     if (++stage == STAGES) stage = 0;
+  }
+  // 0 x sums up to NaN from an infinity or NaN on: P's two parts times an
+  // infinity may be infinities of both signs
+  float odds[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int i = 0; i < NK; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odds[e] = fmaf(o[n][i][e], 0.0f, odds[e]);
+  odds[0] = (odds[0] + odds[1]) + (odds[2] + odds[3]);
+  if (!__any_sync(0xffffffffu, odds[0] != odds[0])) break;
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();                                   // every ring is idle: the merge area

@@ -736,3 +736,34 @@ def test_sample_masks_of_the_lowest_value(rt, kind):
     for top_p in (0.55, 0.85):
         tokens = compiled(rt, graphs.sample(rows, vocab, top_p=top_p), "float32")(x, u, t)
         check_sample(tokens, x, u, temperature=t.double().clamp(max=1e300), top_p=top_p)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("new,cache,ranks,parts", [(1, 40, 1, 1), (1, 700, 8, 1), (1, 700, 2, 3), (4, 700, 1, 1),
+                                                   (4, 700, 8, 2)])
+def test_window_attention_few_rows_keeps_infinities(new, cache, ranks, parts, dtype):
+    """An infinity in a value that a query sees is that infinity in its output;
+    both of them, or a NaN, are NaN."""
+    b, heads, kv, d, window, sinks = 2, 8, 2, 64, 300, 4
+    rt = MoltenRuntime(tune={"window": {"ranks": ranks, "parts": parts}})
+    ck = window_kernel(rt, 1, 1, 16, heads, kv, d, window, sinks, dtype)
+    q, k, v = attention_inputs(b, new, cache, heads, kv, d, dtype, seed=3)
+    lengths = torch.tensor([cache, cache - 9], dtype=torch.int32, device=DEV)
+    clean = ck(q, k, v, lengths)
+    n, per = cache - new - 2, heads // kv              # (a key that every query of request 0 sees)
+    v[0, n, 0, 1], v[0, 2, 0, 2] = torch.inf, -torch.inf
+    v[0, n, 0, 3], v[0, n - 1, 0, 3] = torch.inf, -torch.inf
+    v[0, n, 0, 4] = torch.nan
+    out = ck(q, k, v, lengths)
+    assert bool((out[0, :, :per, 1] == torch.inf).all()) and bool((out[0, :, :per, 2] == -torch.inf).all())
+    assert bool(torch.isnan(out[0, :, :per, 3:5]).all())
+    keep = torch.ones_like(out, dtype=torch.bool)
+    keep[0, :, :per, 1:5] = False
+    assert bool(torch.isfinite(out[keep]).all())
+    v[0, n - 1:n + 1, 0, 1:5], v[0, 2, 0, 2] = 0.0, 0.0
+    ref, mag, big = attention_reference(q, k, v, lengths, window, sinks)
+    # (check_attention's tolerance)
+    tol = half_step(dtype) * ref.abs() + (2.0 ** -16 + 2.0 ** -19 + 2.0 ** -21 * (1 + big)) * mag + (
+        2.0 ** -24 if dtype == "float16" else 0.0)
+    assert bool(((out.double() - ref).abs() <= tol)[keep].all())
+    assert torch.equal(out[1], clean[1])
