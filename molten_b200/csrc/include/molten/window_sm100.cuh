@@ -731,34 +731,46 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
       OT* dst = static_cast<OT*>(args.out) +
                 (((long long)w.b * args.nq + i) * args.kv_heads * args.per + w.h * args.per + r % args.per) *
                     (long long)args.dim;
-      // whole sectors where rows start on one (each lane writes its own row)
+      // 16 columns at a time, whole sectors where rows start on one (each lane
+      // writes its own row)
+      constexpr int WORDS = 4 * (int)sizeof(OT);     // of 16 values
       const bool wide = args.dim % 16 == 0 && (reinterpret_cast<uintptr_t>(args.out) & 31u) == 0u;
 #pragma unroll 1
       for (int c = 0; c < L::DP; c += 32) {
         float o[32];
         if (run) tmem_ld32(o_at + c, o);             // (the whole warp)
         if (c >= args.dim) continue;
-        uint32_t y[16];
+        uint32_t y[2 * WORDS];
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-          Slot<OT, 2> two;
           const float f[2] = {sum == 0.0f ? 0.0f : o[2 * q] * inv, sum == 0.0f ? 0.0f : o[2 * q + 1] * inv};
-          pack_slot<OT, 2>(two, f);
-          y[q] = *reinterpret_cast<const uint32_t*>(&two);
+          if constexpr (sizeof(OT) == 4) {
+            y[2 * q] = __float_as_uint(f[0]);
+            y[2 * q + 1] = __float_as_uint(f[1]);
+          } else {
+            Slot<OT, 2> two;
+            pack_slot<OT, 2>(two, f);
+            y[q] = *reinterpret_cast<const uint32_t*>(&two);
+          }
         }
         if (!real) continue;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           if (c + 16 * q >= args.dim) break;
           uint32_t* at = reinterpret_cast<uint32_t*>(dst + c + 16 * q);
-          const uint32_t* v = y + 8 * q;
+          const uint32_t* v = y + WORDS * q;
           if (wide) {
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                         :: "l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
-                            "r"(v[7]) : "memory");
+#pragma unroll
+            for (int k = 0; k < WORDS; k += 8)
+              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                           :: "l"(at + k), "r"(v[k]), "r"(v[k + 1]), "r"(v[k + 2]), "r"(v[k + 3]), "r"(v[k + 4]),
+                              "r"(v[k + 5]), "r"(v[k + 6]), "r"(v[k + 7]) : "memory");
           } else {
-            *reinterpret_cast<uint4*>(at) = make_uint4(v[0], v[1], v[2], v[3]);
-            if (c + 16 * q + 8 < args.dim) *reinterpret_cast<uint4*>(at + 4) = make_uint4(v[4], v[5], v[6], v[7]);
+            // (dim is a multiple of 8 columns)
+            const int words = c + 16 * q + 8 < args.dim ? WORDS : WORDS / 2;
+#pragma unroll
+            for (int k = 0; k < WORDS; k += 4)
+              if (k < words) *reinterpret_cast<uint4*>(at + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
           }
         }
       }

@@ -767,3 +767,40 @@ def test_window_attention_few_rows_keeps_infinities(new, cache, ranks, parts, dt
         2.0 ** -24 if dtype == "float16" else 0.0)
     assert bool(((out.double() - ref).abs() <= tol)[keep].all())
     assert torch.equal(out[1], clean[1])
+
+
+@pytest.mark.parametrize("new,cache,d,parts", [(1, 300, 64, None), (3, 300, 128, None), (100, 300, 64, None),
+                                               (90, 700, 80, 1), (90, 700, 24, 1), (300, 900, 128, 3)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_window_attention_in_a_group(new, cache, d, parts, dtype):
+    """Attention -> + residual -> SiLU as one graph: the attention is kept in
+    32 bits between them."""
+    b, heads, kv, window, sinks = 2, 6, 2, 150, 3
+    g = DataflowGraph("attention_residual")
+    ids = [g.add_input("q", TS([b, new, heads, d])), g.add_input("k", TS([b, cache, kv, d])),
+           g.add_input("v", TS([b, cache, kv, d])), g.add_input("n", TS([b]), dtype="int32")]
+    r = g.add_input("r", TS([b, new, heads, d]))
+    g.add_output(g.silu(g.add(g.window_attention(*ids[:3], lengths=ids[3], window=window, sinks=sinks), r)))
+    ck = MoltenRuntime(tune={"window": {"parts": parts}} if parts else {}).compile(compile_graph(g, dtype=dtype)[0])
+    # (another batch than the declared one: planned with the given parts)
+    q, kk, v = attention_inputs(b + 1, new, cache, heads, kv, d, dtype, seed=d)
+    res = torch.randn(b + 1, new, heads, d, generator=gen_of(41), device=DEV).to(DT[dtype])
+    lengths = torch.tensor([cache, new + 7, 0], dtype=torch.int32, device=DEV)
+    v[0, cache - 1, 0, 3] = torch.inf                  # (the last query's alone)
+    out = ck(q, kk, v, lengths, res)
+    plan = ck.specialization(q, kk, v, lengths, res).plan
+    assert [sk.outputs[0].dtype for sk in plan.kernels] == ["float32", dtype]
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[0, -1, :heads // kv, 3] = True
+    assert bool((out[bad] == torch.inf).all())
+    v[0, cache - 1, 0, 3] = 0.0
+    ref, mag, big = attention_reference(q, kk, v, lengths, window, sinks)
+    y = ref + res.double()
+    # P's rounding, scores and exponentials as in check_attention, the sum in
+    # fp32, SiLU's slope of at most 1.1 and one output rounding
+    p_half = half_step(dtype) if plan.kernels[0].config["kind"] == "tiles" else 2.0 ** -16
+    want = torch.nn.functional.silu(y)
+    tol = (half_step(dtype) + 2.0 ** -20) * want.abs() + 1.1 * (
+        (p_half + 2.0 ** -19 + 2.0 ** -21 * (1 + big)) * mag + 2.0 ** -23 * y.abs() + 2.0 ** -24)
+    err = (out.double() - want).abs()
+    assert bool((err <= tol)[~bad].all()), err[~bad].max().item()
