@@ -366,19 +366,42 @@ def launch_model_op(spec, i: int, env: dict, device: int, stream: int) -> None:
     b.run(b.conform(ins), env[b.sk.outputs[0].op_id], stream)
 
 
-def refuse_overlap(sk, tensors, out) -> None:
-    """An output may not lie in memory that other blocks of the same kernel
-    still read.  (RoPE turns pairs where they are: its x may be its output.)"""
-    start, end = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
-    for n, t in enumerate(tensors):
-        if t.numel() == 0 or not out.numel():
-            continue
-        span = 1 + sum((d - 1) * s for d, s in zip(t.shape, t.stride()))
-        if t.data_ptr() < end and start < t.data_ptr() + span * t.element_size():
-            if (sk.config["op"] == ModelOpType.ROTATE_POSITIONS and n == 0 and t.data_ptr() == start
-                    and t.is_contiguous() and t.dtype == out.dtype):
+def _extent(t):
+    """(first byte, byte behind the last) of a tensor's memory."""
+    if t.numel() == 0:
+        return 0, 0
+    span = 1 + sum((d - 1) * s for d, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + span * t.element_size()
+
+
+def refuse_overlap(plan, tensors, outs) -> None:
+    """In a plan with a model operator, an output may not lie in memory that
+    other blocks of its kernel, or a kernel after it, still read, nor in
+    another output's.  (RoPE turns pairs where they are: its x may be its
+    output.  Kernels of the other families are left to the caller.)"""
+    if not any(sk.family == "model" for sk in plan.kernels):
+        return
+    env = dict(zip(plan.inputs, tensors))
+    env.update(zip(plan.outputs, outs))
+    extents = {i: _extent(t) for i, t in env.items()}
+
+    def overlap(a, b):
+        return extents[a][0] < extents[b][1] and extents[b][0] < extents[a][1]
+    for n, o in enumerate(plan.outputs):
+        if any(overlap(o, other) for other in plan.outputs[:n]):
+            raise RuntimeError(f"{plan.name}: two outputs overlap")
+        i = next(i for i, sk in enumerate(plan.kernels) if any(w.op_id == o for w in sk.outputs))
+        for j, sk in enumerate(plan.kernels[i:], i):
+            if "model" not in (sk.family, plan.kernels[i].family):
                 continue
-            raise RuntimeError(f"{sk.config['op'].name}: the output overlaps an input")
+            for operand in sk.operands:
+                t = env.get(operand.op_id)
+                if t is None or operand.op_id == o or not overlap(o, operand.op_id):
+                    continue
+                if (j == i and sk.config["op"] == ModelOpType.ROTATE_POSITIONS and operand.index == 0
+                        and t.data_ptr() == env[o].data_ptr() and t.is_contiguous() and t.dtype == env[o].dtype):
+                    continue
+                raise RuntimeError(f"{plan.name}: an output overlaps the input {operand.name!r}")
 
 
 class ModelCall:

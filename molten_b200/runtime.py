@@ -86,6 +86,7 @@ class _Spec:
         self._tmaps: OrderedDict = OrderedDict()
         self.align = [_alignment_rules(sk) for sk in self.plan.kernels]
         self.single = ModelCall.fits(self)
+        self.model = any(sk.family == "model" for sk in self.plan.kernels)
 
     def module(self, device: int) -> _capi.Module:
         m = self.modules.get(device)
@@ -494,8 +495,8 @@ class CompiledKernel:
         if out is not None:
             outs = list(out) if isinstance(out, (list, tuple)) else [out]
             self._check_outs(spec, outs, dev)
-            if spec.single:
-                refuse_overlap(spec.plan.kernels[0], prepared, outs[0])
+            if spec.model:
+                refuse_overlap(spec.plan, prepared, outs)
         else:
             outs = None
         res = spec.run(prepared, outs, stream, row_offset)

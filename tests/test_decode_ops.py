@@ -449,3 +449,77 @@ def test_clusters_have_started_before_their_memory_is_used(header, entry, first)
     assert "barrier.cluster.wait" in before or "q4_cluster_sync()" in before
     if "barrier.cluster.wait" in before:
         assert before.index("barrier.cluster.arrive") < before.index("barrier.cluster.wait")
+
+
+# ------------------------------------------------ outputs in the inputs' memory
+def check_overlap(g, dtype, tensors, outs):
+    """What the runtime asks before a call writes to given outputs."""
+    from molten_b200.decode_launch import refuse_overlap
+    (k,) = compile_graph(g, dtype=dtype)
+    names = [g.ops[i].name for i in k.plan.inputs]
+    refuse_overlap(k.plan, [tensors[n] for n in names], outs)
+
+
+@pytest.mark.parametrize("order", ["xcsp", "pcsx", "csxp", "cxsp"])
+def test_rope_in_place_whatever_the_inputs_order(order):
+    import torch
+    shapes = {"x": [2, 5, 2, 64], "c": [40, 32], "s": [40, 32], "p": [1, 2, 5]}
+    dtypes = {"x": "float32", "c": "float32", "s": "float32", "p": "int32"}
+    g = wired(order, lambda g, i: g.rope(i["x"], i["c"], sin=i["s"], positions=i["p"]), shapes, dtypes)
+    t = {n: torch.zeros(s, dtype=getattr(torch, dtypes[n])) for n, s in shapes.items()}
+    check_overlap(g, "float32", t, [t["x"]])
+    check_overlap(g, "float32", t, [torch.zeros_like(t["x"])])
+    # over a table, from its start and from inside it
+    for n in "cs":
+        for at in (0, 8):
+            t[n] = torch.zeros(2000)[at:at + 1280].view(40, 32)
+            over = t[n].flatten().as_strided([2, 5, 2, 64], [640, 128, 64, 1])
+            with pytest.raises(RuntimeError, match="overlaps"):
+                check_overlap(g, "float32", t, [over])
+    wide = torch.zeros(1288)
+    t["x"] = wide[:1280].view(2, 5, 2, 64)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        check_overlap(g, "float32", t, [wide[8:].view(2, 5, 2, 64)])
+
+
+def test_overlaps_in_plans_of_several_kernels():
+    import torch
+    g = DataflowGraph("two")
+    ids = {n: g.add_input(n, TS([1, 4, 2, 64]), dtype="bfloat16") for n in "rqkv"}
+    q = g.add(ids["q"], ids["r"])
+    g.add_output(q)
+    g.add_output(g.window_attention(q, ids["k"], ids["v"]))
+    t = {n: torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16) for n in "rqkv"}
+    new = [torch.zeros_like(t["q"]) for _ in range(2)]
+    check_overlap(g, "bfloat16", t, new)
+    for n in "rq":                                     # (read before the attention writes, by nothing after)
+        check_overlap(g, "bfloat16", t, [new[0], t[n]])
+        check_overlap(g, "bfloat16", t, [t[n], new[1]])          # elementwise in place, as ever
+    for n in "kv":
+        for outs in ([new[0], t[n]], [t[n], new[1]], [new[0], t[n].flatten()[128:].as_strided([1, 4, 2, 64], [0, 96, 0, 1])]):
+            with pytest.raises(RuntimeError, match="overlap"):
+                check_overlap(g, "bfloat16", t, outs)
+    with pytest.raises(RuntimeError, match="overlap"):
+        check_overlap(g, "bfloat16", t, [new[0], new[0]])
+
+    # x turned in place is read again by a later kernel
+    g = DataflowGraph("turned")
+    x = g.add_input("x", TS([1, 3, 2, 64]), dtype="float32")
+    c = g.add_input("c", TS([9, 64]), dtype="float32")
+    p = g.add_input("p", TS([1, 1, 3]), dtype="int32")
+    y = g.rope(x, c, positions=p)
+    g.add_output(y)
+    g.add_output(g.add(y, x))
+    t = {"x": torch.zeros(1, 3, 2, 64), "c": torch.zeros(9, 64), "p": torch.zeros(1, 1, 3, dtype=torch.int32)}
+    with pytest.raises(RuntimeError, match="overlap"):
+        check_overlap(g, "float32", t, [t["x"], torch.zeros_like(t["x"])])
+    check_overlap(g, "float32", t, [torch.zeros_like(t["x"]), t["x"]])
+
+
+def test_overlap_is_left_to_plans_without_model_operators():
+    import torch
+    g = DataflowGraph("plain")
+    x = g.add_input("x", TS([4, 64]), dtype="float32")
+    g.add_output(g.silu(x))
+    t = torch.zeros(4, 64)
+    check_overlap(g, "float32", {"x": t}, [t])

@@ -804,3 +804,29 @@ def test_window_attention_in_a_group(new, cache, d, parts, dtype):
         (p_half + 2.0 ** -19 + 2.0 ** -21 * (1 + big)) * mag + 2.0 ** -23 * y.abs() + 2.0 ** -24)
     err = (out.double() - want).abs()
     assert bool((err <= tol)[~bad].all()), err[~bad].max().item()
+
+
+@pytest.mark.parametrize("order", ["pcsx", "cxsp"])
+@pytest.mark.parametrize("shape,style,dtype", [((3, 700, 22, 128), "half", "bfloat16"), ((1, 9, 3, 6), "interleaved", "float32")])
+def test_rope_in_place_with_x_anywhere(rt, order, shape, style, dtype):
+    b, s, h, d = shape
+    g = DataflowGraph("turned")
+    ids = {}
+    for n in order:
+        dims = {"x": shape, "c": (50, d // 2), "s": (50, d // 2), "p": (1, b, s)}[n]
+        ids[n] = g.add_input(n, TS(list(dims)), dtype={"x": dtype, "p": "int32"}.get(n, "float32"))
+    g.add_output(g.rope(ids["x"], ids["c"], sin=ids["s"], positions=ids["p"], style=style))
+    ck = compiled(rt, g, dtype)
+    cos, sin = tables(50, d // 2)
+    x = torch.randn(*shape, generator=gen_of(1), device=DEV).to(DT[dtype])
+    pos = torch.randint(-1, 50, (1, b, s), generator=gen_of(2), device=DEV, dtype=torch.int32)
+    t = {"x": x, "c": cos, "s": sin, "p": pos}
+    want = ck(*[t[n] for n in order])
+    check_rope(want, x, cos, sin, pos, [d // 2], style, dtype)
+    y = x.clone()
+    ck(*[dict(t, x=y)[n] for n in order], out=y)
+    assert torch.equal(y, want)
+    over = torch.zeros(max(x.numel(), cos.numel()), device=DEV, dtype=torch.float32)
+    wide = dict(t, c=over[:cos.numel()].view(cos.shape))
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ck(*[wide[n] for n in order], out=over.view(DT[dtype])[:x.numel()].view(shape))
