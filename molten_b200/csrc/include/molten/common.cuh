@@ -50,7 +50,8 @@ struct alignas((sizeof(T) * VEC) >= 16 ? 16 : (sizeof(T) * VEC)) Slot {
   T v[VEC];
 };
 
-enum LoadHint { kLoadDefault = 0, kLoadStream = 1 };
+// (kLoadInPlace: memory that the same kernel may write to, so not through .nc)
+enum LoadHint { kLoadDefault = 0, kLoadStream = 1, kLoadInPlace = 2 };
 enum StoreHint { kStoreDefault = 0, kStoreStream = 1 };
 
 template <int HINT>
@@ -59,6 +60,9 @@ __device__ __forceinline__ uint4 ld16(const void* p) {
   if (HINT == kLoadStream) {
     asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  } else if (HINT == kLoadInPlace) {
+    asm volatile("ld.global.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
   } else {
     asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
@@ -85,6 +89,14 @@ __device__ __forceinline__ Slot<T, VEC> load_slot(const T* p) {
 #pragma unroll
     for (int i = 0; i < BYTES / 16; ++i)
       reinterpret_cast<uint4*>(&s)[i] = ld16<HINT>(reinterpret_cast<const char*>(p) + 16 * i);
+  } else if constexpr (HINT == kLoadInPlace) {
+    if constexpr (BYTES == 8)
+      asm volatile("ld.global.v2.u32 {%0,%1}, [%2];"
+                   : "=r"(reinterpret_cast<uint32_t*>(&s)[0]), "=r"(reinterpret_cast<uint32_t*>(&s)[1])
+                   : "l"(p) : "memory");
+    else
+      asm volatile("ld.global.u32 %0, [%1];" : "=r"(reinterpret_cast<uint32_t*>(&s)[0]) : "l"(p) : "memory");
+    static_assert(BYTES == 8 || BYTES == 4, "unsupported slot size");
   } else if constexpr (BYTES == 8) {
     *reinterpret_cast<uint2*>(&s) = __ldg(reinterpret_cast<const uint2*>(p));
   } else if constexpr (BYTES == 4) {

@@ -13,7 +13,8 @@
 // loads that slot's cos and sin once and turns up to HPT heads with it, all
 // their loads issued first: the table costs one read per HPT heads instead of
 // one per head (it is fp32 and as wide as x, so it would triple the L1
-// traffic).
+// traffic).  Every element is read and written by one thread, the reads first, so
+// out may be x: x is loaded as memory that changes.
 //
 // Measured, bf16 with fp32 tables: 4 x 4096 tokens of 32 heads of 128, one axis
 // 45.7 us (5.9 TB/s), three axes at random positions 50.4 (each section's table
@@ -114,10 +115,10 @@ __device__ __forceinline__ void rope_positions(const RopePosArgs& a) {
       for (int p = 0; p < PARTS; ++p) {
         const XT* src = x + h * a.x_head + p * (a.dim / 2);
         if constexpr (XVEC) {
-          s[u][p] = load_slot<kLoadStream, XT, VEC>(src);
+          s[u][p] = load_slot<kLoadInPlace, XT, VEC>(src);
         } else {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) s[u][p].v[e] = src[e];
+          for (int e = 0; e < VEC; ++e) s[u][p].v[e] = src[e];     // (out may be x: no .nc)
         }
       }
     }

@@ -523,3 +523,17 @@ def test_overlap_is_left_to_plans_without_model_operators():
     g.add_output(g.silu(x))
     t = torch.zeros(4, 64)
     check_overlap(g, "float32", {"x": t}, [t])
+
+
+def test_rope_reads_x_as_memory_that_it_may_write():
+    """.nc loads are for memory that nothing writes while the kernel runs, and
+    RoPE at positions may turn x in place."""
+    import re
+    from molten_b200.build import CSRC_DIR
+    inc = CSRC_DIR / "include" / "molten"
+    body = (inc / "rope_positions.cuh").read_text()
+    body = body[body.index("void rope_positions("):]
+    assert re.findall(r"load_slot<(\w+), XT", body) == ["kLoadInPlace"]
+    common = (inc / "common.cuh").read_text()
+    for part in common.split("== kLoadInPlace")[1:]:
+        assert ".nc" not in part[:part.index("} else")] and "__ldg" not in part[:part.index("} else")]
