@@ -116,7 +116,7 @@ struct WindowTcShared {
   uint32_t bars;
   uint32_t* tmem_slot;
   volatile int* abort_flag;
-  volatile int* dirty;             // [8] item number + 1 of an item with cleaned infinities or NaN
+  int* dirty;                      // [8] by item number: the latest item + 1 with cleaned infinities or NaN
 };
 
 template <class L>
@@ -128,7 +128,7 @@ __device__ __forceinline__ WindowTcShared window_tc_carve(uint8_t* raw) {
   s.bars = smem_u32(s.q + L::BAR_OFFSET);
   s.tmem_slot = reinterpret_cast<uint32_t*>(s.q + L::BAR_OFFSET + L::NUM_BARS * 8);
   s.abort_flag = reinterpret_cast<volatile int*>(s.tmem_slot + 1);
-  s.dirty = s.abort_flag + 1;
+  s.dirty = reinterpret_cast<int*>(s.tmem_slot + 2);
   return s;
 }
 
@@ -566,7 +566,9 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
             *chunk(q) = x;
           }
         }
-        if (found) s.dirty[seq & 7u] = (int)seq + 1;
+        // (numbers only grow: the cleaning warps may be any number of items ahead of
+        // the softmax, since items without key tiles take no stage of the ring)
+        if (found) atomicMax(&s.dirty[seq & 7u], (int)seq + 1);
         // the writes come before the tensor core's reads
         fence_async_shared();
         __threadfence_block();
@@ -702,7 +704,8 @@ __device__ __forceinline__ void window_tc_roles(const WindowTcShared& s, const W
         tc_fence_after();
       }
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const bool dirty = s.dirty[seq & 7u] == (int)seq + 1;
+      // (a later item's number says nothing of this one: it is looked through)
+      const bool dirty = *(volatile int*)&s.dirty[seq & 7u] > (int)seq;
       if constexpr (PARTS) {
         // this part's sums as they are, with their offset (+inf: no key seen)
         float* mine = args.part + ((long long)(it * 2 + t) * 128 + r) * (args.dim + 4);

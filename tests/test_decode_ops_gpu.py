@@ -830,3 +830,32 @@ def test_rope_in_place_with_x_anywhere(rt, order, shape, style, dtype):
     wide = dict(t, c=over[:cos.numel()].view(cos.shape))
     with pytest.raises(RuntimeError, match="overlaps"):
         ck(*[wide[n] for n in order], out=over.view(DT[dtype])[:x.numel()].view(shape))
+
+
+@pytest.mark.parametrize("gap", [1, 7, 8])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_window_attention_infinities_between_empty_requests(rt, gap, bad):
+    """Requests of one key tile with an infinity, and between those of one CTA
+    requests of length 0, which cost the warps that clean V nothing."""
+    sms, new, heads, d = 148, 40, 1, 64
+    turns = 3 * gap + 1
+    b = sms * turns
+    q, k, v = attention_inputs(b, new, new, heads, 1, d, "bfloat16", seed=5)
+    full = torch.arange(b, device=DEV) // sms % gap == 0
+    lengths = torch.where(full, new, 0).to(torch.int32)
+    ck = window_kernel(rt, b, new, new, heads, 1, d, None, 0, "bfloat16")
+    c = ck.kernel.plan.kernels[0].config
+    assert c["kind"] == "tiles" and c["parts"] == 1 and c["items"] == b
+    clean = ck(q, k, v, lengths)
+    check_attention(clean, q, k, v, lengths, None, 0, "bfloat16", half_step("bfloat16"))
+    at = 5 + torch.arange(b, device=DEV) % 30
+    v[torch.arange(b, device=DEV), at, 0, 9] = bad
+    for _ in range(5):
+        out = ck(q, k, v, lengths)
+        hit = full[:, None] & (torch.arange(new, device=DEV) >= at[:, None])
+        got = out[:, :, 0, 9].float()
+        assert bool((torch.isnan(got) if bad != bad else got == bad)[hit].all())
+        assert bool(torch.isfinite(got[~hit]).all())
+        others = torch.ones(d, dtype=torch.bool, device=DEV)
+        others[9] = False
+        assert torch.equal(out[..., others], clean[..., others])
