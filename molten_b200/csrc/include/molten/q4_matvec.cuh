@@ -30,7 +30,9 @@
 // inputs keep every bit down to 2^-29 of that value and lose at most 2^-40 of
 // it below; fp32 is split into three such planes (2^-33 of the largest value
 // is left out) and meets q - 8 as normal numbers (q4_pair).  The scale and
-// sum_{k in g} x, in fp32, stand beside it.
+// sum_{k in g} x, in fp32, stand beside it.  Infinities and NaN would meet their
+// own sum (inf - z inf) and numbers past 2^120 overflow it: a CTA that staged such
+// a number does the outputs of that row again at the end, from the definition.
 //
 // The warps of a CTA split k; their partial sums meet in shared memory in
 // warp order.  A CTA walks over row tiles with the next weights always in
@@ -142,10 +144,14 @@ struct Q4Smem {
   }
 };
 
+// An infinity, a NaN, or so large that the sum of a group could pass the range.
+__device__ __forceinline__ bool q4_wild(float x) { return !(fabsf(x) < 1.329227995784916e36f); }   // 2^120
+
 // Stage groups [g0, g0 + count) of every row of x: a group of a row to G/8
-// lanes, STEP groups' loads in flight at once.
+// lanes, STEP groups' loads in flight at once.  True: a group holds what q4_wild
+// says.
 template <typename XT, int G, int NT, int PLANES, int WARPS>
-__device__ __forceinline__ void q4_stage(const Q4Args& a, const Q4Smem<G, NT, PLANES, WARPS>& s,
+__device__ __forceinline__ bool q4_stage(const Q4Args& a, const Q4Smem<G, NT, PLANES, WARPS>& s,
                                          int g0, int count) {
   constexpr int W = G / 32, LANES = G / 8;
   constexpr int STEP = NT == 1 ? 2 : 4, UNITS = WARPS * 32 / LANES;
@@ -154,6 +160,7 @@ __device__ __forceinline__ void q4_stage(const Q4Args& a, const Q4Smem<G, NT, PL
   const int total = count * a.m;
   const XT* x = static_cast<const XT*>(a.x) + (long long)g0 * G + 8 * l;
   int row = unit / count, grp = unit - row * count;  // of the next load
+  bool wild = false;
 #pragma unroll 1
   for (int base = 0; base < total; base += UNITS * STEP) {   // (whole warps shuffle)
     Slot<XT, 8> v[STEP];
@@ -179,6 +186,7 @@ __device__ __forceinline__ void q4_stage(const Q4Args& a, const Q4Smem<G, NT, PL
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         sum += __shfl_xor_sync(0xffffffffu, sum, d);
       }
+      wild |= q4_wild(top) || sum != sum;            // (the maximum with NaN is the other)
       // up = 2^(14 - exponent of top), its bits made directly; e is kept where
       // up and its reciprocal are normal numbers
       int e = (int)(__float_as_uint(top) >> 23);
@@ -208,6 +216,45 @@ __device__ __forceinline__ void q4_stage(const Q4Args& a, const Q4Smem<G, NT, PL
           f[1] -= __low2float(h2); f[5] -= __high2float(h2);
           f[3] -= __low2float(h3); f[7] -= __high2float(h3);
         }
+      }
+    }
+  }
+  return wild;
+}
+
+// The rows of x that hold a wild number, with the rows of q of this team's
+// tiles, over all of k in 64 bits: a warp to an output.
+template <typename XT, typename ST, typename OT, int G, bool ZEROS, int WARPS>
+__device__ __noinline__ void q4_wild_rows(const Q4Args& a, int team) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const long long groups = a.k / G;
+#pragma unroll 1
+  for (int row = 0; row < a.m; ++row) {
+    const XT* x = static_cast<const XT*>(a.x) + row * a.x_stride;
+    bool wild = false;
+#pragma unroll 1
+    for (int k = lane; k < a.k; k += 32) wild |= q4_wild(to_f32(x[k]));
+    if (!__any_sync(0xffffffffu, wild)) continue;
+#pragma unroll 1
+    for (int tile = team; tile < a.tiles; tile += a.teams) {
+#pragma unroll 1
+      for (int i = warp; i < 16 << a.warps_n_log; i += WARPS) {
+        const long long n = ((long long)tile << a.warps_n_log) * 16 + i;
+        if (n >= a.n) break;
+        double y = 0.0;
+#pragma unroll 1
+        for (int b = lane; b < a.k / 2; b += 32) {   // a byte of q: two k of one group
+          const int two = a.q[n * (a.k / 2) + b];
+          const long long g = n * groups + 2 * b / G;
+          double z = 8.0;
+          if constexpr (ZEROS) z = (double)to_f32(static_cast<const ST*>(a.zeros)[g]);
+          const double s = (double)to_f32(static_cast<const ST*>(a.scales)[g]);
+          y += (double)to_f32(x[2 * b]) * ((double)(two & 15) - z) * s;
+          y += (double)to_f32(x[2 * b + 1]) * ((double)(two >> 4) - z) * s;
+        }
+#pragma unroll
+        for (int d = 16; d >= 1; d /= 2) y += __shfl_xor_sync(0xffffffffu, y, d);
+        if (lane == 0) static_cast<OT*>(a.out)[row * a.n + n] = from_f32<OT>((float)y);
       }
     }
   }
@@ -256,6 +303,7 @@ __device__ __forceinline__ void q4_matvec(const Q4Args& a, uint8_t* raw) {
   // the sum that this thread adds up at the end of a tile
   const int my_on = threadIdx.x / (16 * a.m), my_rest = threadIdx.x - my_on * (16 * a.m);
 
+  int wild = 0;                                      // (the same in every thread)
   for (int c0 = cta0; c0 < cta1; c0 += a.chunk) {
     const int count = min(a.chunk, cta1 - c0);
     // this warp's groups of the chunk, the same of every tile
@@ -300,8 +348,7 @@ __device__ __forceinline__ void q4_matvec(const Q4Args& a, uint8_t* raw) {
     for (int d = 0; d < DEPTH; ++d) fetch(d);        // weights fly while x is staged
 
     if (c0 != cta0) __syncthreads();                 // the last chunk's x has been used
-    q4_stage<XT, G, NT, PLANES, WARPS>(a, sm, c0, count);
-    __syncthreads();
+    wild |= __syncthreads_or(q4_stage<XT, G, NT, PLANES, WARPS>(a, sm, c0, count));
 
     const bool first = c0 == cta0, last = c0 + count == cta1 && ksplit == 1;
 #pragma unroll 1
@@ -454,6 +501,10 @@ __device__ __forceinline__ void q4_matvec(const Q4Args& a, uint8_t* raw) {
       }
     }
     q4_cluster_sync();                               // peers may still read this CTA's sums
+  }
+  if (wild) {
+    __syncthreads();                                 // (the cluster's CTAs have stored as well)
+    q4_wild_rows<XT, ST, OT, G, ZEROS, WARPS>(a, team);
   }
 }
 

@@ -859,3 +859,46 @@ def test_window_attention_infinities_between_empty_requests(rt, gap, bad):
         others = torch.ones(d, dtype=torch.bool, device=DEV)
         others[9] = False
         assert torch.equal(out[..., others], clean[..., others])
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("m,n,k,group,tune", [
+    (3, 80, 512, 64, {}), (9, 33, 4096, 128, {}), (20, 130, 1024, 32, {}), (5, 300, 8192, 128, {"ksplit": 8}),
+    (32, 700, 14336, 32, {})])
+def test_matvec_q4_infinities_in_x(m, n, k, group, tune, zeros, dtype):
+    """An infinity in x makes every output of its row that infinity times the
+    weight's sign, NaN where the weight is 0 or where signs meet."""
+    x, q, s, z = q4_inputs(m, n, k, group, dtype, zeros, seed=11)
+    if zeros:
+        z = z.round()                                  # (weights of 0 among them)
+    ck = compiled(MoltenRuntime(tune={"q4": tune}), graphs.matvec_q4(1, 16, group, group, dtype=dtype, zeros=zeros),
+                  dtype)
+    x[0, 5] = torch.inf
+    x[1, k - 1] = -torch.inf
+    x[2, 3], x[2, group + 1] = torch.inf, torch.inf
+    rows = 3
+    if m > 4:
+        x[3, 7] = torch.nan
+        x[4, 0], x[4, 9] = torch.inf, -torch.inf
+        rows = 5
+    y = ck(x, q, s, *([z] if zeros else []))
+    w = (torch.stack((q & 15, q >> 4), -1).view(n, s.shape[1], -1).double()
+         - (z.double()[:, :, None] if zeros else 8.0)) * s.double()[:, :, None]
+    ref = torch.stack([(r.double() * w.view(n, k)).sum(1) for r in x[:rows]])
+    assert torch.equal(torch.isnan(y[:rows]), torch.isnan(ref))
+    signs = dict(nan=0.0, posinf=1.0, neginf=-1.0)
+    assert torch.equal(y[:rows].double().nan_to_num(**signs), ref.nan_to_num(**signs))
+    if m > rows:
+        check_q4(y[rows:], x[rows:], q, s, z, dtype)
+
+
+def test_matvec_q4_sums_past_the_range(rt):
+    """Rows near the largest fp32 value, whose sums pass it, with weights that
+    keep the product within it."""
+    m, n, k, group = 4, 48, 512, 64
+    _, q, s, z = q4_inputs(m, n, k, group, "float32", True, seed=13)
+    x = 3e38 * (0.5 + 0.5 * torch.rand(m, k, generator=gen_of(14), device=DEV))
+    s = s * 1e-6
+    y = compiled(rt, graphs.matvec_q4(m, n, k, group, dtype="float32", zeros=True), "float32")(x, q, s, z)
+    check_q4(y, x, q, s, z, "float32")
