@@ -278,12 +278,7 @@ class _Spec:
         env.update(zip(plan.outputs, outs))
         if all(o.numel() == 0 for o in outs):
             return outs                      # empty outputs (no rows or no columns): no launch
-        if stream != torch._C._cuda_getCurrentRawStream(di):
-            # a stream other than the caller's current one: intermediates and
-            # workspaces belong to it, or they would be reused while it runs
-            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=dev)):
-                self._launch(env, dev, di, stream, row_offset)
-        elif torch.cuda.current_device() != di:
+        if torch.cuda.current_device() != di:
             with torch.cuda.device(di):         # the launches make di current
                 self._launch(env, dev, di, stream, row_offset)
         else:
@@ -490,19 +485,33 @@ class CompiledKernel:
             if t.device != dev:
                 raise RuntimeError(f"{self.name}: all inputs must be on {dev}, got {t.device}")
         spec = self._spec_for(prepared)
-        if not all(t.is_contiguous() for t in prepared):
-            prepared = self._conform(spec, prepared)
+        outs = None
         if out is not None:
             outs = list(out) if isinstance(out, (list, tuple)) else [out]
             self._check_outs(spec, outs, dev)
-            if spec.model:
-                refuse_overlap(spec.plan, prepared, outs)
+        torch = _torch()
+        current = torch._C._cuda_getCurrentRawStream(dev.index)
+        if stream is None or stream == current:
+            res = self._run(spec, prepared, outs, current, row_offset)
         else:
-            outs = None
-        res = spec.run(prepared, outs, stream, row_offset)
+            # copies, outputs and workspaces belong to the stream that the kernels
+            # run on; a new output stays until the caller's stream is done with it
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=dev)):
+                res = self._run(spec, prepared, outs, stream, row_offset)
+            if outs is None:
+                for t in res:
+                    t.record_stream(torch.cuda.current_stream(dev))
         if not DEBUG and spec.single:
             self._last = short_call(spec, tensors)
         return res[0] if len(res) == 1 else tuple(res)
+
+    def _run(self, spec: _Spec, tensors, outs, stream: int, row_offset: int):
+        """A call on ``stream``, which is the current one."""
+        if not all(t.is_contiguous() for t in tensors):
+            tensors = self._conform(spec, tensors)
+        if outs is not None and spec.model:
+            refuse_overlap(spec.plan, tensors, outs)
+        return spec.run(tensors, outs, stream, row_offset)
 
     # -- specialisation -------------------------------------------------
     @staticmethod

@@ -584,3 +584,52 @@ def test_many_tokens(rt):
     out = compiled(rt, graphs.rope_positions(1, seq, heads, d, table=100), "bfloat16")(x, cos, sin, pos)
     check_rope(out[:, -3:], x[:, -3:], cos, sin, pos[..., -3:], [d // 2], "half", "bfloat16")
     assert not out[:, :-3].any()
+
+
+# ------------------------------------------------------ calls on a named stream
+@pytest.mark.parametrize("call", CALLS)
+def test_strided_inputs_on_a_named_stream(rt, call):
+    """Copies of strided inputs are made on the stream of the call, which fills
+    them late; on the current one they would hold zeros."""
+    ck, ins = call(rt, 0)
+    want = ck(*ins).clone()
+    wide = [torch.zeros(t.shape + (2,), dtype=t.dtype, device=DEV) for t in ins]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        for w, t in zip(wide, ins):
+            w[..., 0].copy_(t)
+    got = ck(*(w[..., 0] for w in wide), stream=side.cuda_stream)
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_outputs_of_a_named_stream_take_no_memory_in_use(rt):
+    """Memory that was freed while the current stream still reads it is not an
+    output of another stream, and an output that the current stream reads is not
+    taken again by the other one."""
+    x, q, s, z = q4_inputs(32, 16384, 512, 64, "float32", True)
+    ck = compiled(rt, graphs.matvec_q4(32, 16384, 512, 64, zeros=True, dtype="float32"), "float32")
+    want = ck(x, q, s, z).clone()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        old = torch.full_like(want, 7.0)
+        torch.cuda._sleep(20_000_000)
+        kept = old + 1.0
+        del old
+        got = ck(x, q, s, z, stream=side.cuda_stream)
+        torch.cuda.synchronize()
+        assert bool((kept == 8.0).all()) and torch.equal(got, want)
+        del got, kept
+        got = ck(x, q, s, z, stream=side.cuda_stream)
+        side.synchronize()
+        torch.cuda._sleep(20_000_000)
+        kept = got + 1.0
+        del got
+        with torch.cuda.stream(side):
+            torch.full_like(want, 7.0)
+        torch.cuda.synchronize()
+        assert torch.equal(kept, want + 1.0)
+        del kept
