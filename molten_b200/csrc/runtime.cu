@@ -114,6 +114,14 @@ int need_driver() {
   return MOLTEN_OK;
 }
 
+// Calls that a stream's capture forbids this thread (loading a module, allocating
+// the status word), allowed while one of these lives: they touch no stream.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 // Make `device` current on this thread.  With init != 0 also make sure its
 // primary context exists (the runtime creates it lazily); launches pass 0 so
 // that nothing but the launch itself happens while a stream is captured.
@@ -150,6 +158,7 @@ int lookup(Module* m, const char* name, Kernel** out) {
   auto it = m->kernels.find(name);
   if (it == m->kernels.end()) {
     Kernel k;
+    RelaxedCapture relaxed;
     CUresult r = driver().module_get_function(&k.fn, m->mod, name);
     if (r != CUDA_SUCCESS)
       return fail(MOLTEN_ERR_NOT_FOUND, std::string("kernel '") + name + "' not in module");
@@ -207,6 +216,7 @@ int molten_module_load_data(const void* image, size_t nbytes, int device, void**
   *mod = nullptr;
   int rc = need_driver();
   if (rc) return rc;
+  RelaxedCapture relaxed;
   rc = use_device(device);
   if (rc) return rc;
   Module* m = new Module();
@@ -270,6 +280,7 @@ int molten_kernel_info(void* mod, const char* kernel, int* num_regs, int* max_th
 static int ensure_dynamic_smem(Module* m, Kernel* k, uint32_t smem) {
   if (smem > 0 && (int)smem > k->smem_set) {
     std::lock_guard<std::mutex> lock(m->mu);
+    RelaxedCapture relaxed;
     CUresult r = driver().func_set_attribute(k->fn, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
                                              (int)smem);
     if (r != CUDA_SUCCESS) return drv_fail(r, "cuFuncSetAttribute(max dynamic smem)");
@@ -288,6 +299,7 @@ int molten_max_resident(void* mod, const char* kernel, const molten_launch_cfg* 
   Kernel* k = nullptr;
   int rc = lookup(m, kernel, &k);
   if (rc) return rc;
+  RelaxedCapture relaxed;
   rc = use_device(m->device);
   if (rc) return rc;
   rc = ensure_dynamic_smem(m, k, cfg->smem_bytes);
@@ -478,6 +490,7 @@ int molten_status_word(int device, int** dev_ptr) {
   std::lock_guard<std::mutex> lock(g_status_mu);
   if ((int)g_status.size() <= device) g_status.resize(device + 1, nullptr);
   if (!g_status[device]) {
+    RelaxedCapture relaxed;
     int rc = use_device(device);
     if (rc) return rc;
     int* p = nullptr;

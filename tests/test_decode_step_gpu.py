@@ -633,3 +633,67 @@ def test_outputs_of_a_named_stream_take_no_memory_in_use(rt):
         torch.cuda.synchronize()
         assert torch.equal(kept, want + 1.0)
         del kept
+
+
+# ------------------------------------------------------- the first call captured
+def fresh(tmp_path, call):
+    """``call`` with a runtime whose modules are not loaded yet."""
+    import shutil
+    ck, _ = call(MoltenRuntime(), 0)
+    (tmp_path / "cache").mkdir()
+    shutil.copy(ck._module, tmp_path / "cache")
+    return call(MoltenRuntime(cache_dir=str(tmp_path / "cache")), 0)
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_the_first_call_may_be_captured(rt, call, tmp_path):
+    """Modules are loaded by the first call, also where that is recorded."""
+    want = call(rt, 0)[0](*call(rt, 0)[1]).clone()
+    ck, ins = fresh(tmp_path, call)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ck(*ins)
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_the_first_call_of_other_families_may_be_captured(tmp_path):
+    g = graphs.rmsnorm(64, 512, dtype="bfloat16")
+    x = torch.randn(64, 512, generator=gen_of(1), device=DEV).bfloat16()
+    w = torch.ones(512, device=DEV).bfloat16()
+    k = compile_graph(g, dtype="bfloat16")[0]
+    want = MoltenRuntime().compile(k)(x, w)
+    ck = MoltenRuntime(cache_dir=str(tmp_path)).compile(k)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ck(x, w)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    """The status word is allocated with the first kernel that has one."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+from tests.test_decode_step_gpu import rope_call, tiles_call
+from molten_b200.runtime import MoltenRuntime
+rt = MoltenRuntime()
+for call in (rope_call, tiles_call):
+    ck, ins = call(rt, 0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ck(*ins)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, ck(*ins))
+assert MoltenRuntime.read_status(0) == 0
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).parents[1], capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
