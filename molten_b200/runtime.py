@@ -86,6 +86,7 @@ class _Spec:
         self._tmaps: OrderedDict = OrderedDict()
         self.align = [_alignment_rules(sk) for sk in self.plan.kernels]
         self.single = ModelCall.fits(self)
+        self.short: dict = {}      # device -> the short way into a plan that is one model operator
         self.model = any(sk.family == "model" for sk in self.plan.kernels)
 
     def module(self, device: int) -> _capi.Module:
@@ -502,7 +503,10 @@ class CompiledKernel:
                 for t in res:
                     t.record_stream(torch.cuda.current_stream(dev))
         if not DEBUG and spec.single:
-            self._last = short_call(spec, tensors)
+            # (made once for a device: a plan fixes the shapes and types)
+            self._last = spec.short.get(dev.index)
+            if self._last is None:
+                self._last = spec.short[dev.index] = short_call(spec, tensors)
         return res[0] if len(res) == 1 else tuple(res)
 
     def _run(self, spec: _Spec, tensors, outs, stream: int, row_offset: int):

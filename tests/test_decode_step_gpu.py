@@ -697,3 +697,25 @@ assert MoltenRuntime.read_status(0) == 0
     done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).parents[1], capture_output=True, text=True,
                           timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+# ----------------------------------------------------------- cost of a call
+@pytest.mark.parametrize("call", CALLS)
+def test_the_short_way_is_made_once(call, monkeypatch):
+    """Calls that cannot take it (a given output or stream, strided inputs, other
+    shapes in turn) do not make it again."""
+    from molten_b200 import runtime
+    made = []
+    short_call = runtime.short_call
+    monkeypatch.setattr(runtime, "short_call", lambda spec, tensors: made.append(spec) or short_call(spec, tensors))
+    ck, ins = call(MoltenRuntime(), 0)
+    want = ck(*ins).clone()
+    out = torch.empty_like(want)
+    wide = torch.zeros(ins[0].shape + (2,), dtype=ins[0].dtype, device=DEV)
+    wide[..., 0] = ins[0]
+    for _ in range(4):
+        assert torch.equal(ck(*ins, out=out), want)
+        assert torch.equal(ck(*ins, stream=torch.cuda.current_stream().cuda_stream), want)
+        assert torch.equal(ck(wide[..., 0], *ins[1:]), want)
+        assert torch.equal(ck(*ins), want)
+    assert len(made) == 1
