@@ -368,10 +368,32 @@ def launch_model_op(spec, i: int, env: dict, device: int, stream: int) -> None:
 
 def _extent(t):
     """(first byte, byte behind the last) of a tensor's memory."""
+    start = t.data_ptr()
+    if t.is_contiguous():
+        return start, start + t.nbytes
     if t.numel() == 0:
-        return 0, 0
-    span = 1 + sum((d - 1) * s for d, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + span * t.element_size()
+        return start, start
+    return start, start + (1 + sum((d - 1) * s for d, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _overlap_rules(plan) -> list:
+    """What each output may not overlap: [[(place among the inputs, or place
+    among the outputs - their number, the input is RoPE's x, name)]]."""
+    places = {o: n - len(plan.outputs) for n, o in enumerate(plan.outputs)}
+    places.update((o, n) for n, o in enumerate(plan.inputs))
+    rules = []
+    for n, o in enumerate(plan.outputs):
+        found = [(m - len(plan.outputs), False, "another output") for m in range(n)]
+        i = next(i for i, sk in enumerate(plan.kernels) if any(w.op_id == o for w in sk.outputs))
+        for j, sk in enumerate(plan.kernels[i:], i):
+            if "model" not in (sk.family, plan.kernels[i].family):
+                continue
+            for operand in sk.operands:
+                if operand.op_id in places and operand.op_id != o:
+                    turned = (j == i and sk.config["op"] == ModelOpType.ROTATE_POSITIONS and operand.index == 0)
+                    found.append((places[operand.op_id], turned, f"the input {operand.name!r}"))
+        rules.append(found)
+    return rules
 
 
 def refuse_overlap(plan, tensors, outs) -> None:
@@ -379,29 +401,20 @@ def refuse_overlap(plan, tensors, outs) -> None:
     other blocks of its kernel, or a kernel after it, still read, nor in
     another output's.  (RoPE turns pairs where they are: its x may be its
     output.  Kernels of the other families are left to the caller.)"""
-    if not any(sk.family == "model" for sk in plan.kernels):
-        return
-    env = dict(zip(plan.inputs, tensors))
-    env.update(zip(plan.outputs, outs))
-    extents = {i: _extent(t) for i, t in env.items()}
-
-    def overlap(a, b):
-        return extents[a][0] < extents[b][1] and extents[b][0] < extents[a][1]
-    for n, o in enumerate(plan.outputs):
-        if any(overlap(o, other) for other in plan.outputs[:n]):
-            raise RuntimeError(f"{plan.name}: two outputs overlap")
-        i = next(i for i, sk in enumerate(plan.kernels) if any(w.op_id == o for w in sk.outputs))
-        for j, sk in enumerate(plan.kernels[i:], i):
-            if "model" not in (sk.family, plan.kernels[i].family):
-                continue
-            for operand in sk.operands:
-                t = env.get(operand.op_id)
-                if t is None or operand.op_id == o or not overlap(o, operand.op_id):
+    if plan.overlap is None:
+        model = any(sk.family == "model" for sk in plan.kernels)
+        plan.overlap = _overlap_rules(plan) if model else []
+    every = list(tensors) + list(outs)               # (negative places count from the end)
+    extents = [_extent(t) for t in every] if plan.overlap else None
+    for n, rules in enumerate(plan.overlap):
+        start, end = extents[n - len(outs)]
+        for place, turned, name in rules:
+            first, last = extents[place]
+            if max(start, first) < min(end, last):       # (never with an empty tensor)
+                t, out = every[place], outs[n]
+                if turned and first == start and t.is_contiguous() and t.dtype == out.dtype:
                     continue
-                if (j == i and sk.config["op"] == ModelOpType.ROTATE_POSITIONS and operand.index == 0
-                        and t.data_ptr() == env[o].data_ptr() and t.is_contiguous() and t.dtype == env[o].dtype):
-                    continue
-                raise RuntimeError(f"{plan.name}: an output overlaps the input {operand.name!r}")
+                raise RuntimeError(f"{plan.name}: an output overlaps {name}")
 
 
 class ModelCall:

@@ -244,6 +244,7 @@ class GroupPlan:
     # what tells plans of the same source apart: which input feeds which operand,
     # attributes and sizes passed at launch
     key: str = ""
+    overlap: Optional[list] = None    # what outputs may not overlap (decode_launch.refuse_overlap)
 
 
 # ------------------------------------------------------------ group split
