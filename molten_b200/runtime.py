@@ -69,6 +69,26 @@ PDL = os.environ.get("MOLTEN_PDL", "1") != "0"
 DEBUG = os.environ.get("MOLTEN_DEBUG", "0") not in ("", "0")
 
 
+# Shapes of one kernel kept ready to launch; the oldest goes for a new one.
+MAX_SHAPES = 512
+
+_loaded: dict = {}                 # (cubin, device) -> its module, for every shape and runtime
+_loading = threading.Lock()
+
+
+def loaded_module(cubin, device: int) -> _capi.Module:
+    """The module of a cubin on a device.  A cubin's name holds a hash of its
+    source and the engine headers, so the file behind a name stays the same."""
+    key = (str(cubin), device)
+    m = _loaded.get(key)
+    if m is None:
+        with _loading:
+            m = _loaded.get(key)
+            if m is None:
+                m = _loaded[key] = _capi.Module(key[0], device)
+    return m
+
+
 class _Spec:
     """One shape/dtype specialisation of a group, ready to launch."""
 
@@ -77,7 +97,6 @@ class _Spec:
         self.plan = gk.plan
         self.cubin = cubin
         self.modules: dict = {}
-        self.lock = threading.Lock()
         self.entries = [kernel_entry(gk.name, i, len(self.plan.kernels)).encode()
                         for i in range(len(self.plan.kernels))]
         self.out_dtypes = [_torch_dtype(d) for d in self.plan.output_dtypes]
@@ -92,11 +111,7 @@ class _Spec:
     def module(self, device: int) -> _capi.Module:
         m = self.modules.get(device)
         if m is None:
-            with self.lock:
-                m = self.modules.get(device)
-                if m is None:
-                    m = _capi.Module(str(self.cubin), device)
-                    self.modules[device] = m
+            m = self.modules[device] = loaded_module(self.cubin, device)
         return m
 
     def launch_cfg(self, i: int, device: int) -> _capi.LaunchCfg:
@@ -550,6 +565,8 @@ class CompiledKernel:
         cubin = None if _empty_outputs(gk) else \
             build_cubin(gk.source, gk.name, self.runtime.cache_dir, self.runtime.verbose)
         spec = _Spec(gk, cubin)
+        if len(self._specs) >= MAX_SHAPES:
+            self._specs.pop(next(iter(self._specs)), None)
         self._specs[sig] = spec
         return spec
 

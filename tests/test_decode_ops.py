@@ -537,3 +537,44 @@ def test_rope_reads_x_as_memory_that_it_may_write():
     common = (inc / "common.cuh").read_text()
     for part in common.split("== kLoadInPlace")[1:]:
         assert ".nc" not in part[:part.index("} else")] and "__ldg" not in part[:part.index("} else")]
+
+
+# ----------------------------------------------------------- what shapes share
+def test_shapes_and_runtimes_share_modules(monkeypatch, tmp_path):
+    """A source that holds for all sizes is loaded once on a device."""
+    import torch
+    from molten_b200 import runtime
+    loads = []
+
+    class Module:
+        def __init__(self, path, device):
+            loads.append((path, device))
+    monkeypatch.setattr(runtime, "build_cubin", lambda source, name, *a, **kw: tmp_path / f"{name}.cubin")
+    monkeypatch.setattr(runtime._capi, "Module", Module)
+    monkeypatch.setattr(runtime, "_loaded", {})
+    k = compile_graph(graphs.sample(1, 32768, top_k=True), dtype="float32")[0]
+    for rt in (runtime.MoltenRuntime(cache_dir=str(tmp_path)), runtime.MoltenRuntime(cache_dir=str(tmp_path))):
+        ck = rt.compile(k)
+        for rows in range(1, 11):
+            spec = ck._spec_for([torch.empty(s, device="meta", dtype=t) for s, t in (
+                ((rows, 32768), torch.float32), ((rows,), torch.float32), ((rows,), torch.float32),
+                ((rows,), torch.int32))])
+            assert spec.gk.source == k.source
+            assert spec.module(0) is spec.module(0) is not spec.module(1)
+    assert sorted(loads) == [(str(tmp_path / f"{k.name}.cubin"), d) for d in (0, 1)]
+
+
+def test_the_number_of_kept_shapes_is_bounded(monkeypatch, unbuilt):
+    import torch
+    from molten_b200 import runtime
+    monkeypatch.setattr(runtime, "MAX_SHAPES", 8)
+    ck = unbuilt.compile(compile_graph(graphs.matvec_q4(1, 64, 256, 64), dtype="bfloat16")[0])
+
+    def spec_of(m):
+        return ck._spec_for([torch.empty(s, device="meta", dtype=t) for s, t in (
+            ((m, 256), torch.bfloat16), ((64, 128), torch.uint8), ((64, 4), torch.bfloat16))])
+    for turn in range(2):
+        for m in range(1, 20):
+            spec = spec_of(m)
+            assert spec is spec_of(m) and spec.plan.output_shapes == [(m, 64)]
+            assert len(ck._specs) <= 8
