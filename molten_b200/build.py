@@ -40,12 +40,21 @@ def nvcc_path() -> str:
     raise BuildError("nvcc not found (set MOLTEN_NVCC or CUDA_HOME)")
 
 
+_digest: tuple = (None, "")        # of the headers as they were when last read
+
+
 def _engine_digest() -> str:
-    h = hashlib.sha256()
-    for f in sorted((ENGINE_INCLUDE / "molten").glob("*.cuh")):
-        h.update(f.name.encode())
-        h.update(f.read_bytes())
-    return h.hexdigest()
+    """Hash of the engine headers, read again where one has changed."""
+    global _digest
+    with os.scandir(ENGINE_INCLUDE / "molten") as it:
+        stats = sorted((f.name, f.stat().st_mtime_ns, f.stat().st_size) for f in it if f.name.endswith(".cuh"))
+    if _digest[0] != stats:
+        h = hashlib.sha256()
+        for name, _, _ in stats:
+            h.update(name.encode())
+            h.update((ENGINE_INCLUDE / "molten" / name).read_bytes())
+        _digest = (stats, h.hexdigest())
+    return _digest[1]
 
 
 def default_cache_dir() -> Path:

@@ -481,10 +481,10 @@ def native_call():
     return _native or None
 
 
-def short_call(spec, tensors):
+def short_call(spec, tensors, device: int):
     """The short way into ``spec``, whose plan is one model operator, for
-    tensors like these."""
-    call, device = native_call(), tensors[0].get_device()
+    tensors like these (their shapes and types) on ``device``."""
+    call = native_call()
     python = ModelCall(spec, tensors)
     b = _bound(spec, 0, device)
     short = b.short() if call else None

@@ -521,8 +521,23 @@ class CompiledKernel:
             # (made once for a device: a plan fixes the shapes and types)
             self._last = spec.short.get(dev.index)
             if self._last is None:
-                self._last = spec.short[dev.index] = short_call(spec, tensors)
+                self._last = spec.short[dev.index] = short_call(spec, tensors, dev.index)
         return res[0] if len(res) == 1 else tuple(res)
+
+    def _prepare(self, spec: _Spec) -> None:
+        """What a first call on the current device would do besides launching,
+        where this process uses that device already."""
+        torch = _torch()
+        if spec.cubin is None or not torch.cuda.is_initialized():
+            return
+        device = torch.cuda.current_device()
+        if not torch._C._cuda_hasPrimaryContext(device):
+            return
+        spec.module(device)
+        if not DEBUG and spec.single:
+            like = [torch.empty(s, dtype=_torch_dtype(d), device="meta")
+                    for s, d in zip(spec.plan.input_shapes, spec.plan.input_dtypes)]
+            self._last = spec.short[device] = short_call(spec, like, device)
 
     def _run(self, spec: _Spec, tensors, outs, stream: int, row_offset: int):
         """A call on ``stream``, which is the current one."""
@@ -562,9 +577,7 @@ class CompiledKernel:
                     tune[fam] = dict(tune.get(fam) or {}, vec=1)
             gen = CodeGenerator(dtype=None, tune=tune)
             gk = gen.generate(self.kernel.graph, self.kernel.group, shapes, dtypes)
-        cubin = None if _empty_outputs(gk) else \
-            build_cubin(gk.source, gk.name, self.runtime.cache_dir, self.runtime.verbose)
-        spec = _Spec(gk, cubin)
+        spec = _Spec(gk, self.runtime._cubin(gk))
         if len(self._specs) >= MAX_SHAPES:
             self._specs.pop(next(iter(self._specs)), None)
         self._specs[sig] = spec
@@ -752,6 +765,7 @@ class MoltenRuntime:
         self.cache_dir.mkdir(parents=True, exist_ok=True)
         self.tune = tune or {}
         self._compiled: dict = {}
+        self._cubins: dict = {}        # source -> its cubin
         _capi.load_library()           # fail loudly when the runtime is missing
 
     def compile(self, kernel: GeneratedKernel) -> CompiledKernel:
@@ -762,9 +776,7 @@ class MoltenRuntime:
         ck = self._compiled.get(key)
         if ck is not None:
             return ck
-        # a specialisation whose outputs are empty launches nothing: no cubin
-        cubin = None if _empty_outputs(kernel) else \
-            build_cubin(kernel.source, kernel.name, self.cache_dir, self.verbose)
+        cubin = self._cubin(kernel)
         ck = CompiledKernel(name=kernel.name, source=kernel.source, config=kernel.config,
                             _module=str(cubin), kernel=kernel, runtime=self)
         sig = None
@@ -772,10 +784,22 @@ class MoltenRuntime:
             sig = tuple((_torch_dtype(d), tuple(s))
                         for d, s in zip(kernel.plan.input_dtypes, kernel.plan.input_shapes)) + (True,)
             ck._specs[sig] = _Spec(kernel, cubin)
+            ck._prepare(ck._specs[sig])
         self._compiled[key] = ck
         if self.verbose and cubin is not None:
             print(f"molten: built {cubin.name}")
         return ck
+
+    def _cubin(self, kernel: GeneratedKernel) -> Optional[Path]:
+        """The cubin of a kernel: of the same source the same one, and none
+        where the outputs are empty (nothing is launched)."""
+        if _empty_outputs(kernel):
+            return None
+        cubin = self._cubins.get(kernel.source)
+        if cubin is None:
+            cubin = build_cubin(kernel.source, kernel.name, self.cache_dir, self.verbose)
+            self._cubins[kernel.source] = cubin
+        return cubin
 
     def clear_cache(self) -> None:
         if self.cache_dir.exists():
@@ -783,6 +807,7 @@ class MoltenRuntime:
                 if f.suffix in (".cubin", ".cu"):
                     f.unlink()
         self._compiled.clear()
+        self._cubins.clear()
 
     @staticmethod
     def read_status(device: int = 0, reset: bool = True) -> int:

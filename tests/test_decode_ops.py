@@ -578,3 +578,33 @@ def test_the_number_of_kept_shapes_is_bounded(monkeypatch, unbuilt):
             spec = spec_of(m)
             assert spec is spec_of(m) and spec.plan.output_shapes == [(m, 64)]
             assert len(ck._specs) <= 8
+
+
+def test_headers_are_read_again_where_they_changed(monkeypatch, tmp_path):
+    from molten_b200 import build
+    (tmp_path / "molten").mkdir()
+    a, b = tmp_path / "molten" / "a.cuh", tmp_path / "molten" / "b.cuh"
+    a.write_text("one")
+    b.write_text("two")
+    monkeypatch.setattr(build, "ENGINE_INCLUDE", tmp_path)
+    seen = [build._engine_digest()]
+    assert build._engine_digest() == seen[0]
+    for change in (lambda: a.write_text("longer"), lambda: b.unlink(), lambda: b.write_text("2"), lambda: b.rename(a)):
+        change()
+        seen.append(build._engine_digest())
+    assert len(set(seen)) == len(seen)
+
+
+def test_one_source_is_looked_up_once(monkeypatch, tmp_path):
+    import torch
+    from molten_b200 import runtime
+    built = []
+    monkeypatch.setattr(runtime, "build_cubin", lambda source, name, *a, **kw: built.append(source) or tmp_path / "x.cubin")
+    rt = runtime.MoltenRuntime(cache_dir=str(tmp_path))
+    ck = rt.compile(compile_graph(graphs.sample(1, 32768), dtype="float32")[0])
+    for rows in range(0, 9):
+        ck._spec_for([torch.empty(s, device="meta") for s in ((rows, 32768), (rows,), (rows,))])
+    assert len(built) == 1
+    rt.clear_cache()
+    rt.compile(ck.kernel)
+    assert len(built) == 2

@@ -659,6 +659,20 @@ def test_the_first_call_may_be_captured(rt, call, tmp_path):
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("call", CALLS)
+def test_a_compiled_kernel_is_ready(rt, call, monkeypatch):
+    """compile() loads the module and makes the short way: the first call with
+    the declared shapes does neither, and builds no parameter block by itself."""
+    from molten_b200 import runtime
+    torch.zeros(1, device=DEV)
+    ck, ins = call(MoltenRuntime(), 0)
+    assert ck._last is not None
+    monkeypatch.setattr(runtime, "loaded_module", None)
+    monkeypatch.setattr(runtime, "short_call", None)
+    monkeypatch.setattr(type(ck), "_spec_for", None)
+    assert torch.equal(ck(*ins), call(rt, 0)[0](*ins))
+
+
 def test_the_first_call_of_other_families_may_be_captured(tmp_path):
     g = graphs.rmsnorm(64, 512, dtype="bfloat16")
     x = torch.randn(64, 512, generator=gen_of(1), device=DEV).bfloat16()
@@ -707,7 +721,7 @@ def test_the_short_way_is_made_once(call, monkeypatch):
     from molten_b200 import runtime
     made = []
     short_call = runtime.short_call
-    monkeypatch.setattr(runtime, "short_call", lambda spec, tensors: made.append(spec) or short_call(spec, tensors))
+    monkeypatch.setattr(runtime, "short_call", lambda *args: made.append(args) or short_call(*args))
     ck, ins = call(MoltenRuntime(), 0)
     want = ck(*ins).clone()
     out = torch.empty_like(want)
