@@ -608,3 +608,23 @@ def test_one_source_is_looked_up_once(monkeypatch, tmp_path):
     rt.clear_cache()
     rt.compile(ck.kernel)
     assert len(built) == 2
+
+
+@pytest.mark.parametrize("failure", [FileNotFoundError("g++"), "BuildError"])
+def test_kernels_are_built_without_the_short_host_path(failure, monkeypatch, capsys, tmp_path):
+    """The native short path has a complete fallback: what it needs besides nvcc
+    does not keep the kernels from being built."""
+    import __graft_entry__ as entry
+    from molten_b200 import build
+    from oracle import build_ref
+    built = []
+
+    def fails(*a, **kw):
+        raise build.BuildError("torch/extension.h") if failure == "BuildError" else failure
+    monkeypatch.setattr(build, "build_call", fails)
+    monkeypatch.setattr(build, "build_runtime", lambda *a, **kw: built.append("runtime"))
+    monkeypatch.setattr(build, "build_cubin", lambda source, name, *a, **kw: built.append(name))
+    monkeypatch.setattr(build_ref, "build", lambda *a, **kw: None)
+    entry.build()
+    assert "runtime" in built and len(built) > 10
+    assert "short host path was not built" in capsys.readouterr().err
