@@ -39,6 +39,8 @@ WINDOW_STAGES, WINDOW_TILE = 3, 16
 
 SAMPLE_FIXED = 2 * 8 * 24 + 32 * 24 + 2048 + 4096 + 2 * 2048 + 64   # of SampleShared (molten/sample.cuh)
 
+SAMPLE_PARAMS = ("temperature", "top_k", "top_p", "min_p")
+
 ROPE_MAX_AXES = 4
 ROPE_MAX_DIM = 1024
 
@@ -112,11 +114,16 @@ def _window_shape(op, ins):
 
 
 def _sample_shape(op, ins):
+    _need(len(ins) >= 2, "sample takes (logits, u[, parameters])")
     logits, u = ins[:2]
     _need(len(logits) >= 2 and logits[-1] > 0, f"sample needs logits [..., vocabulary], got {logits}")
     lead = logits[:-1]
     _need(u == lead, f"sample: u of shape {u}, expected {lead}")
-    for name, s in zip(op.attrs.get("params", ()), ins[2:]):
+    params = op.attrs.get("params") or ()
+    _need(isinstance(params, (list, tuple)) and len(params) == len(ins) - 2 and len(set(params)) == len(params)
+          and set(params) <= set(SAMPLE_PARAMS),
+          f"sample: parameters {params!r} for {len(ins) - 2} inputs behind logits and u; each one of {SAMPLE_PARAMS}")
+    for name, s in zip(params, ins[2:]):
         _need(s in ((), lead), f"sample: {name} of shape {s}, expected {lead} or a constant")
     return lead
 
@@ -423,6 +430,9 @@ def _plan_sample(op, sk, tune) -> dict:
     logits = sk.operands[0]
     vocab, rows = logits.shape[-1], prod(logits.shape[:-1])
     _need(rows * 8 < 2 ** 31, "sample: sizes beyond 2^31")
+    for pos, value in sk.config["scalars"].items():
+        _need(op.attrs["params"][pos - 2] != "top_k" or value == value // 1,
+              f"sample: top_k {value} is not a whole number")
     o = tune.get("sample") or {}
 
     word = 4 // DTYPE_SIZE[logits.dtype]              # tokens of 32 bits

@@ -23,7 +23,7 @@ import math
 from struct import Struct
 
 from . import _capi
-from .decode import SMS
+from .decode import SAMPLE_PARAMS, SMS
 from .ir import ModelOpType
 from .lowering import DTYPE_SIZE
 
@@ -304,7 +304,7 @@ class _Window(_Bound):
 
 class _Sample(_Bound):
     head = Struct("<7Qq")
-    slots = ("temperature", "top_k", "top_p", "min_p")
+    slots = SAMPLE_PARAMS
 
     def setup(self):
         c = self.c
@@ -323,7 +323,8 @@ class _Sample(_Bound):
         a.temperature_all, a.top_p_all = 1.0, 1.0        # without a parameter: no limit
         for pos, value in c["scalars"].items():
             name = c["params"][pos - 2]
-            setattr(a, name + "_all", int(value) if name == "top_k" else float(value))
+            # (past 32 bits: every token; below 0: no limit)
+            setattr(a, name + "_all", max(-1, min(int(value), 2 ** 31 - 1)) if name == "top_k" else float(value))
 
     def conform(self, ins):
         x = _merged(ins[0], 1)

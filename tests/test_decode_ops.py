@@ -628,3 +628,31 @@ def test_kernels_are_built_without_the_short_host_path(failure, monkeypatch, cap
     entry.build()
     assert "runtime" in built and len(built) > 10
     assert "short host path was not built" in capsys.readouterr().err
+
+
+# --------------------------------------------- parameters by name and by number
+@pytest.mark.parametrize("params", [[], ["temperature"], ["topk", "top_p"], ["top_k", "top_k"], ["top_k", "top_p", "min_p"],
+                                    "top_k", None])
+def test_sample_parameters_that_do_not_fit_its_inputs(params):
+    """Inputs without a name, or with one that is not known, would be left out."""
+    g = DataflowGraph("sample")
+    x, u = g.add_input("x", TS([4, 100]), dtype="float32"), g.add_input("u", TS([4]), dtype="float32")
+    k, p = g.add_input("k", TS([4]), dtype="int32"), g.add_input("p", TS([4]), dtype="float32")
+    attrs = {} if params is None else {"params": params}
+    g.add_output(g.add_op(ModelOpType.SAMPLE, [x, u, k, p], "token", **attrs))
+    refused(g, "sample: parameters", "float32")
+
+
+@pytest.mark.parametrize("value,text", [(float("nan"), "top_k"), (float("inf"), "top_k"), (2.5, "top_k")])
+def test_sample_top_k_is_a_whole_number(value, text):
+    refused(graphs.sample(4, 100, top_k=value), text, "float32")
+
+
+def test_sample_top_k_past_32_bits_is_no_limit():
+    from molten_b200.decode_launch import _Sample
+    for value, want in ((40, 40), (40.0, 40), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 32 + 5, 2 ** 31 - 1), (-2 ** 40, -1), (0, 0)):
+        (k,) = compile_graph(graphs.sample(4, 100, top_k=value), dtype="float32")
+        bound = object.__new__(_Sample)
+        bound.c, a = k.plan.kernels[0].config, _capi.SampleArgs()
+        bound.fill(a)
+        assert min(a.top_k_all, 100) == min(want, 100) and (a.top_k_all > 0) == (want > 0)
