@@ -30,7 +30,9 @@ from . import __version__
 from .compiler import ZeroCompiler
 from .ir import DataflowGraph, ModelOpType, OpType, TensorShape
 
-_ATTR_KEYS = ("eps", "value", "min", "max", "period", "offset", "kind", "dim")
+# attributes that may stand beside an op's type instead of in its "attrs"
+_ATTR_KEYS = ("eps", "value", "min", "max", "period", "offset", "kind", "dim",
+              "style", "sections", "packed", "window", "sinks", "scale", "params")
 
 
 def graph_from_json(data: dict) -> DataflowGraph:

@@ -656,3 +656,20 @@ def test_sample_top_k_past_32_bits_is_no_limit():
         bound.c, a = k.plan.kernels[0].config, _capi.SampleArgs()
         bound.fill(a)
         assert min(a.top_k_all, 100) == min(want, 100) and (a.top_k_all > 0) == (want > 0)
+
+
+def test_json_attributes_beside_the_type():
+    """Attributes of these operators may stand beside the type, as eps may."""
+    ops = [{"type": "INPUT", "name": n, "inputs": [], "shape": s, "dtype": "bfloat16"}
+           for n, s in (("q", [1, 1, 4, 64]), ("k", [1, 90, 2, 64]), ("v", [1, 90, 2, 64]))]
+    ops += [{"type": "WINDOW_ATTENTION", "inputs": [0, 1, 2], "window": 20, "sinks": 3, "scale": 0.5},
+            {"type": "OUTPUT", "inputs": [3]}]
+    g = cli.graph_from_json({"name": "a", "ops": ops})
+    assert config_of(g, "bfloat16") == config_of(
+        graphs.window_attention(1, 1, 90, 4, 2, 64, window=20, sinks=3, scale=0.5, lengths=False), "bfloat16")
+    ops = [{"type": "INPUT", "name": n, "inputs": [], "shape": s, "dtype": d}
+           for n, s, d in (("x", [1, 5, 2, 64], "bfloat16"), ("f", [9, 64], "float32"), ("p", [2, 1, 5], "int32"))]
+    ops += [{"type": "ROTATE_POSITIONS", "inputs": [0, 1, 2], "sections": [20, 12], "style": "half", "packed": True},
+            {"type": "OUTPUT", "inputs": [3]}]
+    c = config_of(cli.graph_from_json({"name": "a", "ops": ops}), "bfloat16")
+    assert c["sections"] == [20, 12] and c["half"] and c["packed"]
