@@ -24,7 +24,9 @@
 //
 // P is the sum of two 16-bit values (P and what its rounding leaves), two
 // MMAs: P V is exact to 2^-16, so the output rounding is the only one that
-// shows, and the second MMA hides behind the loads.
+// shows, and the second MMA hides behind the loads.  fp16 weights (and with them
+// O and the sum) are taken times 2^15: their largest is 2^15, and the two parts
+// keep their bits down to 2^-28 of it (without: down to 2^-13, nothing below 2^-25).
 //
 // Keys that no query sees are not read: their slots are zero-filled, so
 // whatever a cache holds behind its last token or outside the window never
@@ -332,8 +334,11 @@ __device__ __forceinline__ void window_decode(const WindowArgs& a, uint8_t* raw)
         fix[n][e] = fast_exp2(mx[n][e] - base);
         moved |= mn != mx[n][e];
         mx[n][e] = mn;
-        x0 = fast_exp2(x0 - base);
-        x1 = fast_exp2(x1 - base);
+        x0 -= base;
+        x1 -= base;
+        if constexpr (std::is_same<T, f16>::value) { x0 += 15.0f; x1 += 15.0f; }
+        x0 = fast_exp2(x0);
+        x1 = fast_exp2(x1);
         sum[n][e] = sum[n][e] * fix[n][e] + (x0 + x1);
         s[n][e] = x0;
         s[n][e + 2] = x1;

@@ -902,3 +902,24 @@ def test_matvec_q4_sums_past_the_range(rt):
     s = s * 1e-6
     y = compiled(rt, graphs.matvec_q4(m, n, k, group, dtype="float32", zeros=True), "float32")(x, q, s, z)
     check_q4(y, x, q, s, z, "float32")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("new,gap", [(1, 12.0), (1, 17.0), (4, 17.0), (100, 12.0), (100, 16.0)])
+def test_window_attention_weights_far_below_the_largest(rt, new, gap, dtype):
+    """A first key that takes nearly all the weight and has a value of 0, as
+    sinks do: the output is what e^-12 to e^-17 of it leaves to 20000 others."""
+    b, cache, heads, kv, d = 1, 20000, 4, 1, 64
+    q, k, v = attention_inputs(b, new, cache, heads, kv, d, dtype, seed=9)
+    k = 0.3 * k
+    q[..., 0], k[..., 0] = 4.0, 0.0
+    k[:, 0] = 0.0
+    k[:, 0, :, 0] = gap * d ** 0.5 / 4.0
+    v = v + 1.0
+    v[:, 0] = 0.0
+    lengths = torch.tensor([cache - 3], dtype=torch.int32, device=DEV)
+    ck = window_kernel(rt, b, new, cache, heads, kv, d, 19000, 2, dtype)
+    out = ck(q, k, v, lengths)
+    half = half_step(dtype) if ck.kernel.plan.kernels[0].config["kind"] == "tiles" else 2.0 ** -16
+    check_attention(out, q, k, v, lengths, 19000, 2, dtype, half)
+    assert bool((out > 0).all())
