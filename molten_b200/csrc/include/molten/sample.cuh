@@ -562,8 +562,11 @@ __device__ __noinline__ int sample_draw(Sampler<T, THREADS>& k, int per, float l
     if (tau > -INFINITY && goal > got.z) {           // inside the ties of top_k's border
       ties = fmin(ties, fmax(1.0, ceil((goal - got.z) / wt)));
     } else if (goal > 0.0) {
-      const bool narrow = -got.x < k.sure && k.sure < k.m;
-      tau = k.border(true, -got.x, narrow ? k.sure : k.m, count, goal, narrow ? got.w : 0.0, &ties);
+      // (not below m - 40 T, as above: an interval down to a mask's value, of which
+      // the bins hold all weights in one, would not narrow)
+      const float low = fmaxf(-got.x, (float)((double)k.m - 40.0 * 256.0 * 1.4426950408889634074 / k.c));
+      const bool narrow = low < k.sure && k.sure < k.m;
+      tau = k.border(true, low, narrow ? k.sure : k.m, count, goal, narrow ? got.w : 0.0, &ties);
       ties = fmax(ties, 1.0);
     } else {
       tau = k.m;                                     // the largest token at least

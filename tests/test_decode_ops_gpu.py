@@ -923,3 +923,22 @@ def test_window_attention_weights_far_below_the_largest(rt, new, gap, dtype):
     half = half_step(dtype) if ck.kernel.plan.kernels[0].config["kind"] == "tiles" else 2.0 ** -16
     check_attention(out, q, k, v, lengths, 19000, 2, dtype, half)
     assert bool((out > 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("use", ["p", "kp", "pm"])
+@pytest.mark.parametrize("rows,vocab", [(3, 22670), (18, 164945)])
+def test_sample_masks_of_the_lowest_value_in_flat_rows(rt, rows, vocab, use, dtype):
+    """Masked tokens that are finite, in rows of which the filters keep too many
+    tokens for the packed list."""
+    x, u = sample_inputs(rows, vocab, dtype, seed=vocab, spread=1.0)
+    g = gen_of(51)
+    x[torch.rand(rows, vocab, generator=g, device=DEV) < 0.3] = torch.finfo(x.dtype).min
+    params = {"temperature": 1.0 + 7.0 * torch.rand(rows, generator=g, device=DEV)}
+    if "k" in use:
+        params["top_k"] = torch.full((rows,), vocab * 3 // 5, dtype=torch.int32, device=DEV)
+    params["top_p"] = 0.5 + 0.499 * torch.rand(rows, generator=g, device=DEV)
+    if "m" in use:
+        params["min_p"] = torch.full((rows,), 1e-3, device=DEV)
+    ck = compiled(rt, graphs.sample(rows, vocab, dtype=dtype, top_k="k" in use, top_p=True, min_p="m" in use), dtype)
+    check_sample(ck(x, u, *params.values()), x, u, **params)
