@@ -35,11 +35,10 @@
 // 100003 fp32, some rows with each filter, 156 us; the same unfiltered 103 us
 // (0.99 TB/s).
 //
-// Only the tail that top_p surely drops, of which it needs nothing but the
-// total, has fp32 terms (summed by a thread, then in fp64).  Each is off by up to
-// some 2^-20, without a common part, so the total of thousands by near 1e-8 of
-// itself; that moves the border past a token (of some 1e-5 of the whole) for one
-// row in 10^3 or fewer, and the token at the border is one of the least likely.
+// The tail that top_p surely drops, of which it needs nothing but the total, has
+// 64-bit terms as well: with ex2.approx ones the total of thousands was off by near
+// 1e-8 of itself, which moved the border past a token for one row in 10^3 (64 x
+// 131072 took 108 us then, 114 now).
 //
 // All CTAs of a cluster compute the same values from the same numbers, so they
 // take the same steps.
@@ -801,23 +800,19 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, uint8_t* raw) {
   double tail = 0.0;
   bool packed = false, gather = false;
   if (from > -INFINITY) {
-    // the tokens from there up; the weight of the rest, in fp32
+    // the tokens from there up; the weight of the rest
     int hits = 0;
-    float rest = 0.0f;
-    // (two floats: an error of the factor would be the same in every term; half
-    // differences down to the cut, so that both products are finite)
-    const float c1 = (float)(k.c / 128.0), c1_low = (float)(k.c / 128.0 - (double)c1);
+    double rest = 0.0;
     if (by_weight && top_p < 1.0f)
       sm_each(mine, a.run, [&](int, float x) {
         hits += x >= from ? 1 : 0;
-        const float d = 0.5f * fmaxf(x, k.cut) - 0.5f * k.m;
-        const float e = fast_exp2(fmaf(d, c1, d * c1_low));
-        rest += x < from && x >= k.cut ? e : 0.0f;
+        const double w = k.weight(x);
+        rest += x < from ? w : 0.0;
       });
     else
       sm_each(mine, a.run, [&](int, float x) { hits += x >= from ? 1 : 0; });
     SampleSums all;
-    int place = (int)sm_scan<THREADS>(sh, {(double)rest, (float)hits, 0.0f}, &all).y - hits;
+    int place = (int)sm_scan<THREADS>(sh, {rest, (float)hits, 0.0f}, &all).y - hits;
     const SampleShare* ex = sm_publish(sh, a.ranks, rank, {0.0f, 0.0f, (double)all.y, all.x});
     int most = 0, first = 0;
     many = 0;

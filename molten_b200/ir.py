@@ -265,8 +265,8 @@ class DataflowGraph:
         the first, by index, at which the running weight of the kept tokens
         exceeds u times their sum.  ``temperature`` below 1e-30 takes the
         largest logit.  NaN logits and -inf are never drawn (a row of nothing
-        else gives -1); +inf counts as the largest finite number of its type.  Weights and sums have 64 bits, but for the weight that
-        ``top_p`` surely drops, whose total has 32-bit terms."""
+        else gives -1); +inf counts as the largest finite number of its
+        type.  Weights and sums have 64 bits."""
         params = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
         given = [k for k, v in params.items() if v is not None]
         return self.add_op(ModelOpType.SAMPLE, [logits, u] + [params[k] for k in given], name,

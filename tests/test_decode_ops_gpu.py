@@ -942,3 +942,22 @@ def test_sample_masks_of_the_lowest_value_in_flat_rows(rt, rows, vocab, use, dty
         params["min_p"] = torch.full((rows,), 1e-3, device=DEV)
     ck = compiled(rt, graphs.sample(rows, vocab, dtype=dtype, top_k="k" in use, top_p=True, min_p="m" in use), dtype)
     check_sample(ck(x, u, *params.values()), x, u, **params)
+
+
+@pytest.mark.parametrize("rows,vocab", [(64, 30011), (24, 131072)])
+def test_sample_top_p_next_to_a_running_weight(rt, rows, vocab):
+    """top_p within 2e-10 to 1e-9 of what the tokens down to one of them weigh: it
+    is the last one kept, or the first one dropped, and u near 1 draws it."""
+    x, _ = sample_inputs(rows, vocab, "float32", seed=vocab)
+    x = x.sort(-1, descending=True).values
+    w = np.exp((x - x[:, :1]).double().cpu().numpy())
+    reach = np.cumsum(w, 1) / w.sum(1, keepdims=True)
+    p = reach.astype(np.float32)
+    off = np.abs(p.astype(np.float64) - reach)
+    fits = (reach > 0.6) & (reach < 0.97) & (off > 2e-10) & (off < 1e-9)
+    at = fits.argmax(1)
+    assert fits.any(1).mean() > 0.9
+    top_p = torch.from_numpy(p[np.arange(rows), at]).to(DEV)
+    u = torch.full((rows,), 1.0 - 2.0 ** -24, device=DEV)
+    t = torch.ones(rows, device=DEV)
+    check_sample(compiled(rt, graphs.sample(rows, vocab, top_p=True), "float32")(x, u, t, top_p), x, u, top_p=top_p)
