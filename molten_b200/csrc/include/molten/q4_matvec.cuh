@@ -20,9 +20,9 @@
 // scale.  k may be summed in any order, so nothing is shuffled: the pairs of
 // x are permuted to match once, as x is staged in shared memory.
 // (As 128 + q in bf16, minus 136, with x permuted on every use and every loop
-// unrolled, 3 x 100003 x 5120 took 92 us; it takes 63.5, 4.2 TB/s.  1 x 4096 x
-// 4096 takes 5.7 us, of it some 3 the latency of a launch, staging x and one
-// chain of groups; 8 x 14336 x 4096 with zero points and groups of 64 22.9: x is
+// unrolled, 3 x 100003 x 5120 took 92 us; it takes 62.6, 4.2 TB/s.  1 x 4096 x
+// 4096 takes 5.8 us, of it some 3 the latency of a launch, staging x and one
+// chain of groups; 8 x 14336 x 4096 with zero points and groups of 64 22.8: x is
 // staged once by each CTA, and the two sums of a group cost as much as its MMAs.)
 //
 // x is staged as fp16 whatever its type: each group of a row is scaled by a

@@ -17,7 +17,7 @@
 // out may be x: x is loaded as memory that changes.
 //
 // Measured, bf16 with fp32 tables: 4 x 4096 tokens of 32 heads of 128, one axis
-// 45.7 us (5.9 TB/s), three axes at random positions 50.4 (each section's table
+// 45.0 us (6.0 TB/s), three axes at random positions 49.6 (each section's table
 // rows come from L2); 48 tokens of 40 heads 2.1 us.
 #pragma once
 

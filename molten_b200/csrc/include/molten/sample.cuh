@@ -29,16 +29,15 @@
 // each with all.  Rows whose kept tokens do not fit the packed list go the same
 // way with the whole row in its place.
 //
-// Measured: 1 x 32768 fp32 with top_k and top_p 21.7 us; 64 x 131072 bf16 with
-// top_p and min_p, 16000 tokens kept, 100 us (132 with the tokens that are surely
-// kept left in the border's search, 109 with their weights behind a branch); 256 x
-// 100003 fp32, some rows with each filter, 156 us; the same unfiltered 103 us
-// (0.99 TB/s).
+// Measured: 1 x 32768 fp32 with top_k and top_p 22.0 us; 64 x 131072 bf16 with
+// top_p and min_p, 16000 tokens kept, 108 us (before the dropped ones' 64-bit
+// weights 100; 132 with the tokens that are surely kept left in the border's
+// search, 109 with their weights behind a branch); 256 x 100003 fp32, some rows
+// with each filter, 157 us; the same unfiltered 103 us (0.99 TB/s).
 //
 // The tail that top_p surely drops, of which it needs nothing but the total, has
 // 64-bit terms as well: with ex2.approx ones the total of thousands was off by near
-// 1e-8 of itself, which moved the border past a token for one row in 10^3 (64 x
-// 131072 took 108 us then, 114 now).
+// 1e-8 of itself, which moved the border past a token for one row in 10^3.
 //
 // All CTAs of a cluster compute the same values from the same numbers, so they
 // take the same steps.

@@ -32,8 +32,8 @@
 // factor, so nothing is lost.  (fp16 weights are taken times 2^7.)
 //
 // Measured: 8192 tokens, 32 heads over 8, head dim 128, window 2048: 256 us (941
-// TFLOP/s of visible pairs); 4 x 500 tokens over up to 2900, head dim 64, window
-// 1000: 27.3 us.  With a whole row of S in registers (spills) the first took 489,
+// TFLOP/s of visible pairs), 288 (837) at the clock that seconds of such calls
+// leave; 4 x 500 tokens over up to 2900, head dim 64, window 1000: 27.1 us.  With a whole row of S in registers (spills) the first took 489,
 // with its maximum first 314.  S by halves, so that it can be computed ahead:
 // 270 (N = 64 takes the tensor core as long as N = 128); an issuing warp for
 // each Q tile: 310; 4 of 32 exponentials on the FMA pipe: 274 where none was 271;

@@ -9,8 +9,8 @@ and captured graphs never share one.
 A call has two ways in.  ``launch_model_op`` runs a model operator among the
 sub-kernels of any plan and brings operands into a layout the kernel takes.
 ``short_call`` is the short way for a graph that is one model operator, called
-again with the shapes of its last call: single tokens run for a few
-microseconds, less than the general path's bookkeeping.  It declines
+with the declared shapes or again with those of its last call: single tokens run
+for a few microseconds, less than the general path's bookkeeping.  It declines
 (``NotImplemented``) whatever is not plain, and the general path takes over.
 Its steps are native (``csrc/call.cpp``) where that library is built, 4 to 6 us a
 call, else ``ModelCall``'s, 9 to 11.
