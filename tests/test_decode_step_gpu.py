@@ -733,3 +733,27 @@ def test_the_short_way_is_made_once(call, monkeypatch):
         assert torch.equal(ck(wide[..., 0], *ins[1:]), want)
         assert torch.equal(ck(*ins), want)
     assert len(made) == 1
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_a_named_stream_inside_a_capture(rt, call):
+    """A branch of a recorded graph: the call's stream follows the captured one
+    and is joined again."""
+    ck, ins = call(rt, 0)
+    want = ck(*ins).clone()
+    wide = torch.zeros(ins[0].shape + (2,), dtype=ins[0].dtype, device=DEV)
+    wide[..., 0] = ins[0]
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        out = ck(wide[..., 0], *ins[1:], stream=side.cuda_stream)
+        here.wait_stream(side)
+        copy = out.clone()
+        del out
+    for _ in range(3):
+        copy.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(copy, want)
