@@ -6,7 +6,10 @@
 // axis(i) is the section that holds pair i (bound[a] = first pair after
 // section a).  Pairs are (i, i + D/2) ("half") or (2i, 2i + 1).  A negative
 // position marks padding: those pairs are copied.  A position past the table
-// sets kRopePositionRange in the status word, and its pairs are copied too.
+// sets kRopePositionRange in the status word, and its pairs are copied too.  (A
+// thread whose slot holds such a pair takes a way of its own, so that the other
+// keeps its registers: with the choice among the products 4 x 4096 tokens took 60
+// us for 51.)
 // fp32 arithmetic, one rounding to the output type.
 //
 // Bound by HBM (x in, x out).  A thread keeps one slot of pairs of one token,
@@ -40,8 +43,9 @@ struct RopePosArgs {
 
 enum RopePosStatus { kRopePositionRange = 4096 };
 
+// cos and sin of the NP pairs from p0 on; bit e of the result: pair e stays as it is.
 template <typename TT, int NP, bool PACKED, bool TVEC>
-__device__ __forceinline__ void rope_table(const RopePosArgs& a, long long token, int p0,
+__device__ __forceinline__ uint32_t rope_table(const RopePosArgs& a, long long token, int p0,
                                            float (&cs)[NP], float (&sn)[NP]) {
   const int half = a.dim / 2;
   int ax = 0;
@@ -66,9 +70,11 @@ __device__ __forceinline__ void rope_table(const RopePosArgs& a, long long token
       if (row >= 0 && a.status) atomicOr(a.status, kRopePositionRange);
 #pragma unroll
       for (int e = 0; e < NP; ++e) { cs[e] = 1.0f; sn[e] = 0.0f; }
+      return (1u << NP) - 1u;
     }
-    return;
+    return 0u;
   }
+  uint32_t stay = 0u;
 #pragma unroll
   for (int e = 0; e < NP; ++e) {
     const int p = p0 + e;
@@ -76,6 +82,7 @@ __device__ __forceinline__ void rope_table(const RopePosArgs& a, long long token
     const long long row = a.pos[(long long)ax * a.tokens + token];
     const bool in = row >= 0 && row < a.table_rows;
     if (row >= a.table_rows && a.status) atomicOr(a.status, kRopePositionRange);
+    stay |= (in ? 0u : 1u) << e;
     if constexpr (PACKED) {
       cs[e] = in ? to_f32(ct[row * a.dim + 2 * p]) : 1.0f;
       sn[e] = in ? to_f32(ct[row * a.dim + 2 * p + 1]) : 0.0f;
@@ -84,6 +91,7 @@ __device__ __forceinline__ void rope_table(const RopePosArgs& a, long long token
       sn[e] = in ? to_f32(st[row * half + p]) : 0.0f;
     }
   }
+  return stay;
 }
 
 // VEC elements of x per slot (a slot and its partner with HALF); XVEC: slots
@@ -123,8 +131,38 @@ __device__ __forceinline__ void rope_positions(const RopePosArgs& a) {
       }
     }
     if (!have) {
-      rope_table<TT, NP, PACKED, TVEC>(a, token, p0, cs, sn);
+      const uint32_t stay = rope_table<TT, NP, PACKED, TVEC>(a, token, p0, cs, sn);
       have = true;
+      if (stay != 0u) {
+        // padding: a turn by 0 would make NaN of an infinity's partner, and 0 of -0
+#pragma unroll 1
+        for (int h = hl; h < a.heads; h += a.head_lanes) {
+          const XT* src = x + h * a.x_head;
+          OT* dst = out + (long long)h * a.dim;
+          if constexpr (XVEC) if (stay == (1u << NP) - 1u) {     // (a whole slot: all axes, mostly)
+#pragma unroll 1
+            for (int p = 0; p < PARTS; ++p) {
+              const Slot<XT, VEC> slot = load_slot<kLoadInPlace, XT, VEC>(src + p * (a.dim / 2));
+              float f[VEC];
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) f[e] = to_f32(slot.v[e]);
+              Slot<OT, VEC> so;
+              pack_slot<OT, VEC>(so, f);
+              store_slot<kStoreDefault, OT, VEC>(dst + p * (a.dim / 2), so);
+            }
+            continue;
+          }
+#pragma unroll
+          for (int e = 0; e < NP; ++e) {
+            const int i0 = HALF ? e : 2 * e, i1 = HALF ? e + a.dim / 2 : 2 * e + 1;
+            const float v0 = to_f32(src[i0]), v1 = to_f32(src[i1]);
+            const bool left = stay >> e & 1u;
+            dst[i0] = from_f32<OT>(left ? v0 : v0 * cs[e] - v1 * sn[e]);
+            dst[i1] = from_f32<OT>(left ? v1 : v0 * sn[e] + v1 * cs[e]);
+          }
+        }
+        return;
+      }
     }
 #pragma unroll
     for (int u = 0; u < HPT; ++u) {

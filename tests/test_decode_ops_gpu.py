@@ -961,3 +961,28 @@ def test_sample_top_p_next_to_a_running_weight(rt, rows, vocab):
     u = torch.full((rows,), 1.0 - 2.0 ** -24, device=DEV)
     t = torch.ones(rows, device=DEV)
     check_sample(compiled(rt, graphs.sample(rows, vocab, top_p=True), "float32")(x, u, t, top_p), x, u, top_p=top_p)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("style", ["half", "interleaved"])
+@pytest.mark.parametrize("dim,sections", [(128, [64]), (128, [16, 24, 24]), (6, [1, 1, 1]), (80, [13, 27])])
+def test_rope_leaves_padding_as_it_is(rt, dim, sections, style, dtype):
+    """Whatever stands in a pair of padding, or past the table, comes out again:
+    infinities and NaN, whose partners they must not reach, and -0."""
+    b, s, h, rows, axes = 2, 9, 5, 20, len(sections)
+    x = torch.randn(b, s, h, dim, generator=gen_of(61), device=DEV)
+    odd = torch.tensor([float("inf"), -float("inf"), float("nan"), -0.0, 0.0], device=DEV)
+    pick = torch.randint(0, 10, x.shape, generator=gen_of(62), device=DEV)
+    x = torch.where(pick < 5, odd[pick.clamp(max=4)], x).to(DT[dtype])
+    cos, sin = tables(rows, dim // 2)
+    pos = torch.randint(-1, 2, (axes, b, s), generator=gen_of(63), device=DEV, dtype=torch.int32)
+    pos[pos == 1] = rows + 3                           # (0: the one that is turned)
+    out = compiled(rt, graphs.rope_positions(b, s, h, dim, rows, sections, dtype=dtype, style=style), dtype)(
+        x, cos, sin, pos)
+    MoltenRuntime.read_status(0)
+    axis = torch.repeat_interleave(torch.arange(axes), torch.tensor(sections)).to(DEV)
+    stays = (pos[axis] != 0).movedim(0, -1)[:, :, None].expand(b, s, h, dim // 2)      # by pair
+    stays = torch.cat((stays, stays), -1) if style == "half" else stays.repeat_interleave(2, -1)
+    bits = {2: torch.int16, 4: torch.int32}[x.element_size()]
+    same = (out.view(bits) == x.view(bits)) | (torch.isnan(out) & torch.isnan(x))
+    assert bool(same[stays].all())
