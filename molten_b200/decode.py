@@ -430,6 +430,9 @@ def _plan_sample(op, sk, tune) -> dict:
     logits = sk.operands[0]
     vocab, rows = logits.shape[-1], prod(logits.shape[:-1])
     _need(rows * 8 < 2 ** 31, "sample: sizes beyond 2^31")
+    for o in sk.operands[2:]:                         # (constants have no shape: infer_shape takes them)
+        _need(o.shape == logits.shape[:-1], f"sample: {op.attrs['params'][o.index - 2]} of shape {o.shape}, expected "
+                                            f"{logits.shape[:-1]} or a constant")
     for pos, value in sk.config["scalars"].items():
         _need(op.attrs["params"][pos - 2] != "top_k" or value == value // 1,
               f"sample: top_k {value} is not a whole number")

@@ -673,3 +673,23 @@ def test_json_attributes_beside_the_type():
             {"type": "OUTPUT", "inputs": [3]}]
     c = config_of(cli.graph_from_json({"name": "a", "ops": ops}), "bfloat16")
     assert c["sections"] == [20, 12] and c["half"] and c["packed"]
+
+
+@pytest.mark.parametrize("name", ["temperature", "top_k", "top_p", "min_p"])
+def test_sample_parameters_are_vectors_or_constants(name):
+    """A tensor of no dimension holds one number, not one a row."""
+    g = DataflowGraph("sample")
+    x, u = g.add_input("x", TS([4, 100]), dtype="float32"), g.add_input("u", TS([4]), dtype="float32")
+    p = g.add_input(name, TS([]), dtype="int32" if name == "top_k" else "float32")
+    g.add_output(g.sample(x, u, **{name: p}))
+    refused(g, f"{name} of shape", "float32")
+
+
+def test_sample_parameters_of_a_call_are_vectors(unbuilt):
+    import torch
+    ck = unbuilt.compile(compile_graph(graphs.sample(4, 100), dtype="float32")[0])
+    good = [torch.empty(s, device="meta") for s in ((4, 100), (4,), (4,))]
+    ck._spec_for(good)
+    for shape in ((), (1,), (5,), (4, 1)):
+        with pytest.raises(LoweringError):
+            ck._spec_for(good[:2] + [torch.empty(shape, device="meta")])
