@@ -757,3 +757,32 @@ def test_a_named_stream_inside_a_capture(rt, call):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(copy, want)
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_outputs_stay_inside_their_memory(rt, call):
+    ck, ins = call(rt, 0)
+    want, guard = ck(*ins).clone(), 2048
+    kept = [t.clone() for t in ins]
+    bits = {2: torch.int16, 4: torch.int32}[want.element_size()]
+    buf = torch.randint(-1000, 1000, (want.numel() + 2 * guard,), generator=gen_of(71), device=DEV, dtype=bits)
+    before = buf.clone()
+    out = buf[guard:-guard].view(want.dtype).view(want.shape)
+    ck(*ins, out=out)
+    assert torch.equal(out, want)
+    assert torch.equal(buf[:guard], before[:guard]) and torch.equal(buf[-guard:], before[-guard:])
+    assert all(torch.equal(a, b) for a, b in zip(ins, kept))
+
+
+@pytest.mark.parametrize("d", [8, 24, 72, 104])
+@pytest.mark.parametrize("new,heads,kv", [(1, 5, 1), (3, 6, 2), (60, 7, 1), (130, 6, 2)])
+def test_odd_head_dims_stay_inside_their_memory(rt, d, new, heads, kv):
+    b, cache = 2, 150
+    q, k, v = attention_inputs(b, new, cache, heads, kv, d, "bfloat16", d)
+    n = torch.tensor([150, 131], dtype=torch.int32, device=DEV)
+    ck = window_kernel(rt, b, new, cache, heads, kv, d, 40, 2, "bfloat16")
+    buf = torch.full((q.numel() + 4096,), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = buf[2048:-2048].view(q.shape)
+    ck(q, k, v, n, out=out)
+    check_attention(out, q, k, v, n, 40, 2, "bfloat16", half_step("bfloat16"))
+    assert bool((buf[:2048] == 7.0).all()) and bool((buf[-2048:] == 7.0).all())
