@@ -137,18 +137,21 @@ def plan_group(graph: DataflowGraph, group_op_ids, input_shapes: dict,
             sub.config["planes"] = planes
         kernels.append(sub)
 
+    # the graph by places instead of op ids, so that equal groups share a kernel;
+    # attributes as they were given: other shapes are planned from them
+    every = inputs + [i for i in ext if i not in inputs] + ordered
+    place = {i: n for n, i in enumerate(every)}
+    key = repr(([place[o] for o in outs], len(inputs),
+                [(graph.ops[o].op_type.name, [place[i] for i in graph.ops[o].inputs], graph.ops[o].attrs)
+                 for o in every[len(inputs):]],
+                [([place[i] for i in sk.op_ids], sk.config) for sk in kernels if sk.family == "model"]))
     return GroupPlan(
         name=name, inputs=inputs,
         input_dtypes=[dts[i] for i in inputs],
         input_shapes=[known[i] for i in inputs],
         outputs=list(outs), output_dtypes=[dts[o] for o in outs],
         output_shapes=[shapes[o] for o in outs],
-        kernels=kernels, temps=temps,
-        # (attributes as they were given: other shapes are planned from them)
-        key=repr((inputs, outs,
-                  [(o, graph.ops[o].op_type.name, graph.ops[o].inputs, graph.ops[o].attrs)
-                   for o in ordered + [i for i in ext if i not in inputs]],
-                  [(sk.op_ids, sk.config) for sk in kernels if sk.family == "model"])))
+        kernels=kernels, temps=temps, key=key)
 
 
 SPLIT3_BLOCK = 256

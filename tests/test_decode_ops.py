@@ -693,3 +693,24 @@ def test_sample_parameters_of_a_call_are_vectors(unbuilt):
     for shape in ((), (1,), (5,), (4, 1)):
         with pytest.raises(LoweringError):
             ck._spec_for(good[:2] + [torch.empty(shape, device="meta")])
+
+
+@pytest.mark.parametrize("kind", ["window_attention", "rms_norm"])
+def test_equal_layers_share_a_kernel(kind, unbuilt):
+    """Groups that differ in their op numbers alone, as the layers of a model."""
+    def kernel(before):
+        g = DataflowGraph("layer")
+        for n in range(before):                        # (used by nothing: later numbers)
+            g.add_input(f"other{n}", TS([4, 64]), dtype="bfloat16")
+        if kind == "window_attention":
+            ids = [g.add_input(n, TS([1, 4, 2, 64]), dtype="bfloat16") for n in "qkv"]
+            y = g.window_attention(*ids, window=3)
+        else:
+            y = g.rms_norm(g.add_input("x", TS([4, 512]), dtype="bfloat16"),
+                           g.add_input("w", TS([512]), dtype="bfloat16"), "norm")
+        g.add_output(y)
+        (k,) = compile_graph(g, dtype="bfloat16")
+        return k
+    a, b = kernel(0), kernel(3)
+    assert a.source == b.source and a.plan.inputs != b.plan.inputs
+    assert unbuilt.compile(a) is unbuilt.compile(b)
